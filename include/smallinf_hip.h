@@ -563,6 +563,172 @@ int32_t sipa_rope(void* x, int64_t x_stride, const void* cos, const void* sin, i
 int32_t sipa_silu_mul(const void* gate_up, int64_t gu_stride, void* out, int64_t out_stride, int32_t T, int32_t I,
                       void* stream);
 
+/*
+ * A forward over drafted trees (speculative decoding; no counterpart in the reference, which decodes one token at a time).
+ * Sequence s has start_s cached tokens and counts[s] drafted nodes behind them, node i in the slot of position
+ * start_s + i. parents[t] is the index of the node's parent within its sequence, smaller than its own, or -1; a node sees
+ * the cached tokens, its ancestors and itself, and stands at position start_s + (number of its ancestors).
+ *
+ * sipa_tree_maps: the forward's metadata from the lengths, in one launch and with nothing read by the host:
+ *   query_starts [S + 1]: exclusive sums of counts (negative counts are taken as 0; the sums end at num_tokens);
+ *   for every node t: positions, slots (table[p / B] * B + p % B at its cache position p), slot_blocks, slot_offsets
+ *   and its ancestors and itself as bits, node a in bit a % 64 of ancestors[t * words + a / 64];
+ *   for every sequence: context_lens (start + count), last_rows (query_starts[s + 1] - 1) and block_tables
+ *   [s, :out_width], its first ceil(context / B) table entries, then -1.
+ * tables, rows and starts are as for sipa_paged_metadata. Rows of the outputs past the last sequence's nodes (num_tokens
+ * may be a capacity) are left as they are. A parent that is not smaller than its node ends the node's chain, as -1 does;
+ * nodes past 64 words have no bit. num_seqs <= 8192.
+ */
+typedef struct sipa_tree_maps_params {
+  int32_t struct_size; /* sizeof(sipa_tree_maps_params) */
+  int32_t num_seqs, num_tokens, block_size, out_width, words;
+  int32_t table_rows, table_width;
+  int64_t table_stride;
+  const int32_t* tables;  /* [table_rows, table_width] */
+  const int32_t* rows;    /* [S] */
+  const int32_t* starts;  /* [S] */
+  const int32_t* counts;  /* [S] */
+  const int32_t* parents; /* [num_tokens] */
+  int64_t* positions;     /* [num_tokens], like the next three */
+  int64_t* slots;
+  int64_t* slot_blocks;
+  int64_t* slot_offsets;
+  int64_t* last_rows;     /* [S] */
+  int32_t* query_starts;  /* [S + 1] */
+  int32_t* context_lens;  /* [S] */
+  int32_t* block_tables;  /* [S, out_width] */
+  uint64_t* ancestors;    /* [num_tokens, words] */
+} sipa_tree_maps_params;
+
+int32_t sipa_tree_maps(const sipa_tree_maps_params* p, void* stream);
+
+/*
+ * sipa_commit_tokens: after a tree's verification, the accepted nodes' K and V move to the positions they now have, in
+ * every layer: for i = 0 .. num_accepted[s] - 1, position starts[s] + i takes the rows of position starts[s] +
+ * accepted[s, i]. accepted rows are node indices in ascending order (a root-to-leaf path is), so that no row is
+ * overwritten before it is read; other orders give unspecified contents of the rows that are moved to. Pools
+ * [L, Hkv, N, B, row bytes]; rows of row_bytes (a multiple of 16) at strides in bytes, and where k_scale is given
+ * per-token fp16 scales [L, Hkv, N, B] with them. Indices are clamped to the tables and the pool.
+ */
+typedef struct sipa_commit_params {
+  int32_t struct_size; /* sizeof(sipa_commit_params) */
+  int32_t num_layers, num_kv_heads, num_blocks, block_size, row_bytes;
+  int32_t num_seqs, max_accepted, bt_width;
+  void* k_pool;
+  void* v_pool;
+  int64_t k_stride_l, k_stride_h, v_stride_l, v_stride_h; /* bytes; blocks and rows contiguous */
+  void* k_scale; /* NULL, or fp16 */
+  void* v_scale;
+  int64_t ks_stride_l, ks_stride_h, vs_stride_l, vs_stride_h; /* elements */
+  const int32_t* block_tables; /* [S, bt_width] */
+  int64_t bt_stride_s;
+  const int32_t* starts;       /* [S] */
+  const int32_t* accepted;     /* [S, max_accepted] */
+  int64_t acc_stride_s;
+  const int32_t* num_accepted; /* [S] */
+} sipa_commit_params;
+
+int32_t sipa_commit_tokens(const sipa_commit_params* p, void* stream);
+
+/*
+ * Rules on a forward's logits before a token is taken from them (the reference's engine takes the argmax of the raw logits;
+ * no counterpart). For row r of sequence s and token v, with l = logits[r, v] in fp32:
+ *   made = times v occurs among the sequence's generated tokens (history[prompt_lens[s] ..]) and on the row's path, the
+ *          tokens of the nodes in its mask; seen = made > 0 or v occurs in the prompt (history[.. prompt_lens[s] - 1])
+ *   l = l > 0 ? l / repetition[s] : l * repetition[s]        where seen
+ *   l = l - frequency[s] * made - presence[s]                where made > 0
+ *   l = l + the sum of the values that the sequence's bias list gives v, added up in the list's order
+ *   l = -inf                                                 where the row has a grammar state whose bit v is 0
+ * rounded once to the logits' type. out may be logits itself. Rows belong to sequences by query_starts [S + 1] (row r to
+ * the sequence with query_starts[s] <= r < query_starts[s + 1]), or row r to sequence r where it is NULL. Rows behind the
+ * last sequence's are copied as they are. Tokens outside [0, vocab) in the lists, and -1 as padding, are ignored. NULL
+ * pointers leave their rule out: history (all three penalties then see the path alone), prompt_lens (0), repetition (1),
+ * frequency, presence (0), tokens and masks (no path), bias_starts, grammar_rows. A grammar row outside [0, states) leaves
+ * its row free.
+ */
+typedef struct sipa_logits_params {
+  int32_t struct_size; /* sizeof(sipa_logits_params) */
+  int32_t num_rows, vocab, num_seqs;
+  int32_t dtype;       /* SIPA_F32, SIPA_BF16 or SIPA_F16: logits and out */
+  int32_t words;       /* of a mask: 1 .. 4 */
+  const void* logits;  /* [num_rows, vocab], last dim contiguous */
+  int64_t logits_stride;
+  void* out;
+  int64_t out_stride;
+  const int32_t* query_starts;   /* [S + 1] or NULL */
+  const int32_t* history;        /* all sequences' tokens, one after the other */
+  const int64_t* history_starts; /* [S + 1] */
+  const int32_t* prompt_lens;    /* [S] */
+  const float* repetition;       /* [S], positive */
+  const float* frequency;        /* [S] */
+  const float* presence;         /* [S] */
+  const int64_t* tokens;         /* [num_rows] the rows' own tokens */
+  const uint64_t* masks;         /* [num_rows, words] */
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  const int32_t* bias_starts;    /* [S + 1] */
+  const uint32_t* grammar;       /* [states, grammar_stride]: bit v % 32 of word v / 32 allows token v */
+  int64_t grammar_stride;        /* words, at least ceil(vocab / 32) */
+  int32_t grammar_states;
+  const int32_t* grammar_rows;   /* [num_rows] state of each row, -1 for none */
+} sipa_logits_params;
+
+int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream);
+
+/*
+ * Attention of drafted trees over the paged cache, with the nodes' own K and V already in their slots:
+ *   out[t, h*G + g, :] = sum_j softmax_j(scale * q[t, h*G + g, :] . k_j) v_j over the keys j that row t sees: the positions
+ *   below start_s = context_lens[s] - n_s, and start_s + a for every bit a < n_s of its mask (see sipa_tree_maps),
+ * n_s = query_starts[s + 1] - query_starts[s] rows from row query_starts[s] on. A row that sees no key gets zeros; rows
+ * behind the last sequence's are left as they are. K and V in hidden places may hold anything, infinities and NaN too.
+ * bf16 q and out; pools bf16 (SIPA_KV_PLAIN) or int8 with per-token scales (SIPA_KV_INT8_TOKEN: the codes enter the products
+ * exactly, the scales in fp32). head_dim 64 or 128, blocks of 16, 32 or 64 tokens, any group of query heads up to 64.
+ */
+typedef struct sipa_tree_params {
+  int32_t struct_size; /* sizeof(sipa_tree_params) */
+  int32_t num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
+  int32_t max_context;  /* largest context length, known on the host; context lengths are clamped to it */
+  int32_t max_nodes;    /* largest n_s, at most 64 words; rows past it are left as they are */
+  int32_t words;        /* of a mask: 1 .. 4 */
+  float scale;          /* positive and finite */
+  const void* q;        /* [num_tokens, Hq, D]; last dim contiguous, rows 16-byte aligned */
+  int64_t q_stride_t, q_stride_h;
+  const void* k_cache;  /* [Hkv, N, B, D], each head's blocks contiguous */
+  const void* v_cache;
+  int64_t kv_stride_h, kv_stride_n;
+  const int32_t* block_tables; /* [S, bt_width], bt_width >= ceil(max_context / B); ids are clamped to [0, num_blocks) */
+  int64_t bt_stride_s;
+  int32_t bt_width;
+  const int32_t* context_lens; /* [S] cached tokens and nodes */
+  const int32_t* query_starts; /* [S + 1] */
+  const uint64_t* masks;       /* [num_tokens, words] */
+  void* out;                   /* [num_tokens, Hq, D] */
+  int64_t out_stride_t, out_stride_h;
+  int32_t kv_mode;             /* SIPA_KV_PLAIN or SIPA_KV_INT8_TOKEN */
+  const void* k_scale;         /* [Hkv, N, B], last dim contiguous */
+  int32_t k_scale_dtype;       /* SIPA_F16 or SIPA_F32 */
+  int64_t ks_stride_h, ks_stride_n;
+  const void* v_scale;
+  int32_t v_scale_dtype;
+  int64_t vs_stride_h, vs_stride_n;
+  int32_t num_splits;          /* key splits; <= 0: the library's choice */
+  /* sipa_tree_workspace_bytes() bytes, 256-byte aligned: merge counters, zero before the first call and left at zero by
+     every call, and partial results. Calls that may run at the same time (other streams, graphs replayed side by side) need
+     workspaces of their own. May be NULL where that is 0. */
+  void* workspace;
+  int64_t workspace_bytes;
+} sipa_tree_params;
+
+int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream);
+
+/* Workspace bytes the call needs, 0 for none, or a negative return code; *counter_bytes (may be NULL): the merge counters'
+ * share, at the start. Reads the sizes, kv_mode and num_splits. */
+int64_t sipa_tree_workspace_bytes(const sipa_tree_params* p, int64_t* counter_bytes);
+
+/* The id of the graph capture that `stream` is in, 0 when it is in none: workspaces that a graph keeps the address of belong
+ * to its capture. */
+uint64_t sipa_capture_id(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

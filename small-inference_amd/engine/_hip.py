@@ -107,6 +107,57 @@ class LayerOutParams(ctypes.Structure):
     ]
 
 
+class TreeParams(ctypes.Structure):
+    """Mirror of struct sipa_tree_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_seqs", i32), ("num_tokens", i32), ("num_q_heads", i32), ("num_kv_heads", i32),
+        ("head_dim", i32), ("block_size", i32), ("num_blocks", i32), ("max_context", i32), ("max_nodes", i32),
+        ("words", i32), ("scale", f32),
+        ("q", vp), ("q_stride_t", i64), ("q_stride_h", i64),
+        ("k_cache", vp), ("v_cache", vp), ("kv_stride_h", i64), ("kv_stride_n", i64),
+        ("block_tables", vp), ("bt_stride_s", i64), ("bt_width", i32), ("context_lens", vp), ("query_starts", vp),
+        ("masks", vp), ("out", vp), ("out_stride_t", i64), ("out_stride_h", i64),
+        ("kv_mode", i32), ("k_scale", vp), ("k_scale_dtype", i32), ("ks_stride_h", i64), ("ks_stride_n", i64),
+        ("v_scale", vp), ("v_scale_dtype", i32), ("vs_stride_h", i64), ("vs_stride_n", i64),
+        ("num_splits", i32), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class TreeMapsParams(ctypes.Structure):
+    """Mirror of struct sipa_tree_maps_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_seqs", i32), ("num_tokens", i32), ("block_size", i32), ("out_width", i32),
+        ("words", i32), ("table_rows", i32), ("table_width", i32), ("table_stride", i64),
+        ("tables", vp), ("rows", vp), ("starts", vp), ("counts", vp), ("parents", vp),
+        ("positions", vp), ("slots", vp), ("slot_blocks", vp), ("slot_offsets", vp), ("last_rows", vp),
+        ("query_starts", vp), ("context_lens", vp), ("block_tables", vp), ("ancestors", vp),
+    ]
+
+
+class CommitParams(ctypes.Structure):
+    """Mirror of struct sipa_commit_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_layers", i32), ("num_kv_heads", i32), ("num_blocks", i32), ("block_size", i32),
+        ("row_bytes", i32), ("num_seqs", i32), ("max_accepted", i32), ("bt_width", i32), ("k_pool", vp), ("v_pool", vp),
+        ("k_stride_l", i64), ("k_stride_h", i64), ("v_stride_l", i64), ("v_stride_h", i64),
+        ("k_scale", vp), ("v_scale", vp),
+        ("ks_stride_l", i64), ("ks_stride_h", i64), ("vs_stride_l", i64), ("vs_stride_h", i64),
+        ("block_tables", vp), ("bt_stride_s", i64), ("starts", vp), ("accepted", vp), ("acc_stride_s", i64),
+        ("num_accepted", vp),
+    ]
+
+
+class LogitsParams(ctypes.Structure):
+    """Mirror of struct sipa_logits_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_rows", i32), ("vocab", i32), ("num_seqs", i32), ("dtype", i32), ("words", i32),
+        ("logits", vp), ("logits_stride", i64), ("out", vp), ("out_stride", i64), ("query_starts", vp),
+        ("history", vp), ("history_starts", vp), ("prompt_lens", vp), ("repetition", vp), ("frequency", vp),
+        ("presence", vp), ("tokens", vp), ("masks", vp), ("bias_tokens", vp), ("bias_values", vp), ("bias_starts", vp),
+        ("grammar", vp), ("grammar_stride", i64), ("grammar_states", i32), ("grammar_rows", vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "sipa_abi_version": (i32, []),
@@ -144,6 +195,12 @@ SIGNATURES = {
     "sipa_rms_norm": (i32, [vp, i64, vp, i64, vp, f32, vp, i64, vp, i64, i32, i32, vp]),
     "sipa_rope": (i32, [vp, i64, vp, vp, i32, i32, i32, vp]),
     "sipa_silu_mul": (i32, [vp, i64, vp, i64, i32, i32, vp]),
+    "sipa_adjust_logits": (i32, [_c.POINTER(LogitsParams), vp]),
+    "sipa_tree_attention": (i32, [_c.POINTER(TreeParams), vp]),
+    "sipa_tree_workspace_bytes": (i64, [_c.POINTER(TreeParams), _c.POINTER(i64)]),
+    "sipa_capture_id": (_c.c_uint64, [vp]),
+    "sipa_tree_maps": (i32, [_c.POINTER(TreeMapsParams), vp]),
+    "sipa_commit_tokens": (i32, [_c.POINTER(CommitParams), vp]),
 }
 
 _lib = None
@@ -199,6 +256,24 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_of(t: torch.Tensor) -> int:
     """The current torch stream of t's device, as a hipStream_t value."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())  # current_stream(t.device).cuda_stream, at a tenth of its time
+
+
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Makes `device` the current one around a launch: a stream's kernels are launched from its own device."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def require_gpu(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
