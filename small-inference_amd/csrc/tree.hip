@@ -11,17 +11,20 @@
 //   O^T[16 d x 16 rows] += V^T . P^T
 // INT8 pools: the codes go to LDS as bf16, exactly; the scores are multiplied by K's scales and the probabilities by V's in
 // fp32. Splits write (m, l, O) and the last of a unit's to arrive merges them.
-// P is rounded to bf16 for the second product, as the model's own attention rounds its probabilities (2^-9 of each, which
-// averages out over the keys): V has no more bits, and a second term would double that product.
+// P enters the second product as two bf16 terms, 16 bits of it: one alone gives errors as large as the result's own rounding
+// (2.3e-3 of it in all against 1.7e-3). The second is taken from p (1 + 2^-20), so that it is never zero against an infinite
+// V.
 #include <algorithm>
+#include <type_traits>
 
 #include "decode_common.h"
 
 namespace sipa {
 
-constexpr int kTreeRows = 64;         // rows of a workgroup: 4 waves of 16
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kTreeMaxSplits = 128;
-constexpr int kTreeMaxChunk = 32768;
+constexpr int kTreeMaxChunk = 16384;  // block ids of a split in LDS: 4 KB
 constexpr int kTreeMaxGroup = 64;
 constexpr int kTreeMaxNodes = 256;
 
@@ -46,210 +49,481 @@ struct TreeArgs {
   int32_t S, T, Hkv, G, words, nb, max_ctx, max_nodes;
   int32_t log_b;           // blocks of 1 << log_b tokens
   int32_t groups;          // row groups of the longest sequence
-  int32_t units, nsplit, chunk;
+  int32_t nsplit, chunk;
   float scale_log2;
   int* counters;           // [units]
-  float* pm;               // [units][nsplit][kTreeRows]
-  float* pl;
-  float* part;             // [units][nsplit][kTreeRows][D]
+  float* pm;               // [units][nsplit][rows of a group]
+  float* pl;               // the same
+  uint16_t* part;          // [units][nsplit][rows of a group][D] fp16
 };
 
-__device__ __forceinline__ float tree_scale(const void* base, bool f32, int64_t i) {
-  return f32 ? ((const float*)base)[i] : f16_bits_to_f32(((const uint16_t*)base)[i]);
+// A scale as it lies in memory, and its value: apart, so that the load is waited for only where the value is needed.
+__device__ __forceinline__ uint32_t scale_bits(const void* base, bool f32, int64_t i) {
+  return f32 ? ((const uint32_t*)base)[i] : (uint32_t)((const uint16_t*)base)[i];
 }
 
-template <int D, int MODE>
-__global__ void __launch_bounds__(256) tree_attention_kernel(const TreeArgs a) {
-  constexpr int KT = 32, P = D + 16, KS = D / 32, DT = D / 16;
-  constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, LPT = (KT * CPK + 255) / 256;  // 16-byte parts of a tile
-  __shared__ __align__(16) uint16_t sk[KT * P];
-  __shared__ __align__(16) uint16_t sv[KT * P];
-  __shared__ float sks[KT], svs[KT];
-  __shared__ int last_flag;
+__device__ __forceinline__ float scale_value(uint32_t bits, bool f32) {
+  return f32 ? __uint_as_float(bits) : f16_bits_to_f32(bits);
+}
 
-  const int u = (int)blockIdx.x % a.units, sp = (int)blockIdx.x / a.units;
-  const int rg = u % a.groups, s = u / a.groups % a.S, h = u / a.groups / a.S;
-  const int row0 = a.qs[s], n = min(min(a.qs[s + 1] - row0, a.max_nodes), a.T - row0);
-  const int G = a.G, M = n * G, m0 = rg * kTreeRows;
+// Eight int8 codes (two words) as bf16, exactly.
+__device__ __forceinline__ u32x4 tree_codes(uint32_t w0, uint32_t w1) {
+  u32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? w0 : w1;
+    const int b = 16 * (i & 1);
+    x[i] = pack_bf16x2((float)(int8_t)(w >> b), (float)(int8_t)(w >> (b + 8)));
+  }
+  return x;
+}
+
+// MR row tiles of 16 per wave, RW waves side by side over the rows, KW waves one after the other over the keys, each KPW
+// keys of a stage of KW KPW; NPRE stages in flight in registers.
+template <int D, int MODE, int MR, int RW, int KW, int KPW, int NPRE>
+__global__ void __launch_bounds__(64 * RW * KW, D == 64 && MODE == 0 && KPW == 32 ? 4 : 2) tree_attention_kernel(const TreeArgs a) {
+  constexpr int KT = KW * KPW, MT = KPW / 16, HT = KPW / 32, P = D + 16, KS = D / 32, DT = D / 16;
+  constexpr int PT = 64 * RW * KW, ROWS = 16 * MR * RW;
+  constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, NCH = KT * CPK;  // 16-byte parts of a key, of a stage
+  constexpr int LPT = (NCH + PT - 1) / PT, SPT = MODE == 0 ? 0 : (2 * KT + PT - 1) / PT;
+  constexpr int TE = KT * P;
+  __shared__ __align__(16) uint16_t sm[2][2][TE];  // [buffer][K, V][key][P]
+  __shared__ __align__(16) float sscale[MODE == 0 ? 1 : 2][2][MODE == 0 ? 4 : KT];  // [buffer][K, V][key]
+  __shared__ int bids[kTreeMaxChunk / 16];
+  __shared__ uint64_t masks[ROWS * 4];  // [node of the group][word]
+  __shared__ int last_flag, dirty;
+
+  // Workgroup L is dealt to XCD L % 8: a pair's row groups and splits share one, so that its L2 serves the groups the same
+  // keys and the merge its partials.
+  const int L = blockIdx.x, per = a.nsplit * a.groups;
+  const int pair = (L & 7) + 8 * ((L >> 3) / per), in = (L >> 3) % per;
+  if (pair >= a.S * a.Hkv) return;  // the grid is padded to whole groups of 8 pairs
+  const int sp = in / a.groups, rg = in % a.groups, s = pair % a.S, h = pair / a.S;
+  const int u = pair * a.groups + rg;
+  const int row0 = a.qs[s], all = a.qs[s + 1] - row0, n = min(min(all, a.max_nodes), a.T - row0);
+  const int G = a.G, M = n * G, m0 = rg * ROWS;
   if (n <= 0 || row0 < 0 || m0 >= M) return;
-  const int ctx = min(a.ctx[s], a.max_ctx), start = ctx - (a.qs[s + 1] - row0);
+  const int ctx = min(a.ctx[s], a.max_ctx), start = ctx - all;
   const int nvalid = max(1, (ctx + a.chunk - 1) / a.chunk);
   if (sp >= nvalid) return;
   const int k_lo = sp * a.chunk, k_hi = min(k_lo + a.chunk, ctx);
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW;
+  // odd key waves take the rows in reverse: a last row tile that is missing then costs each SIMD alike
+  const int rw = kw & 1 ? RW - 1 - wave % RW : wave % RW;
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
-  const int m = m0 + 16 * wave + r;
-  const bool valid = m < M;
-  const int node = (valid ? m : M - 1) / G, g = (valid ? m : M - 1) - node * G;
-  bf16x8 qop[KS];
+  const int nkeys = max(k_hi - k_lo, 0), first_col = k_lo >> a.log_b;
+  const int32_t* table = a.bt + (int64_t)s * a.bt_ss;
+  for (int i = tid; i << a.log_b < nkeys; i += PT) bids[i] = min(max(table[min(first_col + i, a.bt_w - 1)], 0), a.nb - 1);
+
+  const int node0 = m0 / G, nodes = min((m0 + ROWS - 1) / G, n - 1) - node0 + 1;  // the group's nodes, at most ROWS
+  for (int i = tid; i < nodes * a.words; i += PT) masks[i] = a.masks[(int64_t)(row0 + node0) * a.words + i];
+  if (tid == 0) dirty = 0;
+  int node[MR], head[MR];
+  bool tile_valid[MR];  // wave-uniform
+  bf16x8 qop[MR][KS];
 #pragma unroll
-  for (int j = 0; j < KS; ++j)
-    qop[j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(a.q + (int64_t)(row0 + node) * a.q_st +
-                                                        (int64_t)(h * G + g) * a.q_sh + 32 * j + 8 * q4));
-  const uint64_t* mask = a.masks + (int64_t)(row0 + node) * a.words;
-  float m_run = kNegInf, l_run = 0.f;
-  f32x4 acc[DT];
+  for (int c = 0; c < MR; ++c) {
+    const int m = m0 + 16 * (MR * rw + c) + r, at = min(m, M - 1);
+    tile_valid[c] = m0 + 16 * (MR * rw + c) < M;
+    node[c] = at / G;
+    head[c] = at - node[c] * G;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < KS; ++j)
+      qop[c][j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(a.q + (int64_t)(row0 + node[c]) * a.q_st +
+                                                             (int64_t)(h * G + head[c]) * a.q_sh + 32 * j + 8 * q4));
+  }
+  constexpr float kSlack = 8.f, kFastRange = 16.f;
+  const float inv_scale_log2 = MODE == 0 ? 1.f / a.scale_log2 : 1.f;
+  float m_run[MR], m_off[MR], fast_thr[MR];  // m_off: m_run, or 0 while that is -inf
+  f32x4 l_run[MR];  // MODE 0: an accumulator whose every row holds the sum; MODE 1: a lane's own four sums
+  f32x4 acc[MR][DT];
+#pragma unroll
+  for (int c = 0; c < MR; ++c) {
+    m_run[c] = fast_thr[c] = kNegInf, m_off[c] = 0.f, l_run[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int tr_off = tr16_offset(r, q4, P);
+  bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
+  asm volatile("" : "+v"(ones));  // kept in registers
+  __syncthreads();  // block ids
 
-  for (int t0 = k_lo; t0 < k_hi; t0 += KT) {
-    __syncthreads();  // the tile before this one is done with
+  const int ntiles = (nkeys + KT - 1) / KT;
+  u32x4 rk[NPRE][LPT], rv[NPRE][LPT];
+  uint32_t rs[NPRE][SPT ? SPT : 1];
+  // A thread's parts of a stage keep their place in their blocks from stage to stage (a stage is whole blocks): what changes
+  // is the block id. Keys past the split's end are read too, inside its last block; they are hidden, and cleaned below.
+  const int es = MODE == 0 ? 2 : 1, last_id = max((nkeys - 1) >> a.log_b, 0);
+  const uint32_t kv_bytes = (uint32_t)a.kv_sn * es;  // of a block (host-checked)
+  const uint8_t* kbase[LPT];
+  const uint8_t* vbase[LPT];
+  int part_id[LPT];
+#pragma unroll
+  for (int i = 0; i < LPT; ++i) {
+    const int c = tid + PT * i, key = c / CPK;
+    const int64_t e = ((int64_t)h * a.kv_sh + (key & ((1 << a.log_b) - 1)) * D + CH * (c % CPK)) * es;
+    kbase[i] = (const uint8_t*)a.k + e;
+    vbase[i] = (const uint8_t*)a.v + e;
+    part_id[i] = key >> a.log_b;
+  }
+  auto gload = [&](int set, int t) {
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
-      const int c = tid + 256 * i;
-      if (c >= KT * CPK) break;
-      const int key = c / CPK, d0 = CH * (c % CPK), pos = min(t0 + key, k_hi - 1);
-      const int64_t blk = min(max(a.bt[(int64_t)s * a.bt_ss + min(pos >> a.log_b, a.bt_w - 1)], 0), a.nb - 1);
-      const int off = pos & ((1 << a.log_b) - 1);
-      const int64_t e = (int64_t)h * a.kv_sh + blk * a.kv_sn + (int64_t)off * D + d0;
+      if (NCH % PT != 0 && tid + PT * i >= NCH) break;
+      const uint64_t at = (uint64_t)(uint32_t)bids[min((KT * t >> a.log_b) + part_id[i], last_id)] * kv_bytes;
+      rk[set][i] = *(const u32x4*)(kbase[i] + at);
+      rv[set][i] = *(const u32x4*)(vbase[i] + at);
+    }
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      const int c = tid + PT * i;
+      if (2 * KT % PT != 0 && c >= 2 * KT) break;
+      const int key = c % KT, off = key & ((1 << a.log_b) - 1);
+      const int64_t blk = bids[min((KT * t >> a.log_b) + (key >> a.log_b), last_id)];
+      rs[set][i] = c < KT ? scale_bits(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + blk * a.ks_sn + off)
+                          : scale_bits(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + blk * a.vs_sn + off);
+    }
+  };
+  // Infinities and NaN among the nodes' V: a row that does not see them must not take 0 * V into its sums. They go to LDS
+  // as zeros, and the rows that see them take them up at the end.
+  auto cleaned = [&](u32x4 v, int key) {
+    if (key < start) return v;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t keep = ((v[w] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((v[w] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+      if (keep != 0xffffffffu && key < k_hi) dirty = 1;
+      v[w] &= keep;
+    }
+    return v;
+  };
+  auto sstore = [&](int set, int t) {
+    const int buf = t & 1;
+    const bool check = k_lo + KT * (t + 1) > start;  // uniform: some key of the stage is a node
+#pragma unroll
+    for (int i = 0; i < LPT; ++i) {
+      const int c = tid + PT * i;
+      if (NCH % PT != 0 && c >= NCH) break;
+      const int e = (c / CPK) * P + CH * (c % CPK);
       if constexpr (MODE == 0) {
-        *(u32x4*)(sk + key * P + d0) = *(const u32x4*)((const uint16_t*)a.k + e);
-        *(u32x4*)(sv + key * P + d0) = *(const u32x4*)((const uint16_t*)a.v + e);
+        *(u32x4*)(&sm[buf][0][e]) = rk[set][i];
+        *(u32x4*)(&sm[buf][1][e]) = check ? cleaned(rv[set][i], k_lo + KT * t + c / CPK) : rv[set][i];
       } else {
-        const u32x4 k = *(const u32x4*)((const int8_t*)a.k + e), v = *(const u32x4*)((const int8_t*)a.v + e);
+        *(u32x4*)(&sm[buf][0][e]) = tree_codes(rk[set][i][0], rk[set][i][1]);
+        *(u32x4*)(&sm[buf][0][e + 8]) = tree_codes(rk[set][i][2], rk[set][i][3]);
+        *(u32x4*)(&sm[buf][1][e]) = tree_codes(rv[set][i][0], rv[set][i][1]);
+        *(u32x4*)(&sm[buf][1][e + 8]) = tree_codes(rv[set][i][2], rv[set][i][3]);
+      }
+    }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+    for (int i = 0; i < SPT; ++i) {
+      const int c = tid + PT * i;
+      if (2 * KT % PT != 0 && c >= 2 * KT) break;
+      sscale[buf][c / KT][c % KT] = c < KT ? scale_value(rs[set][i], a.ks_f32) * a.scale_log2 : scale_value(rs[set][i], a.vs_f32);
+    }
+  };
+  // Which of the keys x0 .. x0 + KPW - 1 the row of a node sees, key x0 + b in bit b.
+  auto sees = [&](int nd, int x0) {
+    const int rel = x0 - start, shift = rel & 63;
+    auto word = [&](int w) {
+      const uint64_t x = masks[(nd - node0) * a.words + min(max(w, 0), a.words - 1)];
+      return w < 0 ? ~0ull : w < a.words ? x : 0ull;
+    };
+    uint64_t bits = word(rel >> 6) >> shift;
+    if (shift) bits |= word((rel >> 6) + 1) << (64 - shift);
+    return k_hi - x0 >= 64 ? bits : bits & ((1ull << (k_hi - x0)) - 1);
+  };
+  auto tile = [&](int t) {
+    const int x0 = k_lo + KT * t + KPW * kw;  // the wave's first key
+    if (x0 >= k_hi || !tile_valid[0]) return;  // wave-uniform
+    const int buf = t & 1;
+    const uint16_t* sk = sm[buf][0] + KPW * kw * P;
+    const uint16_t* sv = sm[buf][1] + KPW * kw * P;
+    const bool masked = x0 + KPW > min(start, k_hi);  // some key is a node, or past the split's end
+    bf16x8 kop[MT][KS];
 #pragma unroll
-          for (int b = 0; b < 4; b += 2) {
-            *(uint32_t*)(sk + key * P + d0 + 4 * w + b) =
-                pack_bf16x2((float)(int8_t)(k[w] >> (8 * b)), (float)(int8_t)(k[w] >> (8 * b + 8)));
-            *(uint32_t*)(sv + key * P + d0 + 4 * w + b) =
-                pack_bf16x2((float)(int8_t)(v[w] >> (8 * b)), (float)(int8_t)(v[w] >> (8 * b + 8)));
-          }
-        if (d0 == 0) {
-          sks[key] = tree_scale(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + blk * a.ks_sn + off);
-          svs[key] = tree_scale(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + blk * a.vs_sn + off);
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < KS; ++j) kop[mt][j] = *(const bf16x8*)(sk + (16 * mt + r) * P + 32 * j + 8 * q4);
+    u32x4 hi[MR][HT], lo[MR][HT];  // bf16 pairs
+#pragma unroll
+    for (int c = 0; c < MR; ++c) {
+      f32x4 sc[MT];  // row (mt, q4, i) holds key 16 mt + 4 q4 + i
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[mt][j], qop[c][j], sc[mt], 0, 0, 0);
+        if constexpr (MODE == 1) sc[mt] *= *(const f32x4*)(sscale[buf][0] + KPW * kw + 16 * mt + 4 * q4);  // log2 units
+      }
+      if (masked) {
+        const uint64_t bits = sees(node[c], x0) >> (4 * q4);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(bits >> (16 * mt + i) & 1)) sc[mt][i] = kNegInf;
+      }
+      // Each lane's largest score. The row's max (two cross-lane steps more) is looked at only when some score exceeds the
+      // running one by more than 2^kFastRange, and raised only past 2^kSlack: p stays far inside fp32 otherwise.
+      float mx = sc[0][0];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = vmax(mx, sc[mt][i]);
+      if (__builtin_amdgcn_ballot_w64(mx > fast_thr[c])) {
+        mx = max_over_rows_swap(mx) * (MODE == 0 ? a.scale_log2 : 1.f);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[c] + kSlack)) {
+          const float m_new = fmaxf(m_run[c], mx);
+          const float alpha = fast_exp2(m_run[c] - (m_new == kNegInf ? 0.f : m_new));  // 0 while the row has seen no key
+          l_run[c] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) acc[c][dt] *= alpha;
+          m_run[c] = m_new;
+          m_off[c] = m_new == kNegInf ? 0.f : m_new;
+          fast_thr[c] = (m_new + kFastRange) * inv_scale_log2;
         }
+      }
+#pragma unroll
+      for (int hf = 0; hf < HT; ++hf) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = sc[2 * hf + (i >> 2)][i & 3];
+          p[i] = fast_exp2(MODE == 0 ? fmaf(x, a.scale_log2, -m_off[c]) : x - m_off[c]);
+        }
+        if constexpr (MODE == 1) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const f32x4 vs = *(const f32x4*)(sscale[buf][1] + KPW * kw + 32 * hf + 4 * i + 4 * q4);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) l_run[c][x] += p[i + x];
+            if (masked) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) p[i + x] = p[i + x] == 0.f ? 0.f : p[i + x] * vs[x];  // a hidden scale may be anything
+            } else {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) p[i + x] *= vs[x];
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          uint32_t cut[2];
+          float rest[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            cut[x] = __float_as_uint(p[i + x]) & 0xffff0000u;
+            rest[x] = fmaf(p[i + x], 1.f + 0x1p-20f, -__uint_as_float(cut[x]));
+          }
+          hi[c][hf][i >> 1] = __builtin_amdgcn_perm(cut[1], cut[0], 0x07060302u);
+          lo[c][hf][i >> 1] = pack_bf16x2(rest[0], rest[1]);
+        }
+        if constexpr (MODE == 0) {  // the sums on the matrix cores, of the values that the product uses
+          l_run[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, hi[c][hf]), l_run[c], 0, 0, 0);
+          l_run[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, lo[c][hf]), l_run[c], 0, 0, 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < HT; ++hf)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const bf16x8 vop = read_v_operand<bf16x8>(sv + 32 * P * hf, tr_off, P, 16 * dt);
+#pragma unroll
+        for (int c = 0; c < MR; ++c) {
+          acc[c][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, hi[c][hf]), acc[c][dt], 0, 0, 0);
+          acc[c][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, lo[c][hf]), acc[c][dt], 0, 0, 0);
+        }
+      }
+  };
+  if (ntiles > 0) {
+#pragma unroll
+    for (int k = 0; k < NPRE; ++k) {
+      gload(k, k);
+      asm volatile("" ::: "memory");  // in this order
+    }
+    sstore(0, 0);
+    __syncthreads();
+    // register set k % NPRE carries stage k to its LDS store; loads past the last stage read its last key again, so that
+    // every wait is for a fixed count, and stages past it compute nothing
+    for (int tb = 0; tb < ntiles; tb += NPRE) {
+#pragma unroll
+      for (int k = 0; k < NPRE; ++k) {
+        const int t = tb + k;
+        gload(k, t + NPRE);
+        tile(t);
+        sstore((k + 1) % NPRE, t + 1);  // that buffer was last read before the last barrier
+        __syncthreads();
+      }
+    }
+  }
+  float l[MR];
+#pragma unroll
+  for (int c = 0; c < MR; ++c) {
+    l[c] = MODE == 0 ? l_run[c][0] : sum_over_rows_swap(l_run[c][0] + l_run[c][1] + l_run[c][2] + l_run[c][3]);
+    if (l[c] != l[c]) m_run[c] = 0.f;  // NaN scores never raise the max: the merges see the row by its sum
+  }
+  if constexpr (KW > 1) {
+    // The key waves' states join in LDS (the tile buffers are free after the last barrier): waves kw > 0 leave theirs,
+    // wave kw = 0 of the same rows takes them up one after the other.
+    constexpr int XS = DT * 4 + 4;  // floats of a lane: O, m, l
+    static_assert((KW - 1) * RW * MR * 64 * XS * 4 <= (int)sizeof(sm), "the states fit the tile buffers");
+    float* xs = (float*)&sm[0][0][0];
+    if (kw > 0) {
+#pragma unroll
+      for (int c = 0; c < MR; ++c) {
+        float* x = xs + ((((kw - 1) * RW + rw) * MR + c) * 64 + lane) * XS;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *(f32x4*)(x + 4 * dt) = acc[c][dt];
+        x[4 * DT] = m_run[c];
+        x[4 * DT + 1] = l[c];
       }
     }
     __syncthreads();
-    float sc[8];  // keys 16 (i / 4) + 4 q4 + i % 4 of the tile
+    if (kw == 0) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 1; k < KW; ++k)
 #pragma unroll
-      for (int j = 0; j < KS; ++j)
-        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(sk + (16 * mt + r) * P + 32 * j + 8 * q4), qop[j],
-                                                    x, 0, 0, 0);
+        for (int c = 0; c < MR; ++c) {
+          const float* x = xs + ((((k - 1) * RW + rw) * MR + c) * 64 + lane) * XS;
+          const float m1 = x[4 * DT], l1 = x[4 * DT + 1];
+          const float top = vmax(m_run[c], m1);
+          if (top == kNegInf) continue;
+          const float f0 = fast_exp2(m_run[c] - top), f1 = fast_exp2(m1 - top);
+          l[c] = f0 * l[c] + f1 * l1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[4 * mt + i] = MODE == 0 ? x[i] : x[i] * sks[16 * mt + 4 * q4 + i];
-    }
-    const bool masked = t0 + KT > min(start, k_hi);  // some key of the tile is a node, or past the split's end
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = t0 + 16 * (i >> 2) + 4 * q4 + (i & 3), rel = key - start;
-        bool sees = key < k_hi;
-        if (rel >= 0) sees = sees && rel < 64 * a.words && (mask[rel >> 6] >> (rel & 63) & 1);
-        if (!sees) sc[i] = kNegInf;
-      }
-    }
-    float mx = sc[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) mx = vmax(mx, sc[i]);
-    mx = max_over_rows_swap(mx) * a.scale_log2;
-    const float m_new = vmax(m_run, mx), base = m_new == kNegInf ? 0.f : m_new;
-    const float alpha = fast_exp2(m_run - base);  // 0 while the row has seen no key
-    m_run = m_new;
-    l_run *= alpha;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-    bf16x8 pop;
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = fast_exp2(fmaf(sc[i], a.scale_log2, -base));
-      l_run += p[i];
-      if constexpr (MODE == 1) {
-        const float scaled = p[i] * svs[16 * (i >> 2) + 4 * q4 + (i & 3)];
-        p[i] = masked && p[i] == 0.f ? 0.f : scaled;  // a hidden key's scale may be anything
-      }
-      pop[i] = (__bf16)p[i];
-    }
-    // Infinities and NaN among the nodes' V: rows that do not see them must not take 0 * V into their sums.
-    bool plain = true;
-    if (MODE == 0 && masked) {
-      bool bad = false;
-      for (int c = lane; c < KT * D / 2; c += 64) {
-        const uint32_t w = *(const uint32_t*)(sv + (2 * c / D) * P + 2 * c % D);
-        bad = bad || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-      }
-      plain = __builtin_amdgcn_ballot_w64(bad) == 0;
-    }
-    if (plain) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_v_operand<bf16x8>(sv, tr_off, P, 16 * dt), pop, acc[dt], 0,
-                                                          0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        for (int from = 0; from < 4; ++from) {  // lane group `from` holds the probability of this key
-          const float pk = __shfl((float)pop[i], 16 * from + r);
-          const uint16_t* v = sv + (16 * (i >> 2) + 4 * from + (i & 3)) * P;
-          if (pk != 0.f)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[dt][e] += pk * bf16_bits_to_f32(v[16 * dt + 4 * q4 + e]);
+          for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f0 * acc[c][dt] + f1 * *(const f32x4*)(x + 4 * dt);
+          m_run[c] = top;
         }
     }
   }
-  const float l = sum_over_rows_swap(l_run);
-  if (nvalid == 1) {
-    if (!valid) return;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros
-    uint16_t* o = a.out + (int64_t)(row0 + node) * a.o_st + (int64_t)(h * G + g) * a.o_sh + 4 * q4;
+  const bool owner = kw == 0;
+  if (MODE == 0 && dirty && owner) {  // (set before the loop's last barrier)
+    for (int key = max(start, k_lo); key < k_hi; ++key) {
+      const uint16_t* v = (const uint16_t*)a.v + (int64_t)h * a.kv_sh + (int64_t)bids[(key >> a.log_b) - first_col] * a.kv_sn +
+                          (int64_t)(key & ((1 << a.log_b) - 1)) * D + 4 * q4;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      uint32_t* w = (uint32_t*)(o + 16 * dt);
-      w[0] = pack_bf16x2(acc[dt][0] * inv, acc[dt][1] * inv);
-      w[1] = pack_bf16x2(acc[dt][2] * inv, acc[dt][3] * inv);
+      for (int c = 0; c < MR; ++c) {
+        const bool on = sees(node[c], key) & 1;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = bf16_bits_to_f32(v[16 * dt + i]);
+            if (on && !(fabsf(x) < __builtin_huge_valf())) acc[c][dt][i] += x;
+          }
+      }
+    }
+  }
+  if (nvalid == 1) {
+    if (!owner) return;
+#pragma unroll
+    for (int c = 0; c < MR; ++c) {
+      if (m0 + 16 * (MR * rw + c) + r >= M) continue;
+      const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];  // no key: zeros
+      uint16_t* o = a.out + (int64_t)(row0 + node[c]) * a.o_st + (int64_t)(h * G + head[c]) * a.o_sh + 4 * q4;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *(u32x2*)(o + 16 * dt) = u32x2{pack_bf16x2(acc[c][dt][0] * inv, acc[c][dt][1] * inv),
+                                       pack_bf16x2(acc[c][dt][2] * inv, acc[c][dt][3] * inv)};
     }
     return;
   }
-  const int64_t base = ((int64_t)u * a.nsplit + sp) * kTreeRows;
-  const int slot = 16 * wave + r;
-  const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
-      a.part + (int64_t)u * a.nsplit * kTreeRows * D, (short)0, a.nsplit * kTreeRows * D * 4, 0x00020000);
-  if (valid) {
+  // The split's state: m and l of each row, and its own output O / l as fp16 (the weighted mean of its V rows: 2^-12 of it),
+  // half the bytes of fp32 sums. A row whose largest |O / l| reaches 2^15 is stored times 2^-e, e in l's low mantissa bits.
+  const int64_t first = (int64_t)u * a.nsplit * ROWS;
+  const int split_bytes = ROWS * D * 2;
+  const __amdgpu_buffer_rsrc_t rows =
+      __builtin_amdgcn_make_buffer_rsrc(a.part + first * D, (short)0, a.nsplit * split_bytes, 0x00020000);
+  if (owner) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[dt]), rows,
-                                             ((sp * kTreeRows + slot) * D + 16 * dt + 4 * q4) * 4, 0, kAuxSc1);
-    if (q4 == 0) {
-      store_coherent(a.pm + base + slot, m_run);
-      store_coherent(a.pl + base + slot, l);
+    for (int c = 0; c < MR; ++c) {
+      const int slot = 16 * (MR * rw + c) + r;
+      if (m0 + slot >= M) continue;
+      const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
+      float big = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big = vmax(big, fabsf(acc[c][dt][i]));
+      big = max_over_rows_swap(big * inv);
+      const int e = big < 32768.f ? 0 : max(__builtin_amdgcn_frexp_expf(big) - 15, 0);  // inf and NaN: 0
+      const float inv_e = __builtin_amdgcn_ldexpf(inv, -e);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            u32x2{pack_f16x2(acc[c][dt][0] * inv_e, acc[c][dt][1] * inv_e),
+                  pack_f16x2(acc[c][dt][2] * inv_e, acc[c][dt][3] * inv_e)},
+            rows, sp * split_bytes + (slot * D + 16 * dt + 4 * q4) * 2, 0, kAuxSc1);
+      if (q4 == 0) {
+        store_coherent(a.pm + first + sp * ROWS + slot, m_run[c]);
+        store_coherent(a.pl + first + sp * ROWS + slot,
+                       __uint_as_float((__float_as_uint(l[c]) & ~0xffu) | (uint32_t)e));
+      }
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (tid == 0)
-    last_flag = __hip_atomic_fetch_add(a.counters + u, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nvalid - 1;
+  if (tid == 0) {
+    // +2^16 from a workgroup that is not on the pair's XCD: the last to arrive then reads through memory, else from its L2
+    uint32_t xcc;
+    asm volatile("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
+    const int away = (int)(xcc & 0xf) != (L & 7);
+    const int prev = __hip_atomic_fetch_add(a.counters + u, 1 + (away << 16), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last_flag = (prev & 0xffff) == nvalid - 1 ? 1 + ((prev >> 16) + away == 0) : 0;
+  }
   __syncthreads();
   if (!last_flag) return;
-  const int64_t first = (int64_t)u * a.nsplit * kTreeRows;
-  for (int i = tid; i < kTreeRows * (D / 4); i += 256) {
-    const int row = i / (D / 4), c = i % (D / 4);
-    if (m0 + row >= M) break;
-    float top = kNegInf, den = 0.f;
-    f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < nvalid; ++j) {
-      const float mj = load_coherent(a.pm + first + j * kTreeRows + row), lj = load_coherent(a.pl + first + j * kTreeRows + row);
-      const f32x4 oj = __builtin_bit_cast(
-          f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, ((j * kTreeRows + row) * D + 4 * c) * 4, 0, kAuxSc1));
-      if (mj == kNegInf && lj == 0.f) continue;  // the row sees no key of this split
-      const float up = vmax(top, mj), f = fast_exp2(top - up), w = fast_exp2(mj - up);
-      den = den * f + lj * w;
-      num = num * f + oj * w;
-      top = up;
+  const __amdgpu_buffer_rsrc_t mrows =
+      __builtin_amdgcn_make_buffer_rsrc(a.pm + first, (short)0, a.nsplit * ROWS * 4, 0x00020000);
+  const __amdgpu_buffer_rsrc_t lrows =
+      __builtin_amdgcn_make_buffer_rsrc(a.pl + first, (short)0, a.nsplit * ROWS * 4, 0x00020000);
+  // Every split's m and l first, in LDS, then each thread 8 channels of a row with kMerge splits' loads in flight.
+  float* lm = (float*)&sm[0][0][0];  // [nvalid][ROWS] m, then l
+  uint32_t* ll = (uint32_t*)(lm + nvalid * ROWS);
+  auto merge = [&](auto tag) {
+    constexpr int AUX = decltype(tag)::value, kMerge = 8;
+    for (int i = tid; i < nvalid * ROWS; i += PT) {
+      lm[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mrows, i * 4, 0, AUX));
+      ll[i] = __builtin_amdgcn_raw_buffer_load_b32(lrows, i * 4, 0, AUX);
     }
-    const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
-    const int nd = (m0 + row) / G, hd = (m0 + row) - nd * G;
-    uint32_t* w = (uint32_t*)(a.out + (int64_t)(row0 + nd) * a.o_st + (int64_t)(h * G + hd) * a.o_sh + 4 * c);
-    w[0] = pack_bf16x2(num[0] * inv, num[1] * inv);
-    w[1] = pack_bf16x2(num[2] * inv, num[3] * inv);
+    __syncthreads();
+    for (int i = tid; i < ROWS * (D / 8); i += PT) {
+      const int slot = i / (D / 8), ch = 8 * (i % (D / 8));
+      if (m0 + slot >= M) break;
+      float top = kNegInf, den = 0.f;
+      for (int j = 0; j < nvalid; ++j) top = fmaxf(top, lm[j * ROWS + slot]);
+      f32x4 num[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int j0 = 0; j0 < nvalid; j0 += kMerge) {
+        u32x4 o[kMerge];
+#pragma unroll
+        for (int x = 0; x < kMerge; ++x)
+          o[x] = __builtin_amdgcn_raw_buffer_load_b128(rows, min(j0 + x, nvalid - 1) * split_bytes + (slot * D + ch) * 2, 0, AUX);
+#pragma unroll
+        for (int x = 0; x < kMerge; ++x) {
+          const int j = min(j0 + x, nvalid - 1);
+          const uint32_t lb = ll[j * ROWS + slot];
+          const float w = j0 + x >= nvalid || top == kNegInf ? 0.f : fast_exp2(lm[j * ROWS + slot] - top) * __uint_as_float(lb & ~0xffu);
+          if (w == 0.f) continue;  // a split without a key for the row
+          den += w;
+          const float wo = __builtin_amdgcn_ldexpf(w, (int)(lb & 0xffu));
+#pragma unroll
+          for (int y = 0; y < 8; ++y) num[y >> 2][y & 3] += wo * f16_bits_to_f32(y & 1 ? o[x][y >> 1] >> 16 : o[x][y >> 1] & 0xffffu);
+        }
+      }
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      const int nd = (m0 + slot) / G, hd = (m0 + slot) - nd * G;
+      *(u32x4*)(a.out + (int64_t)(row0 + nd) * a.o_st + (int64_t)(h * G + hd) * a.o_sh + ch) =
+          u32x4{pack_bf16x2(num[0][0] * inv, num[0][1] * inv), pack_bf16x2(num[0][2] * inv, num[0][3] * inv),
+                pack_bf16x2(num[1][0] * inv, num[1][1] * inv), pack_bf16x2(num[1][2] * inv, num[1][3] * inv)};
+    }
+  };
+  if (last_flag == 2) {
+    asm volatile("buffer_inv sc0" ::: "memory");  // sc0 loads may hit the CU's L1: drop any earlier copy first
+    merge(std::integral_constant<int, kAuxSc0>());
+  } else {
+    merge(std::integral_constant<int, kAuxSc1>());
   }
   if (tid == 0) __hip_atomic_store(a.counters + u, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -259,6 +533,7 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(const TreeArgs a) {
 using namespace sipa;
 
 struct TreeLayout {
+  int variant, rows;  // index into the launch table below, rows of a workgroup
   int groups, units, nsplit, chunk;
   int64_t pm, pl, part, total;  // byte offsets into the workspace; counters first
 };
@@ -284,10 +559,22 @@ static int tree_check(const sipa_tree_params* p) {
   return SIPA_OK;
 }
 
-// About two workgroups per CU, splits of at least 256 keys.
+struct TreeVariant {
+  int mr, rw, kw, kpw;
+};
+constexpr TreeVariant kTreeVariants[] = {{1, 4, 2, 64}, {1, 8, 1, 64}};  // up to 64 rows, more
+
+// Bytes of the kernel's tile buffers, which the merge's m and l have to fit.
+static int tree_tile_bytes(const TreeVariant& v, int D) { return 2 * 2 * v.kw * v.kpw * (D + 16) * 2; }
+
+// About one workgroup per CU, splits of at least 256 keys.
 static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   const int G = p->num_q_heads / p->num_kv_heads;
-  l->groups = (p->max_nodes * G + kTreeRows - 1) / kTreeRows;
+  const int need = p->max_nodes * G;
+  l->variant = need <= 64 ? 0 : 1;
+  const TreeVariant& v = kTreeVariants[l->variant];
+  l->rows = 16 * v.mr * v.rw;
+  l->groups = (need + l->rows - 1) / l->rows;
   const int64_t units = (int64_t)p->num_seqs * p->num_kv_heads * l->groups;
   SIPA_CHECK(units <= 0x7fffffff / kTreeMaxSplits, SIPA_EINVAL, "%lld units exceed the grid limit", (long long)units);
   l->units = (int)units;
@@ -295,21 +582,22 @@ static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   if (splits <= 0) {
     const int cus = sipa_device_cu_count(-1);
     if (cus < 0) return cus;
-    splits = std::min<int64_t>((2 * cus + units - 1) / std::max<int64_t>(units, 1), (p->max_context + 255) / 256);
+    splits = std::min<int64_t>((cus + units - 1) / std::max<int64_t>(units, 1), (p->max_context + 255) / 256);
   }
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, kTreeMaxSplits));
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, std::min<int64_t>(kTreeMaxSplits, tree_tile_bytes(v, p->head_dim) / (8 * l->rows))));
   const int chunk = (int)((p->max_context + splits - 1) / splits);
-  l->chunk = std::min((chunk + 63) / 64 * 64, kTreeMaxChunk);
+  const int kt = v.kw * v.kpw;  // whole stages
+  l->chunk = std::min((chunk + kt - 1) / kt * kt, kTreeMaxChunk);
   l->nsplit = (p->max_context + l->chunk - 1) / l->chunk;
   l->pm = l->pl = l->part = l->total = 0;
   if (l->nsplit > 1) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t rows = units * l->nsplit * kTreeRows;
-    SIPA_CHECK((int64_t)l->nsplit * kTreeRows * p->head_dim * 4 <= 0x7fffffff, SIPA_EINVAL, "split state too large");
+    const int64_t rows = units * l->nsplit * l->rows;
+    SIPA_CHECK((int64_t)l->nsplit * l->rows * p->head_dim * 2 <= 0x7fffffff, SIPA_EINVAL, "split state too large");
     l->pm = up(units * 4);
     l->pl = l->pm + up(rows * 4);
     l->part = l->pl + up(rows * 4);
-    l->total = l->part + up(rows * p->head_dim * 4);
+    l->total = l->part + up(rows * p->head_dim * 2);
   }
   return SIPA_OK;
 }
@@ -336,6 +624,18 @@ extern "C" uint64_t sipa_capture_id(void* stream) {
   return status == hipStreamCaptureStatusNone ? 0 : (uint64_t)id;
 }
 
+template <int D, int MODE, int V>
+static void launch_variant(dim3 grid, hipStream_t st, const TreeArgs& a) {
+  constexpr TreeVariant v = kTreeVariants[V];
+  hipLaunchKernelGGL((tree_attention_kernel<D, MODE, v.mr, v.rw, v.kw, v.kpw, D == 64 ? 4 : 3>), grid, dim3(64 * v.rw * v.kw), 0, st, a);
+}
+
+template <int D, int MODE>
+static void launch_tree(int variant, dim3 grid, hipStream_t st, const TreeArgs& a) {
+  if (variant == 0) launch_variant<D, MODE, 0>(grid, st, a);
+  else launch_variant<D, MODE, 1>(grid, st, a);
+}
+
 extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) {
   int rc = tree_check(p);
   if (rc != SIPA_OK) return rc;
@@ -354,6 +654,8 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   const int per16 = int8 ? 16 : 8;
   SIPA_CHECK((((uintptr_t)p->k_cache | (uintptr_t)p->v_cache) & 15) == 0 && p->kv_stride_h % per16 == 0 &&
                  p->kv_stride_n % per16 == 0, SIPA_EINVAL, "K/V pools must be 16-byte aligned");
+  SIPA_CHECK(p->kv_stride_n >= 0 && p->kv_stride_n <= 0x7fffffff, SIPA_EUNSUPPORTED, "blocks %lld elements apart",
+             (long long)p->kv_stride_n);
   if (int8) {
     SIPA_CHECK(p->k_scale && p->v_scale, SIPA_EINVAL, "INT8 pools need k_scale and v_scale");
     SIPA_CHECK((p->k_scale_dtype == SIPA_F16 || p->k_scale_dtype == SIPA_F32) &&
@@ -405,7 +707,6 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   a.max_nodes = p->max_nodes;
   a.log_b = p->block_size == 16 ? 4 : p->block_size == 32 ? 5 : 6;
   a.groups = l.groups;
-  a.units = l.units;
   a.nsplit = l.nsplit;
   a.chunk = l.chunk;
   a.scale_log2 = p->scale * 1.4426950408889634f;
@@ -413,15 +714,16 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   a.counters = (int*)ws;
   a.pm = (float*)(ws + l.pm);
   a.pl = (float*)(ws + l.pl);
-  a.part = (float*)(ws + l.part);
-  const dim3 grid((unsigned)((int64_t)l.units * l.nsplit));
+  a.part = (uint16_t*)(ws + l.part);
+  const int64_t pairs8 = ((int64_t)p->num_seqs * p->num_kv_heads + 7) / 8 * 8;
+  const dim3 grid((unsigned)(pairs8 * l.groups * l.nsplit));
   hipStream_t st = (hipStream_t)stream;
   if (p->head_dim == 64) {
-    if (int8) hipLaunchKernelGGL((tree_attention_kernel<64, 1>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((tree_attention_kernel<64, 0>), grid, dim3(256), 0, st, a);
+    if (int8) launch_tree<64, 1>(l.variant, grid, st, a);
+    else launch_tree<64, 0>(l.variant, grid, st, a);
   } else {
-    if (int8) hipLaunchKernelGGL((tree_attention_kernel<128, 1>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((tree_attention_kernel<128, 0>), grid, dim3(256), 0, st, a);
+    if (int8) launch_tree<128, 1>(l.variant, grid, st, a);
+    else launch_tree<128, 0>(l.variant, grid, st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(SIPA_EHIP, "tree attention launch failed: %s", hipGetErrorString(e));
