@@ -199,8 +199,8 @@ SIGNATURES = {
     "sipa_tree_attention": (i32, [_c.POINTER(TreeParams), vp]),
     "sipa_tree_workspace_bytes": (i64, [_c.POINTER(TreeParams), _c.POINTER(i64)]),
     "sipa_capture_id": (_c.c_uint64, [vp]),
-    "sipa_tree_maps": (i32, [_c.POINTER(TreeMapsParams), vp]),
-    "sipa_commit_tokens": (i32, [_c.POINTER(CommitParams), vp]),
+    "sipa_tree_maps": (i32, [vp, vp]),  # a packed or ctypes TreeMapsParams
+    "sipa_commit_tokens": (i32, [vp, vp]),  # a packed or ctypes CommitParams
 }
 
 _lib = None

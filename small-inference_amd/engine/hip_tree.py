@@ -14,6 +14,7 @@ row's sequence in bit a % 64 of word a // 64.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -44,8 +45,17 @@ def mask_words(max_nodes: int) -> int:
     return -(-max_nodes // 64)
 
 
+_I32, _I64 = torch.int32, torch.int64
+_split = torch.split_with_sizes
+# sipa_tree_maps_params and sipa_commit_params as bytes (native alignment): a third of the time that filling a ctypes
+# structure takes, in calls whose kernels take a few microseconds
+_MAPS = struct.Struct("8iq14Q")
+_COMMIT = struct.Struct("9i2Q4q2Q4qQq2QqQ")
+assert _MAPS.size == ctypes.sizeof(_hip.TreeMapsParams) and _COMMIT.size == ctypes.sizeof(_hip.CommitParams)
+
+
 def _vector(t: torch.Tensor, n: int, what: str) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 vector of {n}")
 
 
@@ -61,30 +71,36 @@ def tree_maps(tables: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, co
     """
     S, T, words = counts.shape[0], parents.shape[0], mask_words(max_nodes)
     _vector(rows, S, "rows"), _vector(starts, S, "starts"), _vector(counts, S, "counts"), _vector(parents, T, "parents")
-    if tables.dtype is not torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
+    table_rows, columns = tables.shape
+    table_stride, last = tables.stride()
+    if tables.dtype is not _I32 or last != 1:
         raise ValueError("tables must be int32 [rows, columns] with contiguous rows")
     if S < 1 or T < 1 or block_size < 1 or width < 1:
         raise ValueError(f"{S} sequences, {T} nodes, block size {block_size}, width {width}")
     _hip.require_gpu(tables, rows, starts, counts, parents)
     dev = tables.device
     if out is None:
-        d64 = torch.empty(T * (4 + words) + S, dtype=torch.int64, device=dev)
-        d32 = torch.empty(S * (width + 2) + 1, dtype=torch.int32, device=dev)
-        pos, slots, blocks, offs, last, masks = d64.split([T, T, T, T, S, T * words])
-        qs, ctx, bt = d32.split([S + 1, S, S * width])
-        out = TreeMaps(pos, slots, blocks, offs, last, qs, ctx, bt.view(S, width), masks.view(T, words))
+        d64 = torch.empty(T * (4 + words) + S, dtype=_I64, device=dev)
+        d32 = torch.empty(S * (width + 2) + 1, dtype=_I32, device=dev)
+        pos, slots, blocks, offs, last_rows, masks = _split(d64, (T, T, T, T, S, T * words))
+        qs, ctx, bt = _split(d32, (S + 1, S, S * width))
+        out = TreeMaps(pos, slots, blocks, offs, last_rows, qs, ctx, bt.view(S, width), masks.view(T, words))
+        p64, p32 = d64.data_ptr(), d32.data_ptr()
+        at = (p64, p64 + 8 * T, p64 + 16 * T, p64 + 24 * T, p64 + 32 * T, p32, p32 + 4 * (S + 1), p32 + 4 * (2 * S + 1),
+              p64 + 32 * T + 8 * S)
     else:
         shapes = ((T,), (T,), (T,), (T,), (S,), (S + 1,), (S,), (S, width), (T, words))
         for i, (t, shape) in enumerate(zip(out, shapes)):
-            if t.shape != shape or t.dtype is not (torch.int32 if 5 <= i <= 7 else torch.int64) or not t.is_contiguous():
+            if t.shape != shape or t.dtype is not (_I32 if 5 <= i <= 7 else _I64) or not t.is_contiguous():
                 raise ValueError(f"out.{TreeMaps._fields[i]} must be contiguous {shape}, as a call of these sizes returns")
         _hip.require_gpu(tables, *out)
-    a = [t.data_ptr() for t in out]
-    p = _hip.TreeMapsParams(ctypes.sizeof(_hip.TreeMapsParams), S, T, block_size, width, words, tables.shape[0],
-                            tables.shape[1], tables.stride(0), tables.data_ptr(), rows.data_ptr(), starts.data_ptr(),
-                            counts.data_ptr(), parents.data_ptr(), *a)
+        at = tuple(t.data_ptr() for t in out)
+    p = _MAPS.pack(_MAPS.size, S, T, block_size, width, words, table_rows, columns, table_stride, tables.data_ptr(),
+                   rows.data_ptr(), starts.data_ptr(), counts.data_ptr(), parents.data_ptr(), *at)
     with _hip.on_device(dev):
-        _hip.check(_hip.lib().sipa_tree_maps(ctypes.byref(p), _hip.stream_of(tables)), "tree_maps")
+        rc = _hip.lib().sipa_tree_maps(p, _hip.stream_of(tables))
+    if rc:
+        _hip.check(rc, "tree_maps")
     return out
 
 
@@ -100,34 +116,42 @@ def commit_tokens(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
     """
     L, H, N, B, D = k.shape
     S, A = accepted.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
+    if v.shape != k.shape or v.dtype is not k.dtype:
         raise ValueError("K and V pools must have one shape and dtype")
-    if not (_hip.layers_contiguous(k) and _hip.layers_contiguous(v)):
+    block = B * D
+    ks, vs = k.stride(), v.stride()
+    if L < 1 or ks[1:] != (N * block, block, D, 1) or vs[1:] != ks[1:]:
         raise ValueError("each layer of the pools must be contiguous")
+    kss = vss = (0, 0)
+    ksp = vsp = 0
     if (k_scale is None) != (v_scale is None) or (k_scale is None) == (k.dtype is torch.int8):
         raise ValueError("INT8 pools, and only they, have scales of K and V")
     if k_scale is not None:
-        for t in (k_scale, v_scale):
-            if t.shape != k.shape[:4] or t.dtype is not torch.float16 or not _hip.layers_contiguous(t):
-                raise ValueError(f"scales must be fp16 {tuple(k.shape[:4])}, each layer contiguous")
+        kss, vss = k_scale.stride(), v_scale.stride()
+        if k_scale.shape != (L, H, N, B) or v_scale.shape != (L, H, N, B) or k_scale.dtype is not torch.float16 or \
+                v_scale.dtype is not torch.float16 or kss[1:] != (N * B, B, 1) or vss[1:] != kss[1:]:
+            raise ValueError(f"scales must be fp16 {(L, H, N, B)}, each layer contiguous")
+        ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
     _vector(starts, S, "starts"), _vector(num_accepted, S, "num_accepted")
-    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < S or \
-            block_tables.stride(1) != 1 or block_tables.shape[1] < 1:
+    rows, width = block_tables.shape
+    bt_stride, last = block_tables.stride()
+    if block_tables.dtype is not _I32 or rows < S or last != 1 or width < 1:
         raise ValueError(f"block_tables must be int32 with {S} rows")
-    if accepted.dtype is not torch.int32 or (A > 1 and accepted.stride(1) != 1):
+    acc_stride, last = accepted.stride()
+    if accepted.dtype is not _I32 or (A > 1 and last != 1):
         raise ValueError("accepted must be int32 [S, A] with contiguous rows")
     _hip.require_gpu(k, v, block_tables, starts, accepted, num_accepted, k_scale, v_scale)
     if S == 0 or A == 0:
         return
     size = k.element_size()
-    ks, vs = ((k_scale.stride(), v_scale.stride()) if k_scale is not None else ((0, 0), (0, 0)))
-    p = _hip.CommitParams(ctypes.sizeof(_hip.CommitParams), L, H, N, B, D * size, S, A, block_tables.shape[1],
-                          k.data_ptr(), v.data_ptr(), k.stride(0) * size, k.stride(1) * size, v.stride(0) * size,
-                          v.stride(1) * size, _hip.ptr(k_scale), _hip.ptr(v_scale), ks[0], ks[1], vs[0], vs[1],
-                          block_tables.data_ptr(), block_tables.stride(0), starts.data_ptr(), accepted.data_ptr(),
-                          accepted.stride(0), num_accepted.data_ptr())
+    p = _COMMIT.pack(_COMMIT.size, L, H, N, B, D * size, S, A, width, k.data_ptr(), v.data_ptr(), ks[0] * size,
+                     ks[1] * size, vs[0] * size, vs[1] * size, ksp, vsp, kss[0], kss[1], vss[0], vss[1],
+                     block_tables.data_ptr(), bt_stride, starts.data_ptr(), accepted.data_ptr(), acc_stride,
+                     num_accepted.data_ptr())
     with _hip.on_device(k.device):
-        _hip.check(_hip.lib().sipa_commit_tokens(ctypes.byref(p), _hip.stream_of(k)), "commit_tokens")
+        rc = _hip.lib().sipa_commit_tokens(p, _hip.stream_of(k))
+    if rc:
+        _hip.check(rc, "commit_tokens")
 
 
 def tree_supported(q_dtype: torch.dtype, pool_dtype: torch.dtype, block_size: int, head_dim: int, group: int) -> bool:
