@@ -12,15 +12,17 @@ import torch
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_pos: torch.Tensor, k_pos: torch.Tensor,
-              scale: float) -> torch.Tensor:
-    """Causal GQA attention for one sequence; see the module docstring."""
+              scale: float, hidden: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention for one sequence; see the module docstring. hidden [T, S]: which keys each query does not see,
+    in place of the positions' order (drafted trees; every query sees itself)."""
     T, Hq, d = q.shape
     Hkv = k.shape[0]
     g = Hq // Hkv
     qg = q.reshape(T, Hkv, g, d).permute(1, 2, 0, 3).reshape(Hkv, g * T, d)
     scores = torch.bmm(qg, k.transpose(1, 2).contiguous()) * scale  # [Hkv, g*T, S]
-    if T > 1:  # one query is always the newest token and sees every key
+    if hidden is None and T > 1:  # one query is always the newest token and sees every key
         hidden = k_pos[None, :] > q_pos[:, None]  # [T, S]
+    if hidden is not None:
         scores = scores.view(Hkv, g, T, -1).masked_fill(hidden, float("-inf")).view(Hkv, g * T, -1)
     probs = torch.softmax(scores, dim=-1, dtype=torch.promote_types(q.dtype, torch.float32)).to(q.dtype)
     out = torch.bmm(probs, v.contiguous())  # [Hkv, g*T, d]

@@ -159,13 +159,22 @@ class BlockManager:
         """Extend seq_id by one token and return its slot."""
         return self.append_slots(seq_id, 1)[0]
 
-    def free(self, seq_id: int) -> None:
-        """Release seq_id; a block returns to the stack when its reference count reaches 0."""
-        table = self._tables.pop(seq_id)
-        del self._lengths[seq_id]
-        self._arrays.pop(seq_id, None)
+    def truncate(self, seq_id: int, n_tokens: int) -> None:
+        """Keep the first n_tokens of seq_id (drafted tokens that were not accepted are given up); the blocks past them
+        return to the stack, last block first, and free listeners hear of them. Not for an int8-kchannel cache, which cannot
+        take a quantized block back in part. No counterpart in the reference."""
+        if not 0 <= n_tokens <= self._lengths[seq_id]:
+            raise ValueError(f"sequence {seq_id} holds {self._lengths[seq_id]} tokens, {n_tokens} to keep")
+        table, keep = self._tables[seq_id], self.blocks_for(n_tokens)
+        self._lengths[seq_id] = n_tokens
+        released = table[keep:][::-1]
+        del table[keep:]
+        self._release(released)
+
+    def _release(self, blocks: list[int]) -> None:
+        """One holder fewer for each block; those without any go back to the stack, in the order given."""
         released = []
-        for b in table[::-1]:  # last block first, so the stack hands the blocks out again in table order
+        for b in blocks:
             self._ref[b] -= 1
             if self._ref[b] < 0:
                 raise AssertionError(f"block {b} released more often than it was taken")
@@ -174,6 +183,13 @@ class BlockManager:
                 released.append(b)
         for fn in self._free_listeners:
             fn(released)
+
+    def free(self, seq_id: int) -> None:
+        """Release seq_id; a block returns to the stack when its reference count reaches 0."""
+        table = self._tables.pop(seq_id)
+        del self._lengths[seq_id]
+        self._arrays.pop(seq_id, None)
+        self._release(table[::-1])  # last block first, so the stack hands the blocks out again in table order
         for fn in self._table_listeners:
             fn(seq_id, -1)
 

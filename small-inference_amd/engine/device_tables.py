@@ -19,7 +19,8 @@ import torch
 
 from . import _hip
 from .block_manager import BlockManager
-from .paged_cache import PagedMetadata, PerSequence
+from .hip_tree import tree_maps
+from .paged_cache import PagedMetadata, PerSequence, TreeMetadata, check_trees
 
 
 class _LazyList(Sequence):
@@ -103,9 +104,8 @@ class DeviceBlockTables:
         both = torch.from_numpy(np.stack([np.concatenate(flat), np.concatenate(vals)])).to(self.device)
         self.table.view(-1)[both[0]] = both[1].to(torch.int32)
 
-    def build(self, batch: list[tuple[int, int, int]]) -> PagedMetadata:
-        """Metadata for a forward over batch = [(seq_id, start, n), ...], with build_metadata's contents and
-        errors (reference engine/paged_cache.py:55-90), derived on the device."""
+    def _check(self, batch: list[tuple[int, int, int]]) -> tuple:
+        """(sequence ids, starts, counts, contexts) of a forward's batch, with build_metadata's errors."""
         S = len(batch)
         if S == 0:
             raise ValueError("a forward needs at least one sequence")
@@ -127,6 +127,52 @@ class DeviceBlockTables:
             i = int(np.argmax(ctx))
             raise ValueError(f"sequence {seqs[i]}: context {ctx[i]} exceeds the device tables' "
                              f"{self.max_blocks * B} tokens")
+        return seqs, starts, counts, ctx
+
+    def build_tree(self, batch: list[tuple[int, int, list[int]]]) -> TreeMetadata:
+        """Metadata for a forward over drafted trees, batch = [(seq_id, start, parents)], with build_tree_metadata's contents
+        and errors, derived on the device from one upload of lengths and parents (hip_tree.tree_maps)."""
+        lens = check_trees(batch)
+        S, B = len(batch), self.manager.block_size
+        seqs, starts, counts, ctx = self._check(lens)
+        self.sync()
+        rows = np.fromiter((self._row_of[s] for s in seqs), dtype=np.int64, count=S)
+        flat = np.concatenate([rows, starts, counts, *(np.asarray(p, dtype=np.int64) for _, _, p in batch)])
+        d = torch.from_numpy(flat.astype(np.int32)).to(self.device)
+        T, width = int(counts.sum()), int(-(-ctx.max() // B))
+        maps = tree_maps(self.table, d[:S], d[S:2 * S], d[2 * S:3 * S], d[3 * S:], B, width, int(counts.max()))
+        qs = [0, *np.cumsum(counts).tolist()]
+        return TreeMetadata(
+            num_tokens=T, query_starts=qs, context_lens=ctx.tolist(), positions=maps.positions, slot_mapping=maps.slots,
+            slot_blocks=maps.slot_blocks, slot_offsets=maps.slot_offsets, block_tables=maps.block_tables,
+            context_lens_t=maps.context_lens, last_token_indices=maps.last_rows,
+            **self._host_side(seqs, starts, counts, ctx), parents=[list(p) for _, _, p in batch], masks=maps.masks,
+            query_starts_t=maps.query_starts)
+
+    def _host_side(self, seqs: list[int], starts: np.ndarray, counts: np.ndarray, ctx: np.ndarray) -> dict:
+        """The metadata's fields that live on the host, made on access."""
+        m, B, S = self.manager, self.manager.block_size, len(seqs)
+        tables = [m.table_array(s) for s in seqs]  # views, valid for this forward
+        nbs = (-(-ctx // B)).tolist()
+
+        def slot_list() -> list[int]:
+            out: list[int] = []
+            for t, st, n in zip(tables, starts.tolist(), counts.tolist()):
+                pos = np.arange(st, st + n, dtype=np.int64)
+                out.extend((t[pos // B].astype(np.int64) * B + pos % B).tolist())
+            return out
+
+        return dict(
+            slots_cpu=_LazyList(int(counts.sum()), slot_list),
+            block_ids=PerSequence(S, lambda i: torch.from_numpy(tables[i][:nbs[i]].astype(np.int64)).to(self.device)),
+            block_ids_cpu=PerSequence(S, lambda i: tables[i][:nbs[i]].tolist()))
+
+    def build(self, batch: list[tuple[int, int, int]]) -> PagedMetadata:
+        """Metadata for a forward over batch = [(seq_id, start, n), ...], with build_metadata's contents and
+        errors (reference engine/paged_cache.py:55-90), derived on the device."""
+        S = len(batch)
+        m, B = self.manager, self.manager.block_size
+        seqs, starts, counts, ctx = self._check(batch)
         self.sync()
         rows = np.fromiter((self._row_of[s] for s in seqs), dtype=np.int64, count=S)
         qs = np.zeros(S + 1, dtype=np.int64)
@@ -141,27 +187,15 @@ class DeviceBlockTables:
             p(self.table), self.table.stride(0), self.max_seqs, self.max_blocks, p(info), S, T, B, width,
             p(d64), p(d64[T:]), p(d64[2 * T:]), p(d64[3 * T:]), p(d64[4 * T:]), p(d32), p(d32[S * width:]),
             _hip.stream_of(d64)), "paged metadata")
-        tables = [m.table_array(s) for s in seqs]  # views, valid for this forward
-        nbs = (-(-ctx // B)).tolist()
-
-        def slot_list() -> list[int]:
-            out: list[int] = []
-            for t, st, n in zip(tables, starts.tolist(), counts.tolist()):
-                pos = np.arange(st, st + n, dtype=np.int64)
-                out.extend((t[pos // B].astype(np.int64) * B + pos % B).tolist())
-            return out
-
         return PagedMetadata(
             num_tokens=T,
             query_starts=qs.tolist(),
             context_lens=ctx.tolist(),
             positions=d64[:T],
-            slots_cpu=_LazyList(T, slot_list),
             slot_mapping=d64[T:2 * T],
             slot_blocks=d64[2 * T:3 * T],
             slot_offsets=d64[3 * T:4 * T],
-            block_ids=PerSequence(S, lambda i: torch.from_numpy(tables[i][:nbs[i]].astype(np.int64)).to(self.device)),
-            block_ids_cpu=PerSequence(S, lambda i: tables[i][:nbs[i]].tolist()),
+            **self._host_side(seqs, starts, counts, ctx),
             block_tables=d32[:S * width].view(S, width),
             context_lens_t=d32[S * width:],
             last_token_indices=d64[4 * T:],

@@ -31,6 +31,7 @@ from . import _hip
 from .block_manager import BlockManager
 from .device_tables import DeviceBlockTables
 from .hip_decode import decode_workspace_bytes, reserve_workspace
+from .hip_logits import LogitsRules
 from .paged_cache import PagedKVCache, PagedMetadata, PerSequence
 
 SCRATCH_SEQ = -(1 << 40)  # the runner's own sequence id in the block manager: the padding rows' block
@@ -209,10 +210,12 @@ class DecodeGraphRunner:
             raise RuntimeError("the captured decode used a split workspace the runner did not reserve")
         self._graphs[bucket] = (g, logits, ws)
 
-    def step(self, seq_ids: list[int], input_ids: torch.Tensor, graph: bool = True) -> torch.Tensor:
+    def step(self, seq_ids: list[int], input_ids: torch.Tensor, graph: bool = True, rules: LogitsRules | None = None,
+             grammar_rows: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [len(seq_ids), vocab] of one decode step: row i is sequence seq_ids[i]'s newest token
         (input_ids[i], at position manager.seq_len(s) - 1; the caller has appended its slot). graph=False runs the
-        same static-shape step eagerly (the graph's reference)."""
+        same static-shape step eagerly (the graph's reference). rules (of these sequences, in this order): applied to the
+        step's logits after the replay, into a tensor of their own; their histories hold the new tokens too."""
         b = len(seq_ids)
         if input_ids.shape != (b,):
             raise ValueError("one input id per sequence")
@@ -224,11 +227,12 @@ class DecodeGraphRunner:
         self._prepare(seq_ids, bucket)
         # the token ids go device to device (the previous step's argmax need not visit the host)
         self._d64[:b].copy_(input_ids.to(self._d64.device, torch.int64), non_blocking=True)
-        if not graph:
-            return self._forward(bucket)[:b]
-        g, logits, _ = self._graphs[bucket]
-        g.replay()
-        return logits[:b]
+        if graph:
+            g, logits, _ = self._graphs[bucket]
+            g.replay()
+        else:
+            logits = self._forward(bucket)
+        return logits[:b] if rules is None else rules.apply(logits[:b], grammar_rows=grammar_rows)
 
     def close(self) -> None:
         """Drop the graphs, return the scratch block to the manager, and detach device tables made here."""

@@ -199,6 +199,7 @@ class TreePlan:
             raise ValueError(f"masks must be contiguous int64 [{T}, >= {words}]")
         _hip.require_gpu(q, k_cache, v_cache, block_tables, context_lens, query_starts, masks)
         self.shape, self.pool_shape, self.device = (T, Hq, D), tuple(k_cache.shape), q.device
+        self._pool_strides = (N * B * D, B * D, D, 1)  # of a contiguous layer
         self._keep = (block_tables, context_lens, query_starts, masks)
         self._quantized = quant is not None
         p = self.params = _hip.TreeParams(
@@ -263,7 +264,7 @@ class TreePlan:
         the plan called with pools[layer] and the like, without making those views."""
         for t in (k_pools, v_pools):
             if t.shape[1:] != self.pool_shape or t.dtype is not self.pool_dtype or t.device != self.device or \
-                    not _hip.layers_contiguous(t):
+                    t.stride()[1:] != self._pool_strides:
                 raise ValueError("the pools do not match the plan")
         self._check_quant(quant, k_pools.shape[:1])
         self._bind_q(q)

@@ -17,6 +17,8 @@ import torch.nn.functional as F
 
 from . import hip_layer
 from .config import ModelConfig
+from .hip_logits import LogitsRules
+from .paged_cache import TreeMetadata
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -113,16 +115,28 @@ class Qwen2Model:
         return x + F.linear(F.silu(gate) * up, w.down_w)
 
     @torch.inference_mode()
-    def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, cache, meta, last_only: bool = True):
-        """Logits [num_seqs, vocab] (last token of each sequence; every token if not last_only) for a packed batch
-        described by meta (positions must be meta.positions)."""
+    def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, cache, meta, last_only: bool = True,
+                rules: LogitsRules | None = None, grammar_rows: torch.Tensor | None = None):
+        """Logits [num_seqs, vocab] (last token of each sequence; every token if not last_only, and every node of drafted
+        trees) for a packed batch described by meta (positions must be meta.positions). rules: applied to them, with
+        grammar_rows the grammar state of each row returned; a drafted node's path counts as generated, other rows see the
+        rules' histories as they are."""
         cache.begin(input_ids.shape[0], meta)
         x = self.embed[input_ids]
         rot = self.rotary.rows(positions, x.dtype)
         for i in range(self.cfg.num_layers):
             x = self.layer_forward(i, x, positions, cache, rot)
-        if last_only and meta.num_tokens != meta.num_seqs:  # one token a sequence: every row is a last one
+        tree = isinstance(meta, TreeMetadata)
+        if last_only and not tree and meta.num_tokens != meta.num_seqs:  # one token a sequence: every row is a last one
             x = x[meta.last_token_indices]
-        if hip_layer.rows_ok(x, self.final_norm):
-            return F.linear(hip_layer.rms_norm(x, self.final_norm, self.cfg.rms_norm_eps), self.lm_head)
-        return F.linear(rms_norm(x, self.final_norm, self.cfg.rms_norm_eps), self.lm_head)
+        norm = hip_layer.rms_norm if hip_layer.rows_ok(x, self.final_norm) else rms_norm
+        logits = F.linear(norm(x, self.final_norm, self.cfg.rms_norm_eps), self.lm_head)
+        if rules is None:
+            return logits
+        if tree:
+            return rules.apply(logits, query_starts=meta.query_starts_t, tokens=input_ids, masks=meta.masks,
+                               grammar_rows=grammar_rows)
+        starts = None
+        if logits.shape[0] != meta.num_seqs:
+            starts = torch.tensor(meta.query_starts, dtype=torch.int32).to(logits.device)
+        return rules.apply(logits, query_starts=starts, grammar_rows=grammar_rows)

@@ -30,6 +30,7 @@ from .config import ModelConfig
 from .hip_decode import DecodePlan
 from .hip_prefill import paged_prefill_attention, prefill_splits, prefill_supported
 from .hip_quant import store_layer
+from .hip_tree import MAX_NODES, TreePlan, commit_tokens, mask_words, tree_supported
 
 BACKENDS = ("gather", "hip", "triton")
 KERNEL_BACKENDS = ("hip", "triton")
@@ -160,6 +161,60 @@ def build_metadata(manager: BlockManager, batch: list[tuple[int, int, int]],
     )
 
 
+@dataclass
+class TreeMetadata(PagedMetadata):
+    """What a forward over drafted trees needs: PagedMetadata whose positions are the nodes' (cached tokens and ancestors),
+    with the trees themselves. Row query_starts[i] + j is node j of sequence i, its K and V in the slot of position
+    start + j."""
+    parents: list[list[int]]  # per sequence: each node's parent among the nodes before it, -1 for none
+    masks: torch.Tensor  # [T, words] int64: each node's ancestors and itself as bits (engine.hip_tree)
+    query_starts_t: torch.Tensor  # [num_seqs + 1] int32 on the device
+
+    @property
+    def max_nodes(self) -> int:
+        """Nodes of the largest tree."""
+        return max(map(len, self.parents))
+
+    def starts(self) -> list[int]:
+        """Cached tokens of each sequence before the forward."""
+        return [c - len(p) for c, p in zip(self.context_lens, self.parents)]
+
+
+def check_trees(batch: list[tuple[int, int, list[int]]]) -> list[tuple[int, int, int]]:
+    """The (seq_id, start, n) batch of [(seq_id, start, parents)], or ValueError for parents that are no tree of 1 to
+    hip_tree.MAX_NODES nodes in which parents come first."""
+    for seq_id, _, parents in batch:
+        if not 1 <= len(parents) <= MAX_NODES:
+            raise ValueError(f"sequence {seq_id}: a tree of {len(parents)} nodes; 1 to {MAX_NODES} can be drafted")
+        for i, p in enumerate(parents):
+            if not -1 <= p < i:
+                raise ValueError(f"sequence {seq_id}: node {i} has parent {p}; parents come before their nodes (-1 for none)")
+    return [(seq_id, start, len(parents)) for seq_id, start, parents in batch]
+
+
+def build_tree_metadata(manager: BlockManager, batch: list[tuple[int, int, list[int]]],
+                        device: str | torch.device) -> TreeMetadata:
+    """Metadata for a forward over drafted trees, batch = [(seq_id, start, parents)]: the sequence's nodes take the slots of
+    positions start .. start + len(parents) - 1, which the manager already holds. Built on the host
+    (engine.device_tables.DeviceBlockTables.build_tree derives the same on the device)."""
+    base = build_metadata(manager, check_trees(batch), device)
+    words = mask_words(max(len(parents) for _, _, parents in batch))
+    masks = np.zeros((base.num_tokens, words), dtype=np.uint64)
+    depth = np.zeros(base.num_tokens, dtype=np.int64)
+    starts = np.empty(base.num_tokens, dtype=np.int64)
+    for (_, start, parents), first in zip(batch, base.query_starts):
+        for i, p in enumerate(parents):
+            if p >= 0:
+                masks[first + i], depth[first + i] = masks[first + p], depth[first + p] + 1
+            masks[first + i, i // 64] |= np.uint64(1 << (i % 64))
+            starts[first + i] = start
+    fields = {f: getattr(base, f) for f in base.__dataclass_fields__}
+    fields["positions"] = torch.from_numpy(starts + depth).to(device)
+    return TreeMetadata(**fields, parents=[list(parents) for _, _, parents in batch],
+                        masks=torch.from_numpy(masks.view(np.int64)).to(device),
+                        query_starts_t=torch.tensor(base.query_starts, dtype=torch.int32).to(device))
+
+
 def _run(seqs: list[int]) -> slice | None:
     """The slice of increasing indices that are consecutive, None for others: a forward's decode rows (or its chunks)
     usually stand together, and slices of the metadata and of the rows are views, where lists of indices are uploads,
@@ -213,6 +268,9 @@ class PagedKVCache:
         self._decode = None
         self._prefill_launch = None
         self._plan = None  # decode launch parameters, built by the first attend() of the forward
+        self._tree_plan = None
+        if isinstance(meta, TreeMetadata) and self.attn_backend in KERNEL_BACKENDS and self.on_gpu:
+            return  # its rows all go to the tree attention
         if self.attn_backend not in KERNEL_BACKENDS:
             return
         if not self.on_gpu:
@@ -300,6 +358,11 @@ class PagedKVCache:
         m = self.meta
         a, b = m.query_starts[i], m.query_starts[i + 1]
         k, v = self.gather(layer, i)
+        if isinstance(m, TreeMetadata):
+            start, nodes = m.context_lens[i] - (b - a), torch.arange(b - a, device=q.device)
+            hidden = torch.zeros(b - a, m.context_lens[i], dtype=torch.bool, device=q.device)
+            hidden[:, start:] = (m.masks[a:b, nodes // 64] >> (nodes % 64) & 1) == 0
+            return attention(q[a:b], k, v, positions[a:b], self._key_positions(m.context_lens[i]), scale, hidden)
         return attention(q[a:b], k, v, positions[a:b], self._key_positions(m.context_lens[i]), scale)
 
     def _prefill_kernel_ok(self, max_context: int) -> bool:
@@ -323,6 +386,9 @@ class PagedKVCache:
         """Attention of every sequence in the forward over its own context. Returns [T, Hq * d]."""
         m = self.meta
         T, Hq, d = q.shape
+        if isinstance(m, TreeMetadata) and self.attn_backend in KERNEL_BACKENDS and \
+                tree_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads):
+            return self._attend_tree(layer, q, scale)
         if self._decode is None:
             if self._prefill_launch is not None:  # only multi-token rows, all on the prefill kernel
                 out = torch.empty(T, Hq, d, device=q.device, dtype=q.dtype)
@@ -356,6 +422,62 @@ class PagedKVCache:
         for i in self._prefill:
             out[m.query_starts[i]:m.query_starts[i + 1]] = self._attend_gather(layer, i, q, positions, scale)
         return out
+
+    def _attend_tree(self, layer: int, q: torch.Tensor, scale: float) -> torch.Tensor:
+        """Every row of a forward over drafted trees through the tree attention kernel. Returns [T, Hq * d]."""
+        m = self.meta
+        T, Hq, d = q.shape
+        if not _kernel_rows(q):
+            q = q.clone(memory_format=torch.contiguous_format)
+        plan = self._tree_plan
+        if plan is None or self._plan_scale != scale:  # first layer of the forward: validate once
+            self._tree_plan, self._plan_scale = TreePlan(
+                q, self.k[layer], self.v[layer], m.block_tables, m.context_lens_t, m.query_starts_t, m.masks, scale,
+                max(m.context_lens), m.max_nodes, quant=self._kernel_quant(layer)), scale
+            return self._tree_plan(q, self.k[layer], self.v[layer]).view(T, Hq * d)
+        return plan.run_layer(layer, q, self.k, self.v, self._all_quant()).view(T, Hq * d)
+
+    def _commit_pools(self) -> tuple:
+        """(K, V, K scales, V scales): what a token's row of every layer consists of; scales None without any."""
+        return self.k, self.v, None, None
+
+    def commit(self, accepted: list[list[int]], meta: TreeMetadata | None = None) -> None:
+        """Keep the accepted nodes of a forward over drafted trees (meta None: of the last one): node accepted[i][j] of
+        sequence i moves to its position start + j in every layer. Each list ascends, as a path from a root does. The caller
+        then gives up the other nodes' slots with manager.truncate(seq_id, start + len(accepted[i])). No counterpart in the
+        reference."""
+        m = self.meta if meta is None else meta
+        if not isinstance(m, TreeMetadata):
+            raise ValueError("commit needs the metadata of a forward over drafted trees")
+        if len(accepted) != m.num_seqs:
+            raise ValueError(f"{m.num_seqs} sequences, accepted nodes of {len(accepted)}")
+        for i, (path, parents) in enumerate(zip(accepted, m.parents)):
+            if any(b <= a for a, b in zip([-1, *path], path)) or (path and path[-1] >= len(parents)):
+                raise ValueError(f"sequence {i}: accepted nodes {path} must ascend within its {len(parents)} nodes")
+        most = max(map(len, accepted))
+        if most == 0:
+            return
+        starts = m.starts()
+        pools = self._commit_pools()
+        if self.on_gpu and pools[0].shape[-1] * pools[0].element_size() % 16 == 0 and pools[0].data_ptr() % 16 == 0 and \
+                pools[1].data_ptr() % 16 == 0:
+            S = m.num_seqs
+            flat = starts + [len(p) for p in accepted] + [x for p in accepted for x in [*p, *[-1] * (most - len(p))]]
+            d = torch.tensor(flat, dtype=torch.int32).to(self.device, non_blocking=True)
+            commit_tokens(pools[0], pools[1], m.block_tables, d[:S], d[2 * S:].view(S, most), d[S:2 * S],
+                          k_scale=pools[2], v_scale=pools[3])
+            return
+        B = self.block_size
+        frm, to = [], []
+        for i, path in enumerate(accepted):
+            table = m.block_ids_cpu[i]
+            for j, node in enumerate(path):
+                frm.append(table[(starts[i] + node) // B] * B + (starts[i] + node) % B)
+                to.append(table[(starts[i] + j) // B] * B + (starts[i] + j) % B)
+        f, t = torch.tensor(frm, device=self.device), torch.tensor(to, device=self.device)
+        for pool in pools:
+            if pool is not None:
+                pool[:, :, t // B, t % B] = pool[:, :, f // B, f % B]
 
     def _all_quant(self):
         """_kernel_quant's inputs for every layer (a leading layer dimension); None for the model-dtype pool."""

@@ -29,7 +29,7 @@ from .config import ModelConfig
 from .hip_decode import QuantKV
 from .hip_quant import (kchan_write_rows, quantize_store_block_rows, quantize_store_blocks, quantize_store_layer,
                         quantize_store_tokens, store_tokens)
-from .paged_cache import PagedKVCache, PagedMetadata, _run
+from .paged_cache import PagedKVCache, PagedMetadata, TreeMetadata, _run
 from .quant import dequantize, quantize_per_channel, quantize_per_token
 
 FORMATS = ("bf16", "int8", "int8-kchannel")
@@ -201,6 +201,9 @@ class QuantPagedKVCache(PagedKVCache):
 
     def begin(self, n_tokens: int, meta: PagedMetadata | None) -> None:
         """Base bookkeeping, then (format B) the staging plan of every block this forward writes."""
+        if self.fmt == "int8-kchannel" and isinstance(meta, TreeMetadata):
+            raise ValueError("int8-kchannel caches cannot hold drafted trees: a block's channel scales would be taken over "
+                             "nodes that are given up again; use bf16 or int8")
         super().begin(n_tokens, meta)
         if self.fmt != "int8-kchannel":
             return
@@ -338,6 +341,11 @@ class QuantPagedKVCache(PagedKVCache):
         if self.fmt == "int8":
             return QuantKV(1, self.k_scale[layer], self.v_scale[layer])
         return QuantKV(2, self.k_scale[layer], self.v_scale[layer], self.stage[layer], self._tails_dec)
+
+    def _commit_pools(self) -> tuple:
+        if self.fmt != "int8":
+            raise ValueError("int8-kchannel caches cannot hold drafted trees")
+        return self.k, self.v, self.k_scale, self.v_scale
 
     def _all_quant(self) -> QuantKV:
         if self.fmt == "int8":
