@@ -4,16 +4,23 @@
 // head m % G, so that small trees fill whole 16-row tiles whatever the group size. A row sees the sequence's cached tokens
 // and the nodes in its mask. The reference has no counterpart: it decodes one token per step.
 //
-// Work unit: (sequence, KV head, kRows rows); its keys are cut into splits of `chunk`, one workgroup each. The workgroup
-// brings 32 keys at a time into LDS, each of its waves takes 16 rows:
+// Work unit: (sequence, KV head, 64 or 128 rows); its keys are cut into splits of `chunk`, one workgroup each. The workgroup
+// brings 128 or 64 keys at a time into LDS (registers ahead of them carry the next stages), each of its waves takes 16 rows:
 //   S^T[16 keys x 16 rows] = K[16 x 32 d] . Q^T[32 d x 16 rows]   v_mfma_f32_16x16x32_bf16
 //   hidden keys -> -inf; online softmax per row in the exp2 domain
 //   O^T[16 d x 16 rows] += V^T . P^T
 // INT8 pools: the codes go to LDS as bf16, exactly; the scores are multiplied by K's scales and the probabilities by V's in
-// fp32. Splits write (m, l, O) and the last of a unit's to arrive merges them.
+// fp32. Splits write (m, l, O / l) and the last of a unit's to arrive merges them.
 // P enters the second product as two bf16 terms, 16 bits of it: one alone gives errors as large as the result's own rounding
 // (2.3e-3 of it in all against 1.7e-3). The second is taken from p (1 + 2^-20), so that it is never zero against an infinite
 // V.
+//
+// What bounds it: with few rows the pools' bytes (one node, 7 heads a KV head, 32 sequences of 8192 keys: 35 us, 3.8 TB/s);
+// from about 16 nodes on the vector ALUs, which turn each score into two bf16 terms of p, and the wait of the waves for each
+// other at a stage's end: a stage of 64 keys and 128 rows takes some 2400 cycles, 1000 of them the softmax of a SIMD's two
+// waves, 460 the scores, 370 the second product. 16 nodes, 32 sequences of 8192 keys: 48 us of 27 for the bytes; 64 nodes, 16
+// ragged sequences about 12000 long, head_dim 128: 155 us of 43; INT8, 11 nodes, 64 sequences of 4096: 72 us of 28. Short
+// calls take the chain of one workgroup's loads: 11 us for 5 nodes at 1024 keys.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,6 +57,7 @@ struct TreeArgs {
   int32_t log_b;           // blocks of 1 << log_b tokens
   int32_t groups;          // row groups of the longest sequence
   int32_t nsplit, chunk;
+  int32_t log_spread;      // a pair has 1 << log_spread XCDs
   float scale_log2;
   int* counters;           // [units]
   float* pm;               // [units][nsplit][rows of a group]
@@ -81,7 +89,7 @@ __device__ __forceinline__ u32x4 tree_codes(uint32_t w0, uint32_t w1) {
 // MR row tiles of 16 per wave, RW waves side by side over the rows, KW waves one after the other over the keys, each KPW
 // keys of a stage of KW KPW; NPRE stages in flight in registers.
 template <int D, int MODE, int MR, int RW, int KW, int KPW, int NPRE>
-__global__ void __launch_bounds__(64 * RW * KW, D == 64 && MODE == 0 && KPW == 32 ? 4 : 2) tree_attention_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(64 * RW * KW, 2) tree_attention_kernel(const TreeArgs a) {
   constexpr int KT = KW * KPW, MT = KPW / 16, HT = KPW / 32, P = D + 16, KS = D / 32, DT = D / 16;
   constexpr int PT = 64 * RW * KW, ROWS = 16 * MR * RW;
   constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, NCH = KT * CPK;  // 16-byte parts of a key, of a stage
@@ -94,11 +102,14 @@ __global__ void __launch_bounds__(64 * RW * KW, D == 64 && MODE == 0 && KPW == 3
   __shared__ int last_flag, dirty;
 
   // Workgroup L is dealt to XCD L % 8: a pair's row groups and splits share one, so that its L2 serves the groups the same
-  // keys and the merge its partials.
-  const int L = blockIdx.x, per = a.nsplit * a.groups;
-  const int pair = (L & 7) + 8 * ((L >> 3) / per), in = (L >> 3) % per;
-  if (pair >= a.S * a.Hkv) return;  // the grid is padded to whole groups of 8 pairs
-  const int sp = in / a.groups, rg = in % a.groups, s = pair % a.S, h = pair / a.S;
+  // keys and the merge its partials. With few pairs their splits go round 1 << a.log_spread XCDs.
+  // The heads' sequences are shifted against each other, so that no XCD has the same long sequence twice (4 sequences of up to
+  // 128 nodes x 15000 keys, INT8: 97 -> 86 us).
+  const int L = blockIdx.x, log_side = 3 - a.log_spread;  // 1 << log_side pairs side by side
+  const int per = ((a.nsplit + (1 << a.log_spread) - 1) >> a.log_spread) * a.groups, turn = (L >> 3) / per, in = (L >> 3) - turn * per;
+  const int pair = (L & ((1 << log_side) - 1)) + (turn << log_side), sp = ((in / a.groups) << a.log_spread) + ((L & 7) >> log_side);
+  if (pair >= a.S * a.Hkv || sp >= a.nsplit) return;  // the grid is padded
+  const int rg = in % a.groups, h = pair / a.S, s = (pair + 3 * h) % a.S;
   const int u = pair * a.groups + rg;
   const int row0 = a.qs[s], all = a.qs[s + 1] - row0, n = min(min(all, a.max_nodes), a.T - row0);
   const int G = a.G, M = n * G, m0 = rg * ROWS;
@@ -466,10 +477,10 @@ __global__ void __launch_bounds__(64 * RW * KW, D == 64 && MODE == 0 && KPW == 3
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    // +2^16 from a workgroup that is not on the pair's XCD: the last to arrive then reads through memory, else from its L2
+    // +2^16 from a workgroup that is not on the pair's one XCD: the last to arrive then reads through memory, else from its L2
     uint32_t xcc;
     asm volatile("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
-    const int away = (int)(xcc & 0xf) != (L & 7);
+    const int away = a.log_spread > 0 || (int)(xcc & 0xf) != (L & 7);
     const int prev = __hip_atomic_fetch_add(a.counters + u, 1 + (away << 16), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last_flag = (prev & 0xffff) == nvalid - 1 ? 1 + ((prev >> 16) + away == 0) : 0;
   }
@@ -534,7 +545,7 @@ using namespace sipa;
 
 struct TreeLayout {
   int variant, rows;  // index into the launch table below, rows of a workgroup
-  int groups, units, nsplit, chunk;
+  int groups, units, nsplit, chunk, log_spread;
   int64_t pm, pl, part, total;  // byte offsets into the workspace; counters first
 };
 
@@ -567,7 +578,44 @@ constexpr TreeVariant kTreeVariants[] = {{1, 4, 2, 64}, {1, 8, 1, 64}};  // up t
 // Bytes of the kernel's tile buffers, which the merge's m and l have to fit.
 static int tree_tile_bytes(const TreeVariant& v, int D) { return 2 * 2 * v.kw * v.kpw * (D + 16) * 2; }
 
-// About one workgroup per CU, splits of at least 256 keys.
+// XCDs that a pair's splits go round, as a power of two. Few pairs on one XCD each would leave CUs idle (one sequence of 2 KV
+// heads has 64 of 256), and with a handful of sequences the XCDs' work differs; against that, the merge then reads through
+// memory. One sequence, 16-bit pools, 14 heads of 64, 30000 keys: 120 nodes 115 -> 58 us, 15 nodes 42 -> 33; at 2000 keys 11
+// and 14 us either way. 5 to 16 pairs: 5 to 7 % less in the mean with several row groups, 0 to 2 % with one; 17 to 64: 1 to
+// 4 % more.
+static int tree_log_spread(int64_t pairs, int nsplit) {
+  const int want = pairs == 1 ? 3 : pairs == 2 ? 2 : pairs <= 16 ? 1 : 0;
+  return nsplit == 1 ? 0 : want;
+}
+
+// The number of splits: the cheapest by a count of keys. A workgroup costs its split's keys and 256 more (its start and end), a
+// CU takes one after the other, two at once where both fit (the larger variant over plain pools at head_dim 64: 1.6 times one's
+// time), and a merge costs 256 keys and 24 a split. The lengths are on the device: the count takes every sequence for one of
+// max_context keys; where the trees' sizes differ (the token count shows it) many workgroups find no rows or keys, and half of
+// the count is that of 0.7 of the workgroups. Fitted to 468 batches (1 to 128 sequences, 1 to 128 nodes, contexts to 16384 keys,
+// both types and head sizes, over half ragged): 2.3 % over the best count's time in the mean, 1.6 times at most. One workgroup
+// per CU, rounded up, took 12 % more in the mean: 40 sequences of 2 heads made 320 workgroups of 4 splits each (31 us for 4
+// nodes at 3000 keys, 16-bit pools), where 3 splits fill 240 of the 256 CUs (20 us).
+static int tree_splits(const sipa_tree_params* p, int groups, int kt, bool two, int cus, int most) {
+  const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads, per_xcd = std::max(cus / 8, 1);
+  const bool differ = p->num_tokens < (int64_t)p->num_seqs * p->max_nodes;
+  auto fifths = [&](int64_t wgs) {  // of a lone workgroup's time, for the workgroups of an XCD
+    const int64_t turns = (wgs + per_xcd - 1) / per_xcd;
+    return two ? 8 * (turns / 2) + 5 * (turns % 2) : 5 * turns;
+  };
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= most && (int64_t)128 * (n - 1) < p->max_context; n += 1 + n / 8) {
+    const int64_t chunk = ((p->max_context + n - 1) / n + kt - 1) / kt * kt;
+    const int spread = 1 << tree_log_spread(pairs, n), side = 8 / spread;
+    const int64_t wgs = (pairs + side - 1) / side * groups * ((n + spread - 1) / spread);
+    const int64_t time = fifths(wgs) + fifths(differ ? (7 * wgs + 9) / 10 : wgs);
+    const int64_t cost = time * (chunk + 256) + 10 * (n > 1 ? 256 + 24 * n : 0);
+    if (cost < least) least = cost, best = n;
+  }
+  return best;
+}
+
 static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   const int G = p->num_q_heads / p->num_kv_heads;
   const int need = p->max_nodes * G;
@@ -578,17 +626,18 @@ static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   const int64_t units = (int64_t)p->num_seqs * p->num_kv_heads * l->groups;
   SIPA_CHECK(units <= 0x7fffffff / kTreeMaxSplits, SIPA_EINVAL, "%lld units exceed the grid limit", (long long)units);
   l->units = (int)units;
-  int64_t splits = p->num_splits;
+  const int kt = v.kw * v.kpw;  // whole stages
+  const int most = std::min(kTreeMaxSplits, tree_tile_bytes(v, p->head_dim) / (8 * l->rows));
+  int splits = std::min(p->num_splits, most);
   if (splits <= 0) {
     const int cus = sipa_device_cu_count(-1);
     if (cus < 0) return cus;
-    splits = std::min<int64_t>((cus + units - 1) / std::max<int64_t>(units, 1), (p->max_context + 255) / 256);
+    splits = tree_splits(p, l->groups, kt, l->variant == 1 && p->head_dim == 64 && p->kv_mode == SIPA_KV_PLAIN, cus, most);
   }
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, std::min<int64_t>(kTreeMaxSplits, tree_tile_bytes(v, p->head_dim) / (8 * l->rows))));
-  const int chunk = (int)((p->max_context + splits - 1) / splits);
-  const int kt = v.kw * v.kpw;  // whole stages
+  const int chunk = (p->max_context + splits - 1) / splits;
   l->chunk = std::min((chunk + kt - 1) / kt * kt, kTreeMaxChunk);
   l->nsplit = (p->max_context + l->chunk - 1) / l->chunk;
+  l->log_spread = tree_log_spread((int64_t)p->num_seqs * p->num_kv_heads, l->nsplit);
   l->pm = l->pl = l->part = l->total = 0;
   if (l->nsplit > 1) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
@@ -708,6 +757,7 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   a.log_b = p->block_size == 16 ? 4 : p->block_size == 32 ? 5 : 6;
   a.groups = l.groups;
   a.nsplit = l.nsplit;
+  a.log_spread = l.log_spread;
   a.chunk = l.chunk;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   char* ws = (char*)p->workspace;
@@ -715,8 +765,8 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   a.pm = (float*)(ws + l.pm);
   a.pl = (float*)(ws + l.pl);
   a.part = (uint16_t*)(ws + l.part);
-  const int64_t pairs8 = ((int64_t)p->num_seqs * p->num_kv_heads + 7) / 8 * 8;
-  const dim3 grid((unsigned)(pairs8 * l.groups * l.nsplit));
+  const int64_t side = 8 >> l.log_spread, rounds = ((int64_t)p->num_seqs * p->num_kv_heads + side - 1) / side;
+  const dim3 grid((unsigned)(8 * rounds * l.groups * ((l.nsplit + (1 << l.log_spread) - 1) >> l.log_spread)));
   hipStream_t st = (hipStream_t)stream;
   if (p->head_dim == 64) {
     if (int8) launch_tree<64, 1>(l.variant, grid, st, a);
