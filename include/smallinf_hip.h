@@ -687,7 +687,8 @@ int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream);
 typedef struct sipa_tree_params {
   int32_t struct_size; /* sizeof(sipa_tree_params) */
   int32_t num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
-  int32_t max_context;  /* largest context length, known on the host; context lengths are clamped to it */
+  int32_t max_context;  /* largest context length, known on the host; context lengths are clamped to it. Up to 655360 (head_dim
+                           64) or 1179648 (128), 2097152 for trees of up to 64 rows of query heads */
   int32_t max_nodes;    /* largest n_s, at most 64 words; rows past it are left as they are */
   int32_t words;        /* of a mask: 1 .. 4 */
   float scale;          /* positive and finite */

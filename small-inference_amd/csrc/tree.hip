@@ -575,7 +575,8 @@ struct TreeVariant {
 };
 constexpr TreeVariant kTreeVariants[] = {{1, 4, 2, 64}, {1, 8, 1, 64}};  // up to 64 rows, more
 
-// Bytes of the kernel's tile buffers, which the merge's m and l have to fit.
+// Bytes of the kernel's tile buffers, which the merge's m and l have to fit: the number of splits, and with it the context, is
+// limited by them (40 splits, 655360 keys, for more than 64 rows at head_dim 64).
 static int tree_tile_bytes(const TreeVariant& v, int D) { return 2 * 2 * v.kw * v.kpw * (D + 16) * 2; }
 
 // XCDs that a pair's splits go round, as a power of two. Few pairs on one XCD each would leave CUs idle (one sequence of 2 KV
@@ -637,6 +638,7 @@ static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   const int chunk = (p->max_context + splits - 1) / splits;
   l->chunk = std::min((chunk + kt - 1) / kt * kt, kTreeMaxChunk);
   l->nsplit = (p->max_context + l->chunk - 1) / l->chunk;
+  SIPA_CHECK(l->nsplit <= most, SIPA_EUNSUPPORTED, "max_context %d past %d splits of %d keys", p->max_context, most, kTreeMaxChunk);
   l->log_spread = tree_log_spread((int64_t)p->num_seqs * p->num_kv_heads, l->nsplit);
   l->pm = l->pl = l->part = l->total = 0;
   if (l->nsplit > 1) {
