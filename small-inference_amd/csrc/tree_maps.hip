@@ -36,8 +36,9 @@ __device__ __forceinline__ int32_t tree_table_entry(const TreeMapsArgs& a, int s
   return a.tables[(int64_t)row * a.table_stride + c];
 }
 
-// Every workgroup forms the query starts for itself (S loads that the L2 serves, one scan), so that one launch does it
-// all: bound by its latency, not by bytes.
+// Every workgroup forms the query starts for itself (S loads that the L2 serves, one scan), so that one launch does it all: bound
+// by the latency of its chain of loads, not by bytes: 3.4 us for 1 tree of 5 nodes; 9.0 us for 256 ragged trees of up to 64
+// nodes at 8192 tokens. An ancestor is one load after the other, as many as the tree is deep.
 __global__ void __launch_bounds__(256) tree_maps_kernel(const TreeMapsArgs a) {
   __shared__ int32_t qs[kTreeMaxSeqs + 1];
   __shared__ int32_t part[256];
@@ -117,7 +118,9 @@ struct CommitArgs {
 
 // One thread takes one 16-byte part of the moved rows of a (sequence, pool, layer, head), all its moves in order: source
 // indices ascend and are at least their destinations', so a load never reads what an earlier store has written. Kept at
-// kMoves loads in flight before their stores.
+// kMoves loads in flight before their stores: bound by latency (index, block id, row), 4.4 us for up to 4 nodes of one
+// sequence in 24 layers, 10.7 us for 64 sequences' up to 7 nodes in 28 layers of INT8 pools (a call with the host's part: 7.8
+// and 12.0).
 constexpr int kMoves = 8;
 
 __global__ void __launch_bounds__(256) commit_tokens_kernel(const CommitArgs a) {
