@@ -635,7 +635,7 @@ int32_t sipa_commit_tokens(const sipa_commit_params* p, void* stream);
  * no counterpart). For row r of sequence s and token v, with l = logits[r, v] in fp32:
  *   made = times v occurs among the sequence's generated tokens (history[prompt_lens[s] ..]) and on the row's path, the
  *          tokens of the nodes in its mask; seen = made > 0 or v occurs in the prompt (history[.. prompt_lens[s] - 1])
- *   l = l > 0 ? l / repetition[s] : l * repetition[s]        where seen
+ *   l = l > 0 ? l * (1 / repetition[s]) : l * repetition[s]  where seen
  *   l = l - frequency[s] * made - presence[s]                where made > 0
  *   l = l + the sum of the values that the sequence's bias list gives v, added up in the list's order
  *   l = -inf                                                 where the row has a grammar state whose bit v is 0
@@ -671,6 +671,8 @@ typedef struct sipa_logits_params {
   int64_t grammar_stride;        /* words, at least ceil(vocab / 32) */
   int32_t grammar_states;
   const int32_t* grammar_rows;   /* [num_rows] state of each row, -1 for none */
+  int64_t history_size;          /* entries of history, and of the bias lists: the starts are clamped to them */
+  int32_t num_biases;
 } sipa_logits_params;
 
 int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream);

@@ -28,6 +28,8 @@ struct LogitsArgs {
   const int32_t* btok;
   const float* bval;
   const int32_t* bstarts;
+  int64_t hsize;
+  int32_t nbias;
   const uint32_t* grammar;
   int64_t g_st;
   int32_t states;
@@ -129,12 +131,13 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
     if (a.freq != nullptr) alpha = a.freq[s];
     if (a.pres != nullptr) beta = a.pres[s];
     inv_rho = 1.f / rho;
+    const int b0 = a.bstarts != nullptr ? max(a.bstarts[s], 0) : 0, b1 = a.bstarts != nullptr ? min(a.bstarts[s + 1], a.nbias) : 0;
     *(uint4*)(cnt + 4 * tid) = uint4{0, 0, 0, 0};
     if (E == 8) *(uint4*)(cnt + 4 * tid + 4 * THR) = uint4{0, 0, 0, 0};
     if (tid == 0) num_hits = has_path = 0;
     __syncthreads();
     if (a.history != nullptr) {
-      const int64_t h0 = a.hstarts[s], h1 = a.hstarts[s + 1];
+      const int64_t h0 = min(max(a.hstarts[s], (int64_t)0), a.hsize), h1 = min(a.hstarts[s + 1], a.hsize);
       const int64_t made = h0 + (a.prompt != nullptr ? max(a.prompt[s], 0) : 0);
       constexpr int U = 8, CHUNK = THR * U;  // loads in flight
       for (int64_t at = h0; at < h1; at += CHUNK) {
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
       }
     }
     if (a.bstarts != nullptr)
-      for (int b = a.bstarts[s] + tid; b < a.bstarts[s + 1]; b += THR) {
+      for (int b = b0 + tid; b < b1; b += THR) {
         const uint32_t at = (uint32_t)a.btok[b] - (uint32_t)v0;
         if (at >= (uint32_t)n || a.btok[b] < 0) continue;
         atomicOr(&cnt[at], kBiased);
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
             last = next;
           }
         } else {
-          for (int b = a.bstarts[s]; b < a.bstarts[s + 1]; ++b)
+          for (int b = b0; b < b1; ++b)
             if (a.btok[b] == v0 + i0 + e) bias[e] += a.bval[b];
         }
       }
@@ -289,6 +292,7 @@ extern "C" int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream)
   SIPA_CHECK(p->tokens == nullptr || (p->words >= 1 && p->words <= 4), SIPA_EINVAL, "%d mask words (1 .. 4)", p->words);
   SIPA_CHECK(p->bias_starts == nullptr || (p->bias_tokens && p->bias_values), SIPA_EINVAL,
              "a bias needs tokens and values");
+  SIPA_CHECK(p->history_size >= 0 && p->num_biases >= 0, SIPA_EINVAL, "lists of negative sizes");
   SIPA_CHECK(p->grammar_rows == nullptr ||
                  (p->grammar && p->grammar_states > 0 && p->grammar_stride * 32 >= p->vocab), SIPA_EINVAL,
              "a grammar needs states of ceil(vocab / 32) words");
@@ -314,6 +318,8 @@ extern "C" int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream)
   a.btok = p->bias_tokens;
   a.bval = p->bias_values;
   a.bstarts = p->bias_starts;
+  a.hsize = p->history_size;
+  a.nbias = p->num_biases;
   a.grammar = p->grammar;
   a.g_st = p->grammar_stride;
   a.states = p->grammar_states;

@@ -155,6 +155,7 @@ class LogitsParams(ctypes.Structure):
         ("history", vp), ("history_starts", vp), ("prompt_lens", vp), ("repetition", vp), ("frequency", vp),
         ("presence", vp), ("tokens", vp), ("masks", vp), ("bias_tokens", vp), ("bias_values", vp), ("bias_starts", vp),
         ("grammar", vp), ("grammar_stride", i64), ("grammar_states", i32), ("grammar_rows", vp),
+        ("history_size", i64), ("num_biases", i32),
     ]
 
 

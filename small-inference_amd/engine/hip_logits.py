@@ -32,7 +32,8 @@ class LogitsRules:
     history int32, the sequences' tokens one after the other, with history_starts int64 [S + 1]; prompt_lens int32 [S], how
     many of a sequence's tokens are prompt (0); repetition (positive), frequency, presence fp32 [S]; bias_tokens int32 and
     bias_values fp32, with bias_starts int32 [S + 1]; grammar int32 [states, >= ceil(vocab / 32)], bit v % 32 of word v // 32
-    set where the state allows token v. Tokens outside the vocabulary (-1 as padding) are ignored. The tensors are read at
+    set where the state allows token v. Tokens outside the vocabulary (-1 as padding) are ignored, starts
+    are clamped to their lists. The tensors are read at
     every apply(), so a program may write new values into them between steps."""
 
     def __init__(self, vocab: int, num_seqs: int, *, history: torch.Tensor | None = None,
@@ -86,6 +87,8 @@ class LogitsRules:
             p.history = p.history_starts = p.prompt_lens = None
         if bias_tokens is not None and bias_tokens.numel() == 0:
             p.bias_tokens = p.bias_values = p.bias_starts = None
+        p.history_size = 0 if history is None else history.numel()
+        p.num_biases = 0 if bias_tokens is None else bias_tokens.numel()
         if grammar is not None:
             p.grammar_stride, p.grammar_states = grammar.stride(0), grammar.shape[0]
 
@@ -144,8 +147,8 @@ class LogitsRules:
         """apply() on CPU tensors, row by row."""
         R, V = logits.shape
         qs = list(range(R + 1)) if query_starts is None else query_starts.tolist()
-        hs = None if self.history is None else self.history_starts.tolist()
-        bs = None if self.bias_starts is None else self.bias_starts.tolist()
+        hs = None if self.history is None else self.history_starts.clamp(0, self.history.numel()).tolist()
+        bs = None if self.bias_starts is None else self.bias_starts.clamp(0, self.bias_tokens.numel()).tolist()
         words = None if masks is None else masks.tolist()
         result = logits.float()
         if result is logits:

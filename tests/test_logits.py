@@ -211,6 +211,21 @@ def test_a_token_many_times(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_starts_outside_their_lists_are_clamped(device):
+    # history 0 0 1 and biases of 2 and 3, with starts that point before and far behind them
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    f32 = lambda *x: torch.tensor(x, dtype=torch.float32, device=device)  # noqa: E731
+    # one token a value beside the lists: entries read past them would change the second sequence's logits
+    lists, biases = i32(0, 0, 1, 3, 3, 3, 3, 3), f32(4, 8, 16, 16, 16, 16)
+    rules = LogitsRules(8, 2, history=lists[:3], history_starts=torch.tensor([-5, 2, 1 << 40], device=device),
+                        frequency=f32(1, 1), bias_tokens=i32(2, 3, 4, 5, 6, 7)[:2], bias_values=biases[:2],
+                        bias_starts=i32(-3, 1, 1 << 30))
+    got = rules.apply(torch.zeros(2, 8, device=device)).cpu()
+    want = torch.tensor([[-2., 0, 4, 0, 0, 0, 0, 0], [0., -1, 0, 8, 0, 0, 0, 0]])
+    assert torch.equal(got, want), got
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_empty_lists(device):
     z = lambda dt: torch.zeros(0, dtype=dt, device=device)  # noqa: E731
     rules = LogitsRules(10, 1, history=z(torch.int32), history_starts=torch.zeros(2, dtype=torch.int64, device=device),
