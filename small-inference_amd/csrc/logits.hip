@@ -281,8 +281,8 @@ extern "C" int32_t sipa_adjust_logits(const sipa_logits_params* p, void* stream)
   SIPA_CHECK(p != nullptr && p->struct_size == (int32_t)sizeof(sipa_logits_params), SIPA_EINVAL,
              "struct_size does not match this library's sipa_logits_params (%d bytes)",
              (int)sizeof(sipa_logits_params));
-  SIPA_CHECK(p->num_rows >= 0 && p->num_seqs > 0 && p->vocab > 0 && p->vocab <= 1 << 26, SIPA_EINVAL,
-             "%d rows, %d sequences, vocabulary %d (up to 2^26)", p->num_rows, p->num_seqs, p->vocab);
+  SIPA_CHECK(p->num_rows >= 0 && p->num_seqs > 0 && p->vocab > 0 && p->vocab <= 1 << 25, SIPA_EINVAL,
+             "%d rows, %d sequences, vocabulary %d (up to 2^25)", p->num_rows, p->num_seqs, p->vocab);
   if (p->num_rows == 0) return SIPA_OK;
   SIPA_CHECK(p->dtype == SIPA_F32 || p->dtype == SIPA_BF16 || p->dtype == SIPA_F16, SIPA_EUNSUPPORTED,
              "logits of type %d", p->dtype);

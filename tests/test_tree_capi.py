@@ -125,5 +125,38 @@ def test_commit_of_nothing():
     assert _hip.lib().sipa_commit_tokens(ctypes.byref(commit(max_accepted=0)), None) == 0
 
 
+def logits(**over):
+    base = dict(num_rows=2, vocab=1000, num_seqs=2, dtype=_hip.BF16, words=1, logits_stride=1000, out_stride=1000, history_size=10,
+                num_biases=4, grammar_stride=32, grammar_states=2)
+    return filled(_hip.LogitsParams, **{**base, **over})
+
+
+@pytest.mark.parametrize("over,code", [
+    ({"struct_size": 8}, _hip.EINVAL),
+    ({"num_rows": -1}, _hip.EINVAL),
+    ({"num_seqs": 0}, _hip.EINVAL),
+    ({"vocab": 0}, _hip.EINVAL),
+    ({"vocab": (1 << 25) + 1}, _hip.EINVAL),  # tiles of 1024 fp32 logits, at most 65535 of them in a grid's second dimension
+    ({"dtype": 99}, _hip.EUNSUPPORTED),
+    ({"logits": None}, _hip.EINVAL),
+    ({"history_starts": None}, _hip.EINVAL),
+    ({"masks": None}, _hip.EINVAL),
+    ({"words": 0}, _hip.EINVAL),
+    ({"words": 5}, _hip.EINVAL),
+    ({"bias_values": None}, _hip.EINVAL),
+    ({"history_size": -1}, _hip.EINVAL),
+    ({"num_biases": -1}, _hip.EINVAL),
+    ({"grammar": None}, _hip.EINVAL),
+    ({"grammar_states": 0}, _hip.EINVAL),
+    ({"grammar_stride": 31}, _hip.EINVAL),
+])
+def test_logits_refuse(over, code):
+    assert _hip.lib().sipa_adjust_logits(ctypes.byref(logits(**over)), None) == code
+
+
+def test_logits_of_nothing():
+    assert _hip.lib().sipa_adjust_logits(ctypes.byref(logits(num_rows=0)), None) == 0
+
+
 def test_no_capture_on_the_default_stream():
     assert _hip.lib().sipa_capture_id(None) == 0
