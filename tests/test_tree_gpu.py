@@ -50,6 +50,23 @@ def test_blocks_and_splits(block, splits, int8):
     check(c, attend(c, num_splits=splits))
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("splits", [None, 2, 3, 7, 13])
+@pytest.mark.parametrize("seqs,heads", [(1, (7, 1, 64)), (1, (14, 2, 64)), (3, (6, 1, 128)), (2, (4, 2, 128)), (5, (6, 2, 64)),
+                                        (9, (2, 1, 64)), (9, (14, 2, 64))])
+def test_splits_on_one_or_several_xcds(seqs, heads, splits, int8):
+    # 1, 2, 3 and 4, up to 16 and more pairs of a sequence and a KV head; row groups where the trees are large. The merge
+    # reads splits in their order: a second call on the plan's workspace gives the same bits.
+    c = Case([(1500 - 97 * i, 5 + 9 * (i % 3)) for i in range(seqs)], heads, int8=int8, seed=seqs)
+    print(seqs, heads, splits, int8, flush=True)
+    plan = TreePlan(c.q, c.k, c.v, c.bt, c.ctx, c.qs, c.masks, c.scale, c.max_ctx, c.max_nodes, quant=c.quant(),
+                    num_splits=splits)
+    first = plan(c.q, c.k, c.v)
+    check(c, first)
+    for _ in range(3):
+        assert torch.equal(plan(c.q, c.k, c.v), first)
+
+
 def test_largest_trees():
     c = Case([(50, 256), (0, 255), (1000, 129)], (2, 2, 64), seed=3)
     check(c, attend(c))
