@@ -10,7 +10,7 @@
 //   hidden keys -> -inf; online softmax per row in the exp2 domain
 //   O^T[16 d x 16 rows] += V^T . P^T
 // INT8 pools: the codes go to LDS as bf16, exactly; the scores are multiplied by K's scales and the probabilities by V's in
-// fp32. Splits write (m, l, O / l) and the last of a unit's to arrive merges them.
+// fp32. Splits write (m, l, O), all fp32, and the last of a unit's to arrive merges them.
 // P enters the second product as two bf16 terms, 16 bits of it: one alone gives errors as large as the result's own rounding
 // (2.3e-3 of it in all against 1.7e-3). The second is taken from p (1 + 2^-20), so that it is never zero against an infinite
 // V.
@@ -62,7 +62,7 @@ struct TreeArgs {
   int* counters;           // [units]
   float* pm;               // [units][nsplit][rows of a group]
   float* pl;               // the same
-  uint16_t* part;          // [units][nsplit][rows of a group][D] fp16
+  float* part;             // [units][nsplit][rows of a group][D]
 };
 
 // A scale as it lies in memory, and its value: apart, so that the load is waited for only where the value is needed.
@@ -445,10 +445,10 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) tree_attention_kernel(const T
     }
     return;
   }
-  // The split's state: m and l of each row, and its own output O / l as fp16 (the weighted mean of its V rows: 2^-12 of it),
-  // half the bytes of fp32 sums. A row whose largest |O / l| reaches 2^15 is stored times 2^-e, e in l's low mantissa bits.
+  // The split's state: m, l and O of each row, as the accumulators hold them. (O / l in fp16 takes half the bytes, but holds no
+  // V under 2^-25, and one exponent a row no finite value beside an infinite one.)
   const int64_t first = (int64_t)u * a.nsplit * ROWS;
-  const int split_bytes = ROWS * D * 2;
+  const int split_bytes = ROWS * D * 4;
   const __amdgpu_buffer_rsrc_t rows =
       __builtin_amdgcn_make_buffer_rsrc(a.part + first * D, (short)0, a.nsplit * split_bytes, 0x00020000);
   if (owner) {
@@ -456,25 +456,13 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) tree_attention_kernel(const T
     for (int c = 0; c < MR; ++c) {
       const int slot = 16 * (MR * rw + c) + r;
       if (m0 + slot >= M) continue;
-      const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
-      float big = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) big = vmax(big, fabsf(acc[c][dt][i]));
-      big = max_over_rows_swap(big * inv);
-      const int e = big < 32768.f ? 0 : max(__builtin_amdgcn_frexp_expf(big) - 15, 0);  // inf and NaN: 0
-      const float inv_e = __builtin_amdgcn_ldexpf(inv, -e);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        __builtin_amdgcn_raw_buffer_store_b64(
-            u32x2{pack_f16x2(acc[c][dt][0] * inv_e, acc[c][dt][1] * inv_e),
-                  pack_f16x2(acc[c][dt][2] * inv_e, acc[c][dt][3] * inv_e)},
-            rows, sp * split_bytes + (slot * D + 16 * dt + 4 * q4) * 2, 0, kAuxSc1);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[c][dt]), rows,
+                                               sp * split_bytes + (slot * D + 16 * dt + 4 * q4) * 4, 0, kAuxSc1);
       if (q4 == 0) {
         store_coherent(a.pm + first + sp * ROWS + slot, m_run[c]);
-        store_coherent(a.pl + first + sp * ROWS + slot,
-                       __uint_as_float((__float_as_uint(l[c]) & ~0xffu) | (uint32_t)e));
+        store_coherent(a.pl + first + sp * ROWS + slot, l[c]);
       }
     }
   }
@@ -496,12 +484,12 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) tree_attention_kernel(const T
       __builtin_amdgcn_make_buffer_rsrc(a.pl + first, (short)0, a.nsplit * ROWS * 4, 0x00020000);
   // Every split's m and l first, in LDS, then each thread 8 channels of a row with kMerge splits' loads in flight.
   float* lm = (float*)&sm[0][0][0];  // [nvalid][ROWS] m, then l
-  uint32_t* ll = (uint32_t*)(lm + nvalid * ROWS);
+  float* ll = lm + nvalid * ROWS;
   auto merge = [&](auto tag) {
     constexpr int AUX = decltype(tag)::value, kMerge = 8;
     for (int i = tid; i < nvalid * ROWS; i += PT) {
       lm[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mrows, i * 4, 0, AUX));
-      ll[i] = __builtin_amdgcn_raw_buffer_load_b32(lrows, i * 4, 0, AUX);
+      ll[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(lrows, i * 4, 0, AUX));
     }
     __syncthreads();
     for (int i = tid; i < ROWS * (D / 8); i += PT) {
@@ -511,20 +499,22 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) tree_attention_kernel(const T
       for (int j = 0; j < nvalid; ++j) top = fmaxf(top, lm[j * ROWS + slot]);
       f32x4 num[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       for (int j0 = 0; j0 < nvalid; j0 += kMerge) {
-        u32x4 o[kMerge];
+        f32x4 o[kMerge][2];
 #pragma unroll
         for (int x = 0; x < kMerge; ++x)
-          o[x] = __builtin_amdgcn_raw_buffer_load_b128(rows, min(j0 + x, nvalid - 1) * split_bytes + (slot * D + ch) * 2, 0, AUX);
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            o[x][y] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                rows, min(j0 + x, nvalid - 1) * split_bytes + (slot * D + ch + 4 * y) * 4, 0, AUX));
 #pragma unroll
         for (int x = 0; x < kMerge; ++x) {
           const int j = min(j0 + x, nvalid - 1);
-          const uint32_t lb = ll[j * ROWS + slot];
-          const float w = j0 + x >= nvalid || top == kNegInf ? 0.f : fast_exp2(lm[j * ROWS + slot] - top) * __uint_as_float(lb & ~0xffu);
+          const float f = j0 + x >= nvalid || top == kNegInf ? 0.f : fast_exp2(lm[j * ROWS + slot] - top);
+          const float w = f * ll[j * ROWS + slot];
           if (w == 0.f) continue;  // a split without a key for the row
           den += w;
-          const float wo = __builtin_amdgcn_ldexpf(w, (int)(lb & 0xffu));
 #pragma unroll
-          for (int y = 0; y < 8; ++y) num[y >> 2][y & 3] += wo * f16_bits_to_f32(y & 1 ? o[x][y >> 1] >> 16 : o[x][y >> 1] & 0xffffu);
+          for (int y = 0; y < 2; ++y) num[y] += f * o[x][y];
         }
       }
       const float inv = den == 0.f ? 0.f : 1.f / den;
@@ -648,11 +638,11 @@ static int tree_layout(const sipa_tree_params* p, TreeLayout* l) {
   if (l->nsplit > 1) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     const int64_t rows = units * l->nsplit * l->rows;
-    SIPA_CHECK((int64_t)l->nsplit * l->rows * p->head_dim * 2 <= 0x7fffffff, SIPA_EINVAL, "split state too large");
+    SIPA_CHECK((int64_t)l->nsplit * l->rows * p->head_dim * 4 <= 0x7fffffff, SIPA_EINVAL, "split state too large");
     l->pm = up(units * 4);
     l->pl = l->pm + up(rows * 4);
     l->part = l->pl + up(rows * 4);
-    l->total = l->part + up(rows * p->head_dim * 2);
+    l->total = l->part + up(rows * p->head_dim * 4);
   }
   return SIPA_OK;
 }
@@ -770,7 +760,7 @@ extern "C" int32_t sipa_tree_attention(const sipa_tree_params* p, void* stream) 
   a.counters = (int*)ws;
   a.pm = (float*)(ws + l.pm);
   a.pl = (float*)(ws + l.pl);
-  a.part = (uint16_t*)(ws + l.part);
+  a.part = (float*)(ws + l.part);
   const int64_t side = 8 >> l.log_spread, rounds = ((int64_t)p->num_seqs * p->num_kv_heads + side - 1) / side;
   const dim3 grid((unsigned)(8 * rounds * l.groups * ((l.nsplit + (1 << l.log_spread) - 1) >> l.log_spread)));
   hipStream_t st = (hipStream_t)stream;
