@@ -574,8 +574,9 @@ __global__ void __launch_bounds__(64 * NC / CW * KH) prefill_mfma_bf16(const Pre
     // This split's state for column c, token r: m, l at slot 16 c + r, and the split's own output O / l (the
     // weighted mean of its V rows, so fp16 holds it to 2^-11 relative) at channels 16 dt + 4 q4 .. of that row:
     // half the bytes of unnormalised fp32 partials, which the merge reads back in one or two memory round trips.
-    // A row whose largest |O / l| reaches 2^15 (V values beyond fp16's range) is stored times 2^-e, so that it
-    // stays below 65504, with e in l's low mantissa bits; the merge scales the row back exactly.
+    // The row is stored times 2^-e, which brings its largest finite |O / l| between 2^14 and 2^15, whatever V's
+    // magnitude, with e in l's low mantissa bits; the merge scales the row back exactly. Values down to 2^-29 of that
+    // largest keep their 11 bits; an infinite channel stays one and leaves the others' values.
     const int64_t base = ((int64_t)u * a.nsplit + sp) * kSlots;
     const int split_bytes = kSlots * D * 2;
     const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
@@ -589,11 +590,14 @@ __global__ void __launch_bounds__(64 * NC / CW * KH) prefill_mfma_bf16(const Pre
       float big = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
-        big = vmax(big, vmax(vmax(fabsf(acc[ci][dt][0]), fabsf(acc[ci][dt][1])),
-                             vmax(fabsf(acc[ci][dt][2]), fabsf(acc[ci][dt][3]))));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = fabsf(acc[ci][dt][i]);
+          big = x < __builtin_huge_valf() ? vmax(big, x) : big;
+        }
       big = max_over_rows_swap(big * inv);
-      // big < 2^ex; e = ex - 15 keeps the row under 2^15 (inf and NaN rows keep e = 0 and stay inf and NaN)
-      const int e = big < 32768.f ? 0 : max(__builtin_amdgcn_frexp_expf(big) - 15, 0);
+      // big < 2^ex (ex 0 for big 0); from -100 on, which 2^-e / l and the merge's weights times 2^e are normal numbers for
+      const int e = max(__builtin_amdgcn_frexp_expf(big) - 15, -100);
       const float inv_e = __builtin_amdgcn_ldexpf(inv, -e);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -603,9 +607,9 @@ __global__ void __launch_bounds__(64 * NC / CW * KH) prefill_mfma_bf16(const Pre
                                               kAuxSc1);
       }
       if (q4 == 0) {
-        // e (at most 113) in the low 8 bits of l's mantissa: l changes by less than 2^-15 relative
+        // e (-100 .. 113) in the low 8 bits of l's mantissa: l changes by less than 2^-15 relative
         store_coherent(a.pm + base + slot, m_run[ci]);
-        store_coherent(a.pl + base + slot, __uint_as_float((__float_as_uint(lsum[ci]) & ~0xffu) | (uint32_t)e));
+        store_coherent(a.pl + base + slot, __uint_as_float((__float_as_uint(lsum[ci]) & ~0xffu) | ((uint32_t)e & 0xffu)));
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(64 * NC / CW * KH) prefill_mfma_bf16(const Pre
                                                      mrows, (j * kSlots + slot) * 4, 0, AUX));
               const uint32_t lb = __builtin_amdgcn_raw_buffer_load_b32(lrows, (j * kSlots + slot) * 4, 0, AUX);
               lj[uu] = __uint_as_float(lb & ~0xffu);
-              ej[uu] = (int)(lb & 0xffu);
+              ej[uu] = (int8_t)(lb & 0xffu);
 #pragma unroll
               for (int qd = 0; qd < CB / 4; ++qd)
                 oj[uu][qd] = __builtin_amdgcn_raw_buffer_load_b64(
