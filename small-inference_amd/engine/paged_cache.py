@@ -169,6 +169,7 @@ class TreeMetadata(PagedMetadata):
     parents: list[list[int]]  # per sequence: each node's parent among the nodes before it, -1 for none
     masks: torch.Tensor  # [T, words] int64: each node's ancestors and itself as bits (engine.hip_tree)
     query_starts_t: torch.Tensor  # [num_seqs + 1] int32 on the device
+    attended: bool = False  # a layer has attended over the trees: the nodes' K in the cache is rotated for their positions
 
     @property
     def max_nodes(self) -> int:
@@ -386,9 +387,11 @@ class PagedKVCache:
         """Attention of every sequence in the forward over its own context. Returns [T, Hq * d]."""
         m = self.meta
         T, Hq, d = q.shape
-        if isinstance(m, TreeMetadata) and self.attn_backend in KERNEL_BACKENDS and \
-                tree_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads):
-            return self._attend_tree(layer, q, scale)
+        if isinstance(m, TreeMetadata):
+            m.attended = True
+            if self.attn_backend in KERNEL_BACKENDS and \
+                    tree_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads):
+                return self._attend_tree(layer, q, scale)
         if self._decode is None:
             if self._prefill_launch is not None:  # only multi-token rows, all on the prefill kernel
                 out = torch.empty(T, Hq, d, device=q.device, dtype=q.dtype)
@@ -443,9 +446,11 @@ class PagedKVCache:
 
     def commit(self, accepted: list[list[int]], meta: TreeMetadata | None = None) -> None:
         """Keep the accepted nodes of a forward over drafted trees (meta None: of the last one): node accepted[i][j] of
-        sequence i moves to its position start + j in every layer. Each list ascends, as a path from a root does. The caller
-        then gives up the other nodes' slots with manager.truncate(seq_id, start + len(accepted[i])). No counterpart in the
-        reference."""
+        sequence i moves to its position start + j in every layer. Each list is a path: a root, then a child of the node
+        before it each time (ValueError for another set: its K, rotated for the tree's positions, would not fit its new
+        ones). Where no layer has attended over the trees, so that the nodes' rows are the caller's own, it need only ascend.
+        The caller then gives up the other nodes' slots with manager.truncate(seq_id, start + len(accepted[i])). No
+        counterpart in the reference."""
         m = self.meta if meta is None else meta
         if not isinstance(m, TreeMetadata):
             raise ValueError("commit needs the metadata of a forward over drafted trees")
@@ -454,6 +459,8 @@ class PagedKVCache:
         for i, (path, parents) in enumerate(zip(accepted, m.parents)):
             if any(b <= a for a, b in zip([-1, *path], path)) or (path and path[-1] >= len(parents)):
                 raise ValueError(f"sequence {i}: accepted nodes {path} must ascend within its {len(parents)} nodes")
+            if m.attended and any(parents[b] != a for a, b in zip([-1, *path], path)):
+                raise ValueError(f"sequence {i}: accepted nodes {path} are no path from a root, each a child of the one before")
         most = max(map(len, accepted))
         if most == 0:
             return
