@@ -154,11 +154,17 @@ def commit_tokens(k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, 
         _hip.check(rc, "commit_tokens")
 
 
-def tree_supported(q_dtype: torch.dtype, pool_dtype: torch.dtype, block_size: int, head_dim: int, group: int) -> bool:
+def tree_supported(q_dtype: torch.dtype, pool_dtype: torch.dtype, block_size: int, head_dim: int, group: int,
+                   max_context: int = 1, max_nodes: int = 1) -> bool:
     """Whether the tree attention kernel covers this shape (bf16 q; bf16 or INT8 per-token pool; blocks of 16, 32 or 64
-    tokens, head_dim 64/128, GQA group <= 64); the caches use the gather path otherwise."""
-    return (q_dtype == torch.bfloat16 and pool_dtype in (torch.bfloat16, torch.int8) and block_size in (16, 32, 64) and
-            head_dim in (64, 128) and group <= 64)
+    tokens, head_dim 64/128, GQA group <= 64, trees of up to MAX_NODES nodes, contexts up to 2097152 tokens for up to 64 rows
+    of query heads, 655360 (head_dim 64) or 1179648 (128) for more: the splits that the kernel merges, of 16384 keys each);
+    the caches use the gather path otherwise."""
+    if not (q_dtype == torch.bfloat16 and pool_dtype in (torch.bfloat16, torch.int8) and block_size in (16, 32, 64) and
+            head_dim in (64, 128) and group <= 64 and max_nodes <= MAX_NODES):
+        return False
+    splits = 128 if max_nodes * group <= 64 else 40 if head_dim == 64 else 72
+    return max_context <= splits * 16384
 
 
 class TreePlan:

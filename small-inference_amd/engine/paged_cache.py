@@ -389,8 +389,8 @@ class PagedKVCache:
         T, Hq, d = q.shape
         if isinstance(m, TreeMetadata):
             m.attended = True
-            if self.attn_backend in KERNEL_BACKENDS and \
-                    tree_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads):
+            if self.attn_backend in KERNEL_BACKENDS and (self._tree_plan is not None or tree_supported(
+                    q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads, max(m.context_lens), m.max_nodes)):
                 return self._attend_tree(layer, q, scale)
         if self._decode is None:
             if self._prefill_launch is not None:  # only multi-token rows, all on the prefill kernel
