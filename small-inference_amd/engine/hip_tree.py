@@ -207,7 +207,7 @@ class TreePlan:
         self.shape, self.pool_shape, self.device = (T, Hq, D), tuple(k_cache.shape), q.device
         self._pool_strides = (N * B * D, B * D, D, 1)  # of a contiguous layer
         self._keep = (block_tables, context_lens, query_starts, masks)
-        self._quantized = quant is not None
+        self._quantized, self._own_quant = quant is not None, quant
         p = self.params = _hip.TreeParams(
             struct_size=ctypes.sizeof(_hip.TreeParams), num_seqs=S, num_tokens=T, num_q_heads=Hq, num_kv_heads=Hkv,
             head_dim=D, block_size=B, num_blocks=N, max_context=max_context, max_nodes=max_nodes, words=masks.shape[1],
@@ -287,7 +287,7 @@ class TreePlan:
     def __call__(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, quant: QuantKV | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of q over one layer's pools (quant None: the plan's own scales). Returns out ([T, Hq, D] bf16)."""
-        self._bind(q, k_cache, v_cache, self._quant if quant is None else quant)
+        self._bind(q, k_cache, v_cache, self._own_quant if quant is None else quant)
         return self._run(out)
 
     def _run(self, out: torch.Tensor | None) -> torch.Tensor:
