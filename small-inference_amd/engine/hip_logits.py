@@ -17,6 +17,7 @@ that were accepted.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -34,7 +35,7 @@ class LogitsRules:
     bias_values fp32, with bias_starts int32 [S + 1]; grammar int32 [states, >= ceil(vocab / 32)], bit v % 32 of word v // 32
     set where the state allows token v. Tokens outside the vocabulary (-1 as padding) are ignored, starts
     are clamped to their lists. The tensors are read at
-    every apply(), so a program may write new values into them between steps."""
+    every apply(), so a program may write new values into them between steps. Threads may call apply() at the same time."""
 
     def __init__(self, vocab: int, num_seqs: int, *, history: torch.Tensor | None = None,
                  history_starts: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
@@ -45,6 +46,7 @@ class LogitsRules:
         if vocab < 1 or num_seqs < 1:
             raise ValueError(f"vocabulary {vocab}, {num_seqs} sequences")
         self.vocab, self.num_seqs = vocab, num_seqs
+        self._lock = threading.Lock()  # of the parameter block, from its filling to the launch
         S = num_seqs
 
         def check(t, dtype, n, what):
@@ -134,12 +136,12 @@ class LogitsRules:
         if R == 0:
             return out
         p = self._params
-        p.num_rows, p.dtype = R, _hip.dtype_code(logits.dtype)
-        p.words = 0 if masks is None else masks.shape[1]
-        p.logits, p.logits_stride, p.out, p.out_stride = logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0)
-        p.query_starts, p.tokens, p.masks = _hip.ptr(query_starts), _hip.ptr(tokens), _hip.ptr(masks)
-        p.grammar_rows = _hip.ptr(grammar_rows)
-        with _hip.on_device(dev):
+        with self._lock, _hip.on_device(dev):
+            p.num_rows, p.dtype = R, _hip.dtype_code(logits.dtype)
+            p.words = 0 if masks is None else masks.shape[1]
+            p.logits, p.logits_stride, p.out, p.out_stride = logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0)
+            p.query_starts, p.tokens, p.masks = _hip.ptr(query_starts), _hip.ptr(tokens), _hip.ptr(masks)
+            p.grammar_rows = _hip.ptr(grammar_rows)
             _hip.check(_hip.lib().sipa_adjust_logits(ctypes.byref(p), _hip.stream_of(logits)), "adjust_logits")
         return out
 

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
 from typing import NamedTuple
 
 import torch
@@ -178,7 +179,8 @@ class TreePlan:
     - n_s and the nodes in its mask; a row that sees nothing gets zeros. Rows behind query_starts[S] are left as they are.
 
     The split workspace is the plan's own: it is made for the stream (and the graph capture) of the call that needs it, so
-    plans, streams and graphs share none."""
+    plans, streams and graphs share none. Threads may call one plan at the same time: each call fills the parameter block and
+    launches under the plan's lock."""
 
     def __init__(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                  context_lens: torch.Tensor, query_starts: torch.Tensor, masks: torch.Tensor, scale: float, max_context: int,
@@ -222,6 +224,7 @@ class TreePlan:
             _hip.check(n, "tree attention")
         self._ws_bytes, self._counter_bytes = n, counters.value
         self._workspace = self._owner = None
+        self._lock = threading.Lock()
         self._bind(q, k_cache, v_cache, quant)
 
     def _bind_q(self, q: torch.Tensor) -> None:
@@ -273,22 +276,24 @@ class TreePlan:
                     t.stride()[1:] != self._pool_strides:
                 raise ValueError("the pools do not match the plan")
         self._check_quant(quant, k_pools.shape[:1])
-        self._bind_q(q)
-        p = self.params
-        p.k_cache, p.v_cache = _hip.layer_ptr(k_pools, layer), _hip.layer_ptr(v_pools, layer)
-        p.kv_stride_h, p.kv_stride_n = k_pools.stride(1), k_pools.stride(2)
-        self._k, self._v, self._quant = k_pools, v_pools, quant
-        if quant is not None:
-            ks, vs = quant.k_scale, quant.v_scale
-            self._bind_scales(_hip.layer_ptr(ks, layer), ks.dtype, ks.stride(), _hip.layer_ptr(vs, layer), vs.dtype,
-                              vs.stride())
-        return self._run(out)
+        with self._lock:
+            self._bind_q(q)
+            p = self.params
+            p.k_cache, p.v_cache = _hip.layer_ptr(k_pools, layer), _hip.layer_ptr(v_pools, layer)
+            p.kv_stride_h, p.kv_stride_n = k_pools.stride(1), k_pools.stride(2)
+            self._k, self._v, self._quant = k_pools, v_pools, quant
+            if quant is not None:
+                ks, vs = quant.k_scale, quant.v_scale
+                self._bind_scales(_hip.layer_ptr(ks, layer), ks.dtype, ks.stride(), _hip.layer_ptr(vs, layer), vs.dtype,
+                                  vs.stride())
+            return self._run(out)
 
     def __call__(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, quant: QuantKV | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of q over one layer's pools (quant None: the plan's own scales). Returns out ([T, Hq, D] bf16)."""
-        self._bind(q, k_cache, v_cache, self._own_quant if quant is None else quant)
-        return self._run(out)
+        with self._lock:
+            self._bind(q, k_cache, v_cache, self._own_quant if quant is None else quant)
+            return self._run(out)
 
     def _run(self, out: torch.Tensor | None) -> torch.Tensor:
         p = self.params
