@@ -214,11 +214,13 @@ class DecodeGraphRunner:
              grammar_rows: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [len(seq_ids), vocab] of one decode step: row i is sequence seq_ids[i]'s newest token
         (input_ids[i], at position manager.seq_len(s) - 1; the caller has appended its slot). graph=False runs the
-        same static-shape step eagerly (the graph's reference). rules (of these sequences, in this order): applied to the
-        step's logits after the replay, into a tensor of their own; their histories hold the new tokens too."""
+        same static-shape step eagerly (the graph's reference). rules (of exactly these sequences, in this order): applied
+        to the step's logits after the replay, into a tensor of their own; their histories hold the new tokens too."""
         b = len(seq_ids)
         if input_ids.shape != (b,):
             raise ValueError("one input id per sequence")
+        if rules is not None:
+            rules.check_sequences(b)
         if len(set(seq_ids)) != b:
             raise ValueError("a decode step holds each sequence once")
         bucket = self._bucket(b)

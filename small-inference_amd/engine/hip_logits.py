@@ -94,12 +94,17 @@ class LogitsRules:
         if grammar is not None:
             p.grammar_stride, p.grammar_states = grammar.stride(0), grammar.shape[0]
 
+    def check_sequences(self, n: int) -> None:
+        """ValueError unless these are the rules of n sequences: rows of other batches would take other sequences' rules."""
+        if n != self.num_seqs:
+            raise ValueError(f"rules of {self.num_seqs} sequences for a batch of {n}")
+
     def apply(self, logits: torch.Tensor, *, query_starts: torch.Tensor | None = None, tokens: torch.Tensor | None = None,
               masks: torch.Tensor | None = None, grammar_rows: torch.Tensor | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
         """The adjusted logits [R, vocab], in the logits' type (bf16, fp16 or fp32), in one launch (sipa_adjust_logits).
 
-        Row r is of sequence r, or with query_starts int32 [S + 1] of the sequence whose rows query_starts[s] ..
+        Row r is of sequence r (there may be fewer rows than sequences), or with query_starts int32 [S + 1] of the sequence whose rows query_starts[s] ..
         query_starts[s + 1] - 1 it is among; rows behind the last sequence's are copied as they are. tokens int64 [R] and
         masks int64 [R, words] (engine.hip_tree.tree_maps) give each row its path: the tokens of the nodes of its sequence
         whose bits its mask has. grammar_rows int32 [R]: each row's grammar state, -1 for none. out may be logits itself.

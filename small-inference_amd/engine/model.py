@@ -121,6 +121,8 @@ class Qwen2Model:
         trees) for a packed batch described by meta (positions must be meta.positions). rules: applied to them, with
         grammar_rows the grammar state of each row returned; a drafted node's path counts as generated, other rows see the
         rules' histories as they are."""
+        if rules is not None:
+            rules.check_sequences(meta.num_seqs)
         cache.begin(input_ids.shape[0], meta)
         x = self.embed[input_ids]
         rot = self.rotary.rows(positions, x.dtype)
