@@ -136,7 +136,7 @@ class Qwen2Model:
         if rules is None:
             return logits
         if tree:
-            return rules.apply(logits, query_starts=meta.query_starts_t, tokens=input_ids, masks=meta.masks,
+            return rules.apply(logits, query_starts=meta.query_starts_t, tokens=input_ids.long().contiguous(), masks=meta.masks,
                                grammar_rows=grammar_rows)
         starts = None
         if logits.shape[0] != meta.num_seqs:

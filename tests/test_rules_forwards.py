@@ -56,3 +56,18 @@ def test_runner_steps_with_the_rules_of_other_sequences_are_refused():
         runner.step([0, 2], ids[:2], rules=rules[3])
     runner.step([0, 2], ids[:2], rules=rules[2])
     runner.close()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_paths_of_token_ids_in_any_integer_layout(device):
+    """Token ids that the embedding takes, int32 or strided ones, are a tree's path too."""
+    cfg, m, model, cache, rules = start(device)
+    lens = [m.seq_len(s) for s in range(3)]
+    for s in range(3):
+        m.append_slots(s, 4)
+    meta = build_tree_metadata(m, [(s, lens[s], [-1, 0, 1, 0]) for s in range(3)], device)
+    ids = torch.arange(12, device=device) // 2
+    want = model.forward(ids, meta.positions, cache, meta, rules=rules[3])
+    assert not torch.equal(want, model.forward(ids, meta.positions, cache, meta))
+    for other in (ids.int(), torch.stack([ids, ids], 1)[:, 0], torch.stack([ids.int(), ids.int()], 1)[:, 1]):
+        assert torch.equal(model.forward(other, meta.positions, cache, meta, rules=rules[3]), want)
