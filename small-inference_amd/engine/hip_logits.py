@@ -19,11 +19,29 @@ from __future__ import annotations
 import ctypes
 import threading
 
+import numpy as np
 import torch
 
 from . import _hip
 
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _overlap(logits: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether out [R, V] has rows over each other, or over logits' [R, V] other than as the same rows."""
+    R, V = out.shape
+    size, so, sl = out.element_size(), out.stride(0), logits.stride(0)
+    if R > 1 and so < V:
+        return True
+    at, start = out.data_ptr(), logits.data_ptr()
+    if at >= start + ((R - 1) * sl + V) * size or start >= at + ((R - 1) * so + V) * size or R * V == 0:
+        return False
+    if at == start and (R == 1 or so == sl):
+        return False
+    o, l = at + np.arange(R) * (so * size), start + np.arange(R) * (sl * size)
+    i = np.searchsorted(l, o)  # each row of out against the rows of logits that start before and behind it
+    behind, before = l[np.minimum(i, R - 1)], l[np.maximum(i - 1, 0)]
+    return bool((np.abs(behind - o) < V * size).any() or (np.abs(before - o) < V * size).any())
 
 
 class LogitsRules:
@@ -107,8 +125,8 @@ class LogitsRules:
         Row r is of sequence r (there may be fewer rows than sequences), or with query_starts int32 [S + 1] of the sequence whose rows query_starts[s] ..
         query_starts[s + 1] - 1 it is among; rows behind the last sequence's are copied as they are. tokens int64 [R] and
         masks int64 [R, words] (engine.hip_tree.tree_maps) give each row its path: the tokens of the nodes of its sequence
-        whose bits its mask has. grammar_rows int32 [R]: each row's grammar state, -1 for none. out may be logits itself.
-        CPU tensors are computed by torch operations."""
+        whose bits its mask has. grammar_rows int32 [R]: each row's grammar state, -1 for none. out may be logits itself,
+        and must not overlap it otherwise. CPU tensors are computed by torch operations."""
         if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.dtype not in DTYPES or \
                 (self.vocab > 1 and logits.stride(1) != 1):
             raise ValueError(f"logits must be [rows, {self.vocab}] in bf16, fp16 or fp32 with a contiguous last dim")
@@ -130,6 +148,8 @@ class LogitsRules:
         if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or
                                 (self.vocab > 1 and out.stride(1) != 1)):
             raise ValueError("out must be as logits, with a contiguous last dim")
+        if out is not None and _overlap(logits, out):
+            raise ValueError("out's rows overlap each other or other rows of the logits; it may be logits itself or lie beside them")
         dev = logits.device
         if self.device is not None and self.device != dev:
             raise ValueError(f"logits on {dev}, rules on {self.device}")
