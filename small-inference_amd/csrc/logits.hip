@@ -36,11 +36,10 @@ struct LogitsArgs {
   const int32_t* grows;
 };
 
-constexpr uint32_t kSeen = 0x80000000u;    // in the prompt
-constexpr uint32_t kBiased = 0x40000000u;  // in the bias list
-constexpr uint32_t kPath = 0x20000000u;    // some node's token
-constexpr uint32_t kCount = 0x1fffffffu;   // times among the generated tokens
-constexpr int kLogitThreads = 256, kMaxNodes = 256, kMaxHits = 256;
+constexpr uint32_t kSeen = 0x80000000u;   // in the prompt
+constexpr uint32_t kPath = 0x40000000u;   // some node's token
+constexpr uint32_t kCount = 0x3fffffffu;  // times among the generated tokens
+constexpr int kLogitThreads = 256, kMaxNodes = 256, kTurns = 512;
 
 template <int DT>
 struct LogitsType;  // a row's element: bits, and how many make 16 bytes
@@ -77,9 +76,10 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
     uint32_t w[4];
   };
   __shared__ __align__(16) uint32_t cnt[TILE];
+  __shared__ __align__(16) float sum[TILE];  // of the sequence's biases
+  __shared__ uint32_t turn[kTurns];  // of the entries for tokens i, i + kTurns, ..: whose turn it is
   __shared__ int32_t node_token[kMaxNodes];  // within the tile, or -1
-  __shared__ int32_t hit_entry[kMaxHits], hit_token[kMaxHits];
-  __shared__ int32_t num_hits, has_path;
+  __shared__ int32_t has_path, open_round;
   const int tid = threadIdx.x, s = blockIdx.x, v0 = (int)blockIdx.y * TILE, i0 = tid * E, n = min(TILE, a.V - v0);
   const bool behind = s == a.S;  // rows behind the last sequence's: copied
   const int first = a.qs != nullptr ? (behind ? max(a.qs[a.S], 0) : max(a.qs[s], 0)) : s;
@@ -105,25 +105,28 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
   // A token's rule is l k + c, k = 1 / rho or rho by the logit's sign where it has been seen, else 1. (c = -0 where there is
   // nothing to add, so that the other logits keep their bits.)
   float inv_rho = 1.f, rho = 1.f, alpha = 0.f, beta = 0.f;
+  uint32_t b0 = 0, b1 = 0;  // the sequence's biases
   uint32_t any = 0;
-  float c[E], bias[E];
+  float c[E];
   bool seen[E];
   auto rules = [&]() {
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
       const uint4 w4 = *(const uint4*)(cnt + i0 + e);
+      const float4 b4 = b0 < b1 ? *(const float4*)(sum + i0 + e) : float4{-0.f, -0.f, -0.f, -0.f};
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float made = (float)(w[x] & kCount);
-        any |= w[x];
+        any |= w[x] | (__float_as_uint(bias[x]) != 0x80000000u);
         seen[e + x] = (w[x] & (kSeen | kCount)) != 0;
-        c[e + x] = (w[x] & kCount ? -alpha * made - beta : -0.f) + bias[e + x];
+        c[e + x] = (w[x] & kCount ? -alpha * made - beta : -0.f) + bias[x];
       }
     }
   };
 #pragma unroll
-  for (int e = 0; e < E; ++e) c[e] = bias[e] = -0.f, seen[e] = false;
+  for (int e = 0; e < E; ++e) c[e] = -0.f, seen[e] = false;
   int nodes = 0;
   if (!behind) {
     const bool seq_path = a.tokens != nullptr;
@@ -131,11 +134,17 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
     if (a.freq != nullptr) alpha = a.freq[s];
     if (a.pres != nullptr) beta = a.pres[s];
     inv_rho = 1.f / rho;
-    const int b0 = a.bstarts != nullptr ? max(a.bstarts[s], 0) : 0, b1 = a.bstarts != nullptr ? min(a.bstarts[s + 1], a.nbias) : 0;
-    *(uint4*)(cnt + 4 * tid) = uint4{0, 0, 0, 0};
-    if (E == 8) *(uint4*)(cnt + 4 * tid + 4 * THR) = uint4{0, 0, 0, 0};
-    if (tid == 0) num_hits = has_path = 0;
+    if (a.bstarts != nullptr) b0 = max(a.bstarts[s], 0), b1 = max(min(a.bstarts[s + 1], a.nbias), 0);
+#pragma unroll
+    for (int i = 4 * tid; i < TILE; i += 4 * THR) {
+      *(uint4*)(cnt + i) = uint4{0, 0, 0, 0};
+      if (a.bstarts != nullptr) *(float4*)(sum + i) = float4{-0.f, -0.f, -0.f, -0.f};
+    }
+    if (a.bstarts != nullptr)
+      for (int i = tid; i < kTurns; i += THR) turn[i] = 0;
+    if (tid == 0) has_path = open_round = 0;
     __syncthreads();
+    int entry = b0 < b1 ? a.btok[min(b0 + tid, b1 - 1)] : 0;
     if (a.history != nullptr) {
       const int64_t h0 = min(max(a.hstarts[s], (int64_t)0), a.hsize), h1 = min(a.hstarts[s + 1], a.hsize);
       const int64_t made = h0 + (a.prompt != nullptr ? max(a.prompt[s], 0) : 0);
@@ -169,36 +178,33 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
         }
       }
     }
-    if (a.bstarts != nullptr)
-      for (int b = b0 + tid; b < b1; b += THR) {
-        const uint32_t at = (uint32_t)a.btok[b] - (uint32_t)v0;
-        if (at >= (uint32_t)n || a.btok[b] < 0) continue;
-        atomicOr(&cnt[at], kBiased);
-        const int hit = atomicAdd(&num_hits, 1);
-        if (hit < kMaxHits) hit_entry[hit] = b, hit_token[hit] = (int32_t)at;
-      }
-    __syncthreads();
-    rules();
-    if (any & kBiased) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (!(cnt[i0 + e] & kBiased)) continue;
-        if (num_hits <= kMaxHits) {  // the hits stand in any order: the token's entries from the first of the list on
-          for (int last = -1;;) {
-            int next = 0x7fffffff;
-            for (int i = 0; i < num_hits; ++i)
-              if (hit_token[i] == i0 + e && hit_entry[i] > last) next = min(next, hit_entry[i]);
-            if (next == 0x7fffffff) break;
-            bias[e] += a.bval[next];
-            last = next;
-          }
-        } else {
-          for (int b = b0; b < b1; ++b)
-            if (a.btok[b] == v0 + i0 + e) bias[e] += a.bval[b];
+    // The biases in the list's order, THR entries at a time: of those for one token the first takes its turn (the largest
+    // number), then the next, until none is left: as many rounds as some token has entries among them, mostly one (tokens
+    // kTurns apart take turns too). One row and a run of 4096 neighbouring tokens: 9 us, 20000 of them 20; each biased token's
+    // thread searching the list took 1950 for 4096.
+    int round = 0;
+    for (uint32_t at = b0; at < b1; at += THR) {
+      const uint32_t i = (uint32_t)entry - (uint32_t)v0, number = THR - tid;
+      bool open = i < (uint32_t)n && at + tid < b1;
+      if (at + THR < b1) entry = a.btok[min(at + THR + tid, b1 - 1)];
+      for (;;) {
+        ++round;
+        if (open) {
+          open_round = round;
+          atomicMax(&turn[i % kTurns], number);
         }
+        __syncthreads();
+        if (open_round != round) break;  // uniform: no entry was open (a thread that is ahead may have written the next round)
+        if (open && turn[i % kTurns] == number) {  // (the others find this number, or the 0 after it)
+          sum[i] += a.bval[at + tid];
+          turn[i % kTurns] = 0;
+          open = false;
+        }
+        __syncthreads();
       }
-      rules();
     }
+    if (b0 >= b1) __syncthreads();  // (else the loop's last)
+    rules();
   }
   const bool path = !behind && a.tokens != nullptr && has_path;  // uniform
   const int token = path && tid < nodes ? node_token[tid] : -1;
