@@ -576,7 +576,8 @@ int32_t sipa_silu_mul(const void* gate_up, int64_t gu_stride, void* out, int64_t
  *   for every sequence: context_lens (start + count), last_rows (query_starts[s + 1] - 1) and block_tables
  *   [s, :out_width], its first ceil(context / B) table entries, then -1.
  * tables, rows and starts are as for sipa_paged_metadata. Rows of the outputs past the last sequence's nodes (num_tokens
- * may be a capacity) are left as they are. A parent that is not smaller than its node ends the node's chain, as -1 does;
+ * may be a capacity) are left as they are, or with fill_rest given position 0, the slot rest_slot and no ancestors: a step
+ * whose every row is stored, as a captured one's is, needs a slot for them that no sequence has. A parent that is not smaller than its node ends the node's chain, as -1 does;
  * nodes past 64 words have no bit. num_seqs <= 8192.
  */
 typedef struct sipa_tree_maps_params {
@@ -598,6 +599,8 @@ typedef struct sipa_tree_maps_params {
   int32_t* context_lens;  /* [S] */
   int32_t* block_tables;  /* [S, out_width] */
   uint64_t* ancestors;    /* [num_tokens, words] */
+  int32_t fill_rest;      /* 0: rows past the last sequence's nodes are left as they are */
+  int64_t rest_slot;      /* with fill_rest: their slot, not negative */
 } sipa_tree_maps_params;
 
 int32_t sipa_tree_maps(const sipa_tree_maps_params* p, void* stream);

@@ -28,6 +28,8 @@ struct TreeMapsArgs {
   int32_t* ctx;
   int32_t* bt;
   uint64_t* ancestors;
+  bool fill_rest;
+  int64_t rest_slot;
 };
 
 __device__ __forceinline__ int32_t tree_table_entry(const TreeMapsArgs& a, int s, int64_t col) {
@@ -63,7 +65,15 @@ __global__ void __launch_bounds__(256) tree_maps_kernel(const TreeMapsArgs a) {
   __syncthreads();
   if ((int)blockIdx.x < a.token_groups) {
     const int t = (int)blockIdx.x * 256 + tid;
-    if (t >= qs[a.S]) return;
+    if (t >= qs[a.S]) {
+      if (!a.fill_rest || t >= a.T) return;
+      for (int w = 0; w < a.words; ++w) a.ancestors[(int64_t)t * a.words + w] = 0;
+      a.positions[t] = 0;
+      a.slots[t] = a.rest_slot;
+      a.slot_blocks[t] = a.rest_slot / a.B;
+      a.slot_offsets[t] = a.rest_slot % a.B;
+      return;
+    }
     int lo = 0, hi = a.S;  // the last s with qs[s] <= t: sequences without nodes share their successor's start
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -184,7 +194,10 @@ extern "C" int32_t sipa_tree_maps(const sipa_tree_maps_params* p, void* stream) 
   SIPA_CHECK(p->tables && p->rows && p->starts && p->counts && p->parents && p->positions && p->slots &&
                  p->slot_blocks && p->slot_offsets && p->last_rows && p->query_starts && p->context_lens &&
                  p->block_tables && p->ancestors, SIPA_EINVAL, "NULL pointer");
+  SIPA_CHECK(!p->fill_rest || p->rest_slot >= 0, SIPA_EINVAL, "slot %lld for the rows behind", (long long)p->rest_slot);
   TreeMapsArgs a;
+  a.fill_rest = p->fill_rest != 0;
+  a.rest_slot = p->rest_slot;
   a.tables = p->tables;
   a.table_stride = p->table_stride;
   a.table_rows = p->table_rows;

@@ -130,7 +130,8 @@ class TreeMapsParams(ctypes.Structure):
         ("words", i32), ("table_rows", i32), ("table_width", i32), ("table_stride", i64),
         ("tables", vp), ("rows", vp), ("starts", vp), ("counts", vp), ("parents", vp),
         ("positions", vp), ("slots", vp), ("slot_blocks", vp), ("slot_offsets", vp), ("last_rows", vp),
-        ("query_starts", vp), ("context_lens", vp), ("block_tables", vp), ("ancestors", vp),
+        ("query_starts", vp), ("context_lens", vp), ("block_tables", vp), ("ancestors", vp), ("fill_rest", i32),
+        ("rest_slot", i64),
     ]
 
 

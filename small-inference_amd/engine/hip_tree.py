@@ -50,7 +50,7 @@ _I32, _I64 = torch.int32, torch.int64
 _split = torch.split_with_sizes
 # sipa_tree_maps_params and sipa_commit_params as bytes (native alignment): a third of the time that filling a ctypes
 # structure takes, in calls whose kernels take a few microseconds
-_MAPS = struct.Struct("8iq14Q")
+_MAPS = struct.Struct("8iq14Qiq")
 _COMMIT = struct.Struct("9i2Q4q2Q4qQq2QqQ")
 assert _MAPS.size == ctypes.sizeof(_hip.TreeMapsParams) and _COMMIT.size == ctypes.sizeof(_hip.CommitParams)
 
@@ -61,14 +61,16 @@ def _vector(t: torch.Tensor, n: int, what: str) -> None:
 
 
 def tree_maps(tables: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, parents: torch.Tensor,
-              block_size: int, width: int, max_nodes: int, out: TreeMaps | None = None) -> TreeMaps:
+              block_size: int, width: int, max_nodes: int, out: TreeMaps | None = None, rest_slot: int | None = None) -> TreeMaps:
     """A forward's metadata from device lengths, in one launch (sipa_tree_maps).
 
     tables [rows, columns] int32: persistent block tables, one row per live sequence (engine.device_tables); rows, starts,
     counts [S] int32: each sequence's table row, cached tokens and nodes; parents [T] int32: each node's parent within its
     sequence, -1 for none, sequences one after the other. width: columns of the packed tables, max_nodes: the largest
     count, both known to the host. T may be more than the counts sum to (a captured step's capacity): rows behind the last
-    sequence are left as they are. out: tensors of an earlier call of the same sizes, written again.
+    sequence are left as they are (in tensors made here: undefined, in out: an earlier step's), so none may be stored or
+    looked up; with rest_slot, a slot that no sequence has, they get it, position 0 and no ancestors, and a step may store and
+    attend all T rows. out: tensors of an earlier call of the same sizes, written again.
     """
     S, T, words = counts.shape[0], parents.shape[0], mask_words(max_nodes)
     _vector(rows, S, "rows"), _vector(starts, S, "starts"), _vector(counts, S, "counts"), _vector(parents, T, "parents")
@@ -78,6 +80,8 @@ def tree_maps(tables: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, co
         raise ValueError("tables must be int32 [rows, columns] with contiguous rows")
     if S < 1 or T < 1 or block_size < 1 or width < 1:
         raise ValueError(f"{S} sequences, {T} nodes, block size {block_size}, width {width}")
+    if rest_slot is not None and rest_slot < 0:
+        raise ValueError(f"rest_slot {rest_slot}")
     _hip.require_gpu(tables, rows, starts, counts, parents)
     dev = tables.device
     if out is None:
@@ -97,7 +101,8 @@ def tree_maps(tables: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, co
         _hip.require_gpu(tables, *out)
         at = tuple(t.data_ptr() for t in out)
     p = _MAPS.pack(_MAPS.size, S, T, block_size, width, words, table_rows, columns, table_stride, tables.data_ptr(),
-                   rows.data_ptr(), starts.data_ptr(), counts.data_ptr(), parents.data_ptr(), *at)
+                   rows.data_ptr(), starts.data_ptr(), counts.data_ptr(), parents.data_ptr(), *at, rest_slot is not None,
+                   rest_slot or 0)
     with _hip.on_device(dev):
         rc = _hip.lib().sipa_tree_maps(p, _hip.stream_of(tables))
     if rc:
