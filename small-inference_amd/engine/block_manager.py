@@ -36,6 +36,7 @@ class BlockManager:
         self._arrays: dict[int, np.ndarray] = {}
         self._free_listeners: list[Callable[[list[int]], None]] = []
         self._table_listeners: list[Callable[[int, int], None]] = []
+        self._truncate_checks: list[Callable[[int], None]] = []
 
     # ---- queries -------------------------------------------------------------------------------------------------
 
@@ -107,6 +108,10 @@ class BlockManager:
         """Call fn(blocks) with the blocks each free() returns to the stack."""
         self._free_listeners.append(fn)
 
+    def add_truncate_check(self, fn: Callable[[int], None]) -> None:
+        """Call fn(block) before a truncate() that keeps part of the tokens of a sequence's `block`; an exception refuses it."""
+        self._truncate_checks.append(fn)
+
     def add_table_listener(self, fn: Callable[[int, int], None]) -> None:
         """Call fn(seq_id, first) when a sequence's table is created (first = 0) or gains blocks from index first
         on, and fn(seq_id, -1) when the sequence is freed (no counterpart in the reference: device-side copies
@@ -161,11 +166,14 @@ class BlockManager:
 
     def truncate(self, seq_id: int, n_tokens: int) -> None:
         """Keep the first n_tokens of seq_id (drafted tokens that were not accepted are given up); the blocks past them
-        return to the stack, last block first, and free listeners hear of them. Not for an int8-kchannel cache, which cannot
-        take a quantized block back in part. No counterpart in the reference."""
+        return to the stack, last block first, and free listeners hear of them. An int8-kchannel cache refuses to keep part of
+        a block that it has quantized. No counterpart in the reference."""
         if not 0 <= n_tokens <= self._lengths[seq_id]:
             raise ValueError(f"sequence {seq_id} holds {self._lengths[seq_id]} tokens, {n_tokens} to keep")
         table, keep = self._tables[seq_id], self.blocks_for(n_tokens)
+        if n_tokens % self.block_size and n_tokens < self._lengths[seq_id]:
+            for fn in self._truncate_checks:
+                fn(table[keep - 1])
         self._lengths[seq_id] = n_tokens
         released = table[keep:][::-1]
         del table[keep:]

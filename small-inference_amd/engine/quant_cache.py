@@ -80,6 +80,12 @@ class StagingBook:
             self.assign([block])
         return self.slot_of[block]
 
+    def check_truncate(self, block: int) -> None:
+        """ValueError for a block that is to keep part of its tokens but is no longer staged: its bf16 rows are gone."""
+        if block not in self.slot_of:
+            raise ValueError(f"int8-kchannel: block {block} is quantized and cannot keep part of its tokens; truncate to a "
+                             f"multiple of the block size or within the staged last block")
+
     def release(self, blocks) -> None:
         """Blocks that left staging (quantized into the pool, or freed by the block manager) return their slots,
         in the order given; blocks without a slot are ignored."""
@@ -165,6 +171,7 @@ class QuantPagedKVCache(PagedKVCache):
             self._book = StagingBook(n_stage)
             self._stage_of, self._free_stage = self._book.slot_of, self._book.free
             manager.add_free_listener(self._book.release)
+            manager.add_truncate_check(self._book.check_truncate)
 
     def _allocate(self, shape: tuple, device: str | torch.device, dtype: torch.dtype) -> None:
         """int8 K/V, fp16 scales, and (format B) the bf16 staging slots; all zero-initialised."""
