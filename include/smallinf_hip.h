@@ -643,8 +643,8 @@ int32_t sipa_commit_tokens(const sipa_commit_params* p, void* stream);
  *   l = l + the sum of the values that the sequence's bias list gives v, added up in the list's order
  *   l = -inf                                                 where the row has a grammar state whose bit v is 0
  * rounded once to the logits' type. out may be logits itself. Rows belong to sequences by query_starts [S + 1] (row r to
- * the sequence with query_starts[s] <= r < query_starts[s + 1]), or row r to sequence r where it is NULL. Rows behind the
- * last sequence's are copied as they are. Tokens outside [0, vocab) in the lists, and -1 as padding, are ignored. NULL
+ * the sequence with query_starts[s] <= r < query_starts[s + 1]), or row r to sequence r where it is NULL. Rows before the
+ * first sequence's and behind the last one's are copied as they are. Tokens outside [0, vocab) in the lists, and -1 as padding, are ignored. NULL
  * pointers leave their rule out: history (all three penalties then see the path alone), prompt_lens (0), repetition (1),
  * frequency, presence (0), tokens and masks (no path), bias_starts, grammar_rows. A grammar row outside [0, states) leaves
  * its row free.

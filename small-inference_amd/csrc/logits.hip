@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits_kernel(const Logi
   __shared__ int32_t node_token[kMaxNodes];  // within the tile, or -1
   __shared__ int32_t has_path, open_round;
   const int tid = threadIdx.x, s = blockIdx.x, v0 = (int)blockIdx.y * TILE, i0 = tid * E, n = min(TILE, a.V - v0);
-  const bool behind = s == a.S;  // rows behind the last sequence's: copied
-  const int first = a.qs != nullptr ? (behind ? max(a.qs[a.S], 0) : max(a.qs[s], 0)) : s;
-  const int end = a.qs == nullptr ? (behind ? 0 : min(s + 1, a.R)) : behind ? a.R : min(a.qs[s + 1], a.R);
+  const bool behind = s >= a.S;  // (S, S + 1) rows behind the last sequence's and before the first one's: copied
+  const int first = a.qs == nullptr ? s : s == a.S + 1 ? 0 : max(a.qs[s], 0);
+  const int end = a.qs == nullptr ? min(s + 1, a.R) : s == a.S ? a.R : min(a.qs[s > a.S ? 0 : s + 1], a.R);
   const int r0 = first + (int)blockIdx.z;
   if (r0 >= end) return;
   const int left = n - i0;  // the thread's tokens: E of them, fewer at the vocabulary's end
@@ -279,7 +279,7 @@ static void launch_logits(const LogitsArgs& a, hipStream_t st) {
   const int64_t tiles = (a.V + TILE - 1) / TILE;
   const int64_t per = (a.R + a.S - 1) / a.S;  // rows of a sequence on average
   const int64_t z = std::max<int64_t>(1, std::min<int64_t>((per + 2) / 3, 5000 / (tiles * a.S)));
-  const dim3 grid((unsigned)(a.S + (a.qs != nullptr)), (unsigned)tiles, (unsigned)z);  // frequent tokens first
+  const dim3 grid((unsigned)a.S + (a.qs != nullptr ? 2 : 0), (unsigned)tiles, (unsigned)z);  // frequent tokens first
   hipLaunchKernelGGL((adjust_logits_kernel<DT>), grid, dim3(kLogitThreads), 0, st, a);
 }
 

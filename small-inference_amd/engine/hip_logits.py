@@ -122,11 +122,12 @@ class LogitsRules:
               out: torch.Tensor | None = None) -> torch.Tensor:
         """The adjusted logits [R, vocab], in the logits' type (bf16, fp16 or fp32), in one launch (sipa_adjust_logits).
 
-        Row r is of sequence r (there may be fewer rows than sequences), or with query_starts int32 [S + 1] of the sequence whose rows query_starts[s] ..
-        query_starts[s + 1] - 1 it is among; rows behind the last sequence's are copied as they are. tokens int64 [R] and
-        masks int64 [R, words] (engine.hip_tree.tree_maps) give each row its path: the tokens of the nodes of its sequence
-        whose bits its mask has. grammar_rows int32 [R]: each row's grammar state, -1 for none. out may be logits itself,
-        and must not overlap it otherwise. CPU tensors are computed by torch operations."""
+        Row r is of sequence r (there may be fewer rows than sequences), or with query_starts int32 [S + 1] of the sequence
+        whose rows query_starts[s] .. query_starts[s + 1] - 1 it is among; rows of no sequence, before or behind them, are
+        copied as they are. tokens int64 [R] and masks int64 [R, words] (engine.hip_tree.tree_maps) give each row its path:
+        the tokens of the nodes of its sequence whose bits its mask has. grammar_rows int32 [R]: each row's grammar state, -1
+        for none. out may be logits itself, and must not overlap it otherwise. CPU tensors are computed by torch
+        operations."""
         if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.dtype not in DTYPES or \
                 (self.vocab > 1 and logits.stride(1) != 1):
             raise ValueError(f"logits must be [rows, {self.vocab}] in bf16, fp16 or fp32 with a contiguous last dim")
@@ -173,7 +174,7 @@ class LogitsRules:
     def _apply_torch(self, logits, query_starts, tokens, masks, grammar_rows, out) -> torch.Tensor:
         """apply() on CPU tensors, row by row."""
         R, V = logits.shape
-        qs = list(range(R + 1)) if query_starts is None else query_starts.tolist()
+        qs = list(range(R + 1)) if query_starts is None else query_starts.clamp(0, R).tolist()
         hs = None if self.history is None else self.history_starts.clamp(0, self.history.numel()).tolist()
         bs = None if self.bias_starts is None else self.bias_starts.clamp(0, self.bias_tokens.numel()).tolist()
         words = None if masks is None else masks.tolist()
