@@ -574,12 +574,11 @@ constexpr TreeVariant kTreeVariants[] = {{1, 4, 2, 64}, {1, 8, 1, 64}};  // up t
 static int tree_tile_bytes(const TreeVariant& v, int D) { return 2 * 2 * v.kw * v.kpw * (D + 16) * 2; }
 
 // XCDs that a pair's splits go round, as a power of two. Few pairs on one XCD each would leave CUs idle (one sequence of 2 KV
-// heads has 64 of 256), and with a handful of sequences the XCDs' work differs; against that, the merge then reads through
-// memory. One sequence, 16-bit pools, 14 heads of 64, 30000 keys: 120 nodes 115 -> 58 us, 15 nodes 42 -> 33; at 2000 keys 11
-// and 14 us either way. 5 to 16 pairs: 5 to 7 % less in the mean with several row groups, 0 to 2 % with one; 17 to 64: 1 to
-// 4 % more.
+// heads has 64 of 256); against that, the merge then reads through memory. Times against one XCD a pair, in the mean: 2 pairs
+// (48 batches) 0.86 on two XCDs, 0.815 on four, 0.81 on eight (contexts over 10000 keys and several row groups 0.57, up to 3000
+// no gain or up to 1.24); 3 and 4 pairs (29 batches) 0.97; 5 to 16 pairs (320 batches) 1.00 to 1.05; 17 to 64 (71) 1.02 to 1.20.
 static int tree_log_spread(int64_t pairs, int nsplit) {
-  const int want = pairs == 1 ? 3 : pairs == 2 ? 2 : pairs <= 16 ? 1 : 0;
+  const int want = pairs == 1 ? 3 : pairs == 2 ? 2 : pairs <= 4 ? 1 : 0;
   return nsplit == 1 ? 0 : want;
 }
 
@@ -587,10 +586,10 @@ static int tree_log_spread(int64_t pairs, int nsplit) {
 // CU takes one after the other, two at once where both fit (the larger variant over plain pools at head_dim 64: 1.6 times one's
 // time), and a merge costs 256 keys and 24 a split. The lengths are on the device: the count takes every sequence for one of
 // max_context keys; where the trees' sizes differ (the token count shows it) many workgroups find no rows or keys, and half of
-// the count is that of 0.7 of the workgroups. Fitted to 468 batches (1 to 128 sequences, 1 to 128 nodes, contexts to 16384 keys,
-// both types and head sizes, over half ragged): 2.3 % over the best count's time in the mean, 1.6 times at most. One workgroup
-// per CU, rounded up, took 12 % more in the mean: 40 sequences of 2 heads made 320 workgroups of 4 splits each (31 us for 4
-// nodes at 3000 keys, 16-bit pools), where 3 splits fill 240 of the 256 CUs (20 us).
+// the count is that of 0.7 of the workgroups. Over 508 batches (1 to 128 sequences, 1 to 128 nodes, contexts to 16384 keys, both
+// types and head sizes, over half ragged) it takes 3.6 % over the best count's time in the mean, 1.39 times at most. One
+// workgroup per CU, rounded up, takes 15 % in the mean, 2.4 times at most: 40 sequences of 2 heads make 320 workgroups of 4
+// splits each (31 us for 4 nodes at 3000 keys, 16-bit pools), where 3 splits fill 240 of the 256 CUs (20 us).
 static int tree_splits(const sipa_tree_params* p, int groups, int kt, bool two, int cus, int most) {
   const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads, per_xcd = std::max(cus / 8, 1);
   const bool differ = p->num_tokens < (int64_t)p->num_seqs * p->max_nodes;
