@@ -221,6 +221,8 @@ class DecodeGraphRunner:
             raise ValueError("one input id per sequence")
         if rules is not None:
             rules.check_sequences(b)
+        elif grammar_rows is not None:
+            raise ValueError("grammar_rows without rules")
         if len(set(seq_ids)) != b:
             raise ValueError("a decode step holds each sequence once")
         bucket = self._bucket(b)

@@ -123,6 +123,8 @@ class Qwen2Model:
         rules' histories as they are."""
         if rules is not None:
             rules.check_sequences(meta.num_seqs)
+        elif grammar_rows is not None:
+            raise ValueError("grammar_rows without rules")
         cache.begin(input_ids.shape[0], meta)
         x = self.embed[input_ids]
         rot = self.rotary.rows(positions, x.dtype)

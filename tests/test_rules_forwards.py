@@ -71,3 +71,25 @@ def test_paths_of_token_ids_in_any_integer_layout(device):
     assert not torch.equal(want, model.forward(ids, meta.positions, cache, meta))
     for other in (ids.int(), torch.stack([ids, ids], 1)[:, 0], torch.stack([ids.int(), ids.int()], 1)[:, 1]):
         assert torch.equal(model.forward(other, meta.positions, cache, meta, rules=rules[3]), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grammar_states_without_rules_are_refused(device):
+    """They would be ignored, and the logits come out unmasked."""
+    cfg, m, model, cache, rules = start(device)
+    lens = [m.seq_len(s) for s in range(3)]
+    for s in range(3):
+        m.append_slot(s)
+    meta = build_metadata(m, [(s, lens[s], 1) for s in range(3)], device)
+    states, ids = torch.zeros(3, dtype=torch.int32, device=device), torch.arange(3, device=device)
+    with pytest.raises(ValueError, match="grammar"):
+        model.forward(ids, meta.positions, cache, meta, grammar_rows=states)
+    with pytest.raises(ValueError, match="grammar"):  # rules without a grammar
+        model.forward(ids, meta.positions, cache, meta, rules=rules[3], grammar_rows=states)
+    if device == "cuda":
+        from engine.graph_runner import DecodeGraphRunner
+
+        runner = DecodeGraphRunner(model, cache, m, max_batch=4, max_context=64)
+        with pytest.raises(ValueError, match="grammar"):
+            runner.step([0, 1, 2], ids, grammar_rows=states)
+        runner.close()
