@@ -15,12 +15,12 @@
 // (2.3e-3 of it in all against 1.7e-3). The second is taken from p (1 + 2^-20), so that it is never zero against an infinite
 // V.
 //
-// What bounds it: with few rows the pools' bytes (one node, 7 heads a KV head, 32 sequences of 8192 keys: 35 us, 3.8 TB/s);
+// What bounds it: with few rows the pools' bytes (one node, 7 heads a KV head, 32 sequences of 8192 keys: 31 us, 4.4 TB/s);
 // from about 16 nodes on the vector ALUs, which turn each score into two bf16 terms of p, and the wait of the waves for each
 // other at a stage's end: a stage of 64 keys and 128 rows takes some 2400 cycles, 1000 of them the softmax of a SIMD's two
-// waves, 460 the scores, 370 the second product. 16 nodes, 32 sequences of 8192 keys: 48 us of 27 for the bytes; 64 nodes, 16
-// ragged sequences about 12000 long, head_dim 128: 155 us of 43; INT8, 11 nodes, 64 sequences of 4096: 72 us of 28. Short
-// calls take the chain of one workgroup's loads: 11 us for 5 nodes at 1024 keys.
+// waves, 460 the scores, 370 the second product. 16 nodes, 32 sequences of 8192 keys: 47 us of 27 for the bytes (INT8: 58 of
+// 14); 64 nodes, 16 ragged sequences about 12000 long, head_dim 128: 152 us of 43; INT8, 11 nodes, 64 sequences of 4096,
+// head_dim 128: 72 us of 28. Short calls take the chain of one workgroup's loads: 12 us for 5 nodes at 1024 keys.
 #include <algorithm>
 #include <type_traits>
 
@@ -584,12 +584,12 @@ static int tree_log_spread(int64_t pairs, int nsplit) {
 
 // The number of splits: the cheapest by a count of keys. A workgroup costs its split's keys and 256 more (its start and end), a
 // CU takes one after the other, two at once where both fit (the larger variant over plain pools at head_dim 64: 1.6 times one's
-// time), and a merge costs 256 keys and 24 a split. The lengths are on the device: the count takes every sequence for one of
+// time), and a merge costs 256 keys and 24 a split. The call is not given the lengths: the count takes every sequence for one of
 // max_context keys; where the trees' sizes differ (the token count shows it) many workgroups find no rows or keys, and half of
 // the count is that of 0.7 of the workgroups. Over 508 batches (1 to 128 sequences, 1 to 128 nodes, contexts to 16384 keys, both
 // types and head sizes, over half ragged) it takes 3.6 % over the best count's time in the mean, 1.39 times at most. One
 // workgroup per CU, rounded up, takes 15 % in the mean, 2.4 times at most: 40 sequences of 2 heads make 320 workgroups of 4
-// splits each (31 us for 4 nodes at 3000 keys, 16-bit pools), where 3 splits fill 240 of the 256 CUs (20 us).
+// splits each (36 us for 6 nodes at 3000 keys, 16-bit pools, head_dim 64), where 3 splits fill 240 of the 256 CUs (23 us).
 static int tree_splits(const sipa_tree_params* p, int groups, int kt, bool two, int cus, int most) {
   const int64_t pairs = (int64_t)p->num_seqs * p->num_kv_heads, per_xcd = std::max(cus / 8, 1);
   const bool differ = p->num_tokens < (int64_t)p->num_seqs * p->max_nodes;

@@ -39,7 +39,7 @@ __device__ __forceinline__ int32_t tree_table_entry(const TreeMapsArgs& a, int s
 }
 
 // Every workgroup forms the query starts for itself (S loads that the L2 serves, one scan), so that one launch does it all: bound
-// by the latency of its chain of loads, not by bytes: 3.4 us for 1 tree of 5 nodes; 9.0 us for 256 ragged trees of up to 64
+// by the latency of its chain of loads, not by bytes: 3.5 us for 1 tree of 5 nodes; 9.1 us for 256 ragged trees of up to 64
 // nodes at 8192 tokens. An ancestor is one load after the other, as many as the tree is deep.
 __global__ void __launch_bounds__(256) tree_maps_kernel(const TreeMapsArgs a) {
   __shared__ int32_t qs[kTreeMaxSeqs + 1];
@@ -128,9 +128,10 @@ struct CommitArgs {
 
 // One thread takes one 16-byte part of the moved rows of a (sequence, pool, layer, head), all its moves in order: source
 // indices ascend and are at least their destinations', so a load never reads what an earlier store has written. Kept at
-// kMoves loads in flight before their stores: bound by latency (index, block id, row), 4.4 us for up to 4 nodes of one
-// sequence in 24 layers, 10.7 us for 64 sequences' up to 7 nodes in 28 layers of INT8 pools (a call with the host's part: 7.8
-// and 12.0).
+// kMoves loads in flight before their stores: 4.4 us for up to 4 nodes of one sequence in 24 layers, a short chain of loads
+// (index, block id, row); 10.7 us for 64 sequences' up to 7 nodes in 28 layers of INT8 pools, where the 64-bit divisions by
+// the block size, two a move, and by the thread's dimensions weigh more than the 1.6 us of bytes (a call with the host's part:
+// 8.0 and 11.9).
 constexpr int kMoves = 8;
 
 __global__ void __launch_bounds__(256) commit_tokens_kernel(const CommitArgs a) {

@@ -150,7 +150,7 @@ class LogitsRules:
                                 (self.vocab > 1 and out.stride(1) != 1)):
             raise ValueError("out must be as logits, with a contiguous last dim")
         if out is not None and _overlap(logits, out):
-            raise ValueError("out's rows overlap each other or other rows of the logits; it may be logits itself or lie beside them")
+            raise ValueError("out's rows overlap each other or other rows of the logits (it may be logits itself)")
         dev = logits.device
         if self.device is not None and self.device != dev:
             raise ValueError(f"logits on {dev}, rules on {self.device}")
