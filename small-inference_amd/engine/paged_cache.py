@@ -183,8 +183,12 @@ class TreeMetadata(PagedMetadata):
 
 def check_trees(batch: list[tuple[int, int, list[int]]]) -> list[tuple[int, int, int]]:
     """The (seq_id, start, n) batch of [(seq_id, start, parents)], or ValueError for parents that are no tree of 1 to
-    hip_tree.MAX_NODES nodes in which parents come first."""
+    hip_tree.MAX_NODES nodes in which parents come first, or a sequence that has two."""
+    seen = set()
     for seq_id, _, parents in batch:
+        if seq_id in seen:
+            raise ValueError(f"sequence {seq_id} twice in a batch: its trees would share slots")
+        seen.add(seq_id)
         if not 1 <= len(parents) <= MAX_NODES:
             raise ValueError(f"sequence {seq_id}: a tree of {len(parents)} nodes; 1 to {MAX_NODES} can be drafted")
         for i, p in enumerate(parents):
