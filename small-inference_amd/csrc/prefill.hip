@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(64 * NC / CW * KH) prefill_mfma_bf16(const Pre
           big = x < __builtin_huge_valf() ? vmax(big, x) : big;
         }
       big = max_over_rows_swap(big * inv);
-      // big < 2^ex (ex 0 for big 0); from -100 on, which 2^-e / l and the merge's weights times 2^e are normal numbers for
+      // big < 2^ex (ex 0 for big 0); at least -100, so that 2^-e / l and the merge's weights times 2^e stay normal numbers
       const int e = max(__builtin_amdgcn_frexp_expf(big) - 15, -100);
       const float inv_e = __builtin_amdgcn_ldexpf(inv, -e);
 #pragma unroll
