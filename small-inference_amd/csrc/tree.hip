@@ -576,7 +576,8 @@ static int tree_tile_bytes(const TreeVariant& v, int D) { return 2 * 2 * v.kw * 
 // XCDs that a pair's splits go round, as a power of two. Few pairs on one XCD each would leave CUs idle (one sequence of 2 KV
 // heads has 64 of 256); against that, the merge then reads through memory. Times against one XCD a pair, in the mean: 2 pairs
 // (48 batches) 0.86 on two XCDs, 0.815 on four, 0.81 on eight (contexts over 10000 keys and several row groups 0.57, up to 3000
-// no gain or up to 1.24), so one pair, which has half their CUs, goes round all eight; 3 and 4 pairs (29 batches) 0.97; 5 to 16 pairs (320 batches) 1.00 to 1.05; 17 to 64 (71) 1.02 to 1.20.
+// no gain or up to 1.24), so one pair, which has half their CUs, goes round all eight; 3 and 4 pairs (29 batches) 0.97; 5 to 16
+// pairs (320 batches) 1.00 to 1.05; 17 to 64 (71) 1.02 to 1.20.
 static int tree_log_spread(int64_t pairs, int nsplit) {
   const int want = pairs == 1 ? 3 : pairs == 2 ? 2 : pairs <= 4 ? 1 : 0;
   return nsplit == 1 ? 0 : want;
