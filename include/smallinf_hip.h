@@ -735,6 +735,121 @@ int64_t sipa_tree_workspace_bytes(const sipa_tree_params* p, int64_t* counter_by
  * to its capture. */
 uint64_t sipa_capture_id(void* stream);
 
+/*
+ * Decode attention (one token a sequence) of sequences whose block tables begin with the same blocks: the keys that a group
+ * of them shares are read once for all of it.
+ *   out[s, h*G + g, :] = sum_j softmax_j(scale * q[s, h*G + g, :] . k_j) v_j over the positions j < context_lens[s] of s's
+ * block table; a row without any gets zeros. What is shared changes the time, not the result: a group is a promise of the
+ * caller that its members' tables agree in their first tokens / B entries. A member whose context is shorter than that is
+ * read by itself. bf16 q and out; pools bf16 (SIPA_KV_PLAIN) or int8 with per-token scales (SIPA_KV_INT8_TOKEN). head_dim 64
+ * or 128, blocks of 16, 32 or 64 tokens, groups of up to 16 query heads a KV head. K and V behind the contexts' ends may hold
+ * anything.
+ *
+ * sipa_prefix_plan (host only, no launch): the work list of a batch. Groups g = 0 .. num_groups - 1 have the batch rows
+ * members[group_starts[g] .. group_starts[g + 1] - 1] (each row in one group at most, rows in none read by themselves) and share
+ * tokens[g] tokens, whole blocks; all of these are host memory, as is context_lens (the sequences' lengths, for the split of
+ * their own keys; may be NULL: max_context is taken). Reads the sizes of p and max_context. Writes the layout, and plan (NULL:
+ * the layout alone) of layout->plan_ints values, of which the caller hands a device copy to sipa_prefix_attention with the
+ * same sizes, any tensors and any context lengths up to max_context.
+ */
+typedef struct sipa_prefix_layout {
+  int32_t num_items, num_members, tile_rows, own_splits, own_chunk;
+  int64_t plan_ints, workspace_bytes;
+} sipa_prefix_layout;
+
+typedef struct sipa_prefix_params {
+  int32_t struct_size; /* sizeof(sipa_prefix_params) */
+  int32_t num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
+  int32_t max_context;  /* largest context length, known on the host; context lengths are clamped to it. Up to 2^24 */
+  int32_t kv_mode;      /* SIPA_KV_PLAIN or SIPA_KV_INT8_TOKEN */
+  float scale;          /* positive and finite */
+  const void* q;        /* [S, Hq, D]; last dim contiguous, rows 16-byte aligned */
+  int64_t q_stride_s, q_stride_h;
+  const void* k_cache;  /* [Hkv, N, B, D], each head's blocks contiguous */
+  const void* v_cache;
+  int64_t kv_stride_h, kv_stride_n;
+  const int32_t* block_tables; /* [S, bt_width], bt_width >= ceil(max_context / B); ids are clamped to [0, num_blocks) */
+  int64_t bt_stride_s;
+  int32_t bt_width;
+  const int32_t* context_lens; /* [S], the new token included */
+  void* out;                   /* [S, Hq, D], rows 8-byte aligned */
+  int64_t out_stride_s, out_stride_h;
+  const void* k_scale;         /* [Hkv, N, B], last dim contiguous */
+  int32_t k_scale_dtype;       /* SIPA_F16 or SIPA_F32 */
+  int64_t ks_stride_h, ks_stride_n;
+  const void* v_scale;
+  int32_t v_scale_dtype;
+  int64_t vs_stride_h, vs_stride_n;
+  sipa_prefix_layout layout;   /* of sipa_prefix_plan, for these sizes */
+  const int32_t* plan;         /* device copy of its plan, 16-byte aligned */
+  /* layout.workspace_bytes, 256-byte aligned; holds nothing between calls. Calls that may run at the same time need
+     workspaces of their own. */
+  void* workspace;
+  int64_t workspace_bytes;
+} sipa_prefix_params;
+
+int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_groups, const int32_t* group_starts, const int32_t* members,
+                         const int32_t* tokens, const int32_t* context_lens, int32_t* plan, int64_t capacity,
+                         sipa_prefix_layout* layout);
+
+int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stream);
+
+/*
+ * The best continuations of beams: of the rows of each group, the num_candidates tokens v of largest
+ *   scores[r] + logits[r, v] - log(sum_v exp(logits[r, v])),
+ * in descending order; equal ones by row, then by token. A row's tokens are ordered by their logits, rows against each other
+ * by these sums in 64 bits, from which out_scores are rounded once. Group g has the rows g * beams .. (g + 1) * beams - 1, or
+ * with starts [num_groups + 1] rows starts[g] .. starts[g + 1] - 1 (clamped to the rows, 1024 of a group at most). Tokens of
+ * logit -inf are none of them, nor are those of a row whose score or sum is not finite (NaN or +inf among its logits, all of
+ * them -inf). Where there are fewer than num_candidates: score -inf, beam and token -1.
+ */
+typedef struct sipa_beam_params {
+  int32_t struct_size;    /* sizeof(sipa_beam_params) */
+  int32_t num_rows, vocab;
+  int32_t num_groups, beams;
+  int32_t num_candidates; /* 1 .. 64 */
+  int32_t dtype;          /* SIPA_F32, SIPA_BF16 or SIPA_F16 */
+  const void* logits;     /* [num_rows, vocab], last dim contiguous */
+  int64_t logits_stride;
+  const float* scores;    /* [num_rows] */
+  const int32_t* starts;  /* [num_groups + 1] or NULL */
+  float* out_scores;      /* [num_groups, num_candidates] */
+  int64_t* out_beams;     /* row within the group */
+  int64_t* out_tokens;
+  /* sipa_beam_workspace_bytes() bytes, 256-byte aligned; holds nothing between calls. Calls that may run at the same time
+     need workspaces of their own. */
+  void* workspace;
+  int64_t workspace_bytes;
+} sipa_beam_params;
+
+int32_t sipa_beam_select(const sipa_beam_params* p, void* stream);
+
+/* Workspace bytes the call needs, or a negative return code. Reads the sizes and dtype. */
+int64_t sipa_beam_workspace_bytes(const sipa_beam_params* p);
+
+/*
+ * Copies the first tokens of blocks to other blocks, in all layers and heads of up to four pools (K, V, their scales):
+ * for i < num_copies, rows 0 .. tokens - 1 of block src become those of block dst, (src, dst, tokens) = copies[3 i ..]. Beams
+ * that go on from the same one share its full blocks; its last block, where it is not full, is copied for all but one.
+ * copies is HOST memory, read during the call (a captured call copies the same blocks at every replay). No block may be the
+ * destination of two copies, or of one and the source of another (SIPA_EINVAL).
+ */
+typedef struct sipa_copy_params {
+  int32_t struct_size; /* sizeof(sipa_copy_params) */
+  int32_t num_layers, num_kv_heads, num_blocks, block_size;
+  int32_t num_pools;   /* 1 .. 4 */
+  void* pools[4];      /* each [L, Hkv, N, B, row_bytes], a head's blocks contiguous */
+  int64_t stride_l[4], stride_h[4]; /* in bytes */
+  int32_t row_bytes[4]; /* of a token */
+  const int32_t* copies;
+  int32_t num_copies;
+} sipa_copy_params;
+
+int32_t sipa_copy_blocks(const sipa_copy_params* p, void* stream);
+
+/* SIPA_OK where sipa_copy_blocks takes these copies (host memory), else SIPA_EINVAL. Host only. */
+int32_t sipa_check_copies(const int32_t* copies, int32_t num_copies, int32_t num_blocks, int32_t block_size);
+
 #ifdef __cplusplus
 }
 #endif

@@ -362,7 +362,29 @@ __device__ void finish_split(const DecodeArgs& a, int s, int h, int sp, int nval
 // ---- MFMA kernels --------------------------------------------------------------------------------------------
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// A scale as it lies in memory, and its value: apart, so that the load is waited for only where the value is needed.
+__device__ __forceinline__ uint32_t scale_bits(const void* base, bool f32, int64_t i) {
+  return f32 ? ((const uint32_t*)base)[i] : (uint32_t)((const uint16_t*)base)[i];
+}
+
+__device__ __forceinline__ float scale_value(uint32_t bits, bool f32) {
+  return f32 ? __uint_as_float(bits) : f16_bits_to_f32(bits);
+}
+
+// Eight int8 codes (two words) as bf16, exactly.
+__device__ __forceinline__ u32x4 tree_codes(uint32_t w0, uint32_t w1) {
+  u32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? w0 : w1;
+    const int b = 16 * (i & 1);
+    x[i] = pack_bf16x2((float)(int8_t)(w >> b), (float)(int8_t)(w >> (b + 8)));
+  }
+  return x;
+}
 
 // Transposing LDS read (gfx950 ds_read_b64_tr_b16). Within each group of 16 lanes, lane j passes the address of a
 // 4-element (8-byte) chunk M[j]; lane i receives M[4 k + i / 4][i % 4], k = 0..3. With lane j of group q4 pointing

@@ -67,8 +67,6 @@ struct PrefillArgs {
   float* part;             // [units][nsplit][8 columns][16 tokens][D] each split's output O / l 2^-e, as fp16
 };
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 // Workgroup layouts: NC column tiles (a query head and 16 tokens) per workgroup, CW per wave, NC / CW waves.
 //   SIPA_PREFILL_W4X2 (NC 8, CW 2): 4 waves; each K/V operand read serves two column tiles. Large grids.
 //   SIPA_PREFILL_W8X1 (NC 8, CW 1): 8 waves, twice the waves per CU for grids of at most 2 workgroups per CU.
@@ -138,14 +136,6 @@ __device__ __forceinline__ float chan_scale(const u32x4 (&w)[4], bool f32, int j
   if (f32) return __uint_as_float(w[j >> 2][j & 3]);
   const uint32_t d = w[j >> 3][(j >> 1) & 3];
   return f16_bits_to_f32((j & 1) ? d >> 16 : d & 0xffffu);
-}
-
-__device__ __forceinline__ uint32_t scale_bits(const void* base, bool f32, int64_t i) {
-  return f32 ? ((const uint32_t*)base)[i] : (uint32_t)((const uint16_t*)base)[i];
-}
-
-__device__ __forceinline__ float scale_value(uint32_t bits, bool f32) {
-  return f32 ? __uint_as_float(bits) : f16_bits_to_f32(bits);
 }
 
 // 8 int8 codes -> 8 bf16 of code * scale(j), computed in fp32 and rounded to nearest even (the reference's

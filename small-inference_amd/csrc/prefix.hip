@@ -1,0 +1,827 @@
+// Decode attention of sequences whose block tables begin with the same blocks (gfx950): the shared keys are read once for a
+// whole group of them. The reference reads every sequence's context by itself.
+//
+// One token a sequence. A row (sequence, query head) splits its softmax over the keys of its group's prefix and those of its
+// own: (m, l, O) of each part, m the part's largest score, l = sum 2^(s - m), O = sum 2^(s - m) v, joined as
+//   M = max m,  out = sum 2^(m - M) O / sum 2^(m - M) l.
+// Prefix items: (group, KV head, up to ROWS of the group's rows, keys): the members' G query heads make one matrix of rows
+// that see every key, so the product has full tiles whatever G is. Own items: (sequence, KV head, keys), G rows of 16.
+// Both kinds are workgroups of one launch; a second, small one joins a row's parts.
+#include <algorithm>
+
+#include "decode_common.h"
+
+namespace sipa {
+
+constexpr int kPrefixMaxChunk = 16384;  // keys of a prefix item: its block ids stand in LDS
+constexpr int kPrefixThreads = 512, kPrefixWaves = 8;
+
+struct PrefixArgs {
+  const uint16_t* q;
+  int64_t q_ss, q_sh;
+  const void* k;
+  const void* v;
+  int64_t kv_sh, kv_sn;
+  const int32_t* bt;
+  int64_t bt_ss;
+  int32_t bt_w;
+  const int32_t* ctx;
+  uint16_t* out;
+  int64_t o_ss, o_sh;
+  const void* ks;
+  const void* vs;
+  bool ks_f32, vs_f32;
+  int64_t ks_sh, ks_sn, vs_sh, vs_sn;
+  const int32_t* items;    // [num_items][8]: table row, first member, rows, first row, KV head, first key, end, -
+  const int32_t* rows;     // [S][8]: prefix tokens, first row in the group, first state, splits, row tiles, -
+  const int32_t* members;  // batch rows of the groups, one group after the other
+  int32_t num_items, num_members, S, Hkv, G, nb, max_ctx;
+  int32_t log_b;           // blocks of 1 << log_b tokens
+  int32_t nsplit, chunk;   // of the sequences' own keys
+  int32_t tile_rows;       // rows of a prefix item
+  float scale_log2;
+  float* p_m;              // [num_items][tile_rows]
+  float* p_l;
+  float* p_o;              // [num_items][tile_rows][D]
+  float* s_m;              // [S Hkv][nsplit][G]
+  float* s_l;
+  float* s_o;              // [S Hkv][nsplit][G][D]
+};
+
+// A sequence's keys: the prefix's `shared` (read with its group, or 0), then splits of `chunk` keys of its own. A context that
+// is shorter than its group's prefix is read by itself, from its first key on.
+struct OwnKeys {
+  int shared, ctx, chunk, splits;
+};
+
+__device__ __forceinline__ OwnKeys own_keys(const PrefixArgs& a, int s) {
+  OwnKeys k;
+  const int tokens = a.rows[8 * (int64_t)s];
+  k.ctx = min(max(a.ctx[s], 0), a.max_ctx);
+  k.shared = k.ctx >= tokens ? tokens : 0;
+  const int own = k.ctx - k.shared;
+  k.chunk = max(a.chunk, ((own + a.nsplit - 1) / a.nsplit + 63) & ~63);
+  k.splits = (own + k.chunk - 1) / k.chunk;
+  return k;
+}
+
+// The four scales of consecutive keys, at any alignment, as fp32.
+__device__ __forceinline__ f32x4 four_scales(const void* base, bool f32, int64_t i) {
+  struct __attribute__((packed, aligned(4))) Four {
+    float x[4];
+  };
+  struct __attribute__((packed, aligned(2))) Halves {
+    uint32_t w[2];
+  };
+  if (f32) {
+    const Four s = *(const Four*)((const float*)base + i);
+    return f32x4{s.x[0], s.x[1], s.x[2], s.x[3]};
+  }
+  const Halves s = *(const Halves*)((const uint16_t*)base + i);
+  return f32x4{f16_bits_to_f32(s.w[0] & 0xffff), f16_bits_to_f32(s.w[0] >> 16), f16_bits_to_f32(s.w[1] & 0xffff),
+               f16_bits_to_f32(s.w[1] >> 16)};
+}
+
+// The softmax state of 16 rows in a wave, lane (r, q4) holding row r: O^T in the accumulators' layout (channels 16 dt + 4 q4 + i).
+template <int D>
+struct RowState {
+  static constexpr int DT = D / 16;
+  float m, off, threshold;  // off: m, or 0 while that is -inf
+  f32x4 l;
+  f32x4 acc[DT];
+
+  __device__ __forceinline__ void clear() {
+    m = threshold = kNegInf, off = 0.f, l = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Takes up N keys' scores (hidden ones -inf), N a multiple of 32, score (mt, i) that of key 16 mt + 4 q4 + i: raises the
+  // running max where one exceeds it by more than 2^16 (p stays far inside fp32), and returns the probabilities as two bf16
+  // terms, 16 bits of them: one alone gives errors as large as the result's own rounding. The second is taken from
+  // p (1 + 2^-20), so that it is never zero against an infinite V. MODE 0: raw scores; MODE 1: scores in log2 units, with V's
+  // scales at vs, and l takes the unscaled p.
+  template <int MODE, int N>
+  __device__ __forceinline__ void add(const f32x4 (&sc)[N / 16], float scale_log2, float inv_scale_log2, bf16x8 ones,
+                                      const f32x4* vs, u32x4 (&hi)[N / 32], u32x4 (&lo)[N / 32]) {
+    constexpr float kSlack = 8.f, kFastRange = 16.f;
+    float mx = sc[0][0];
+#pragma unroll
+    for (int mt = 0; mt < N / 16; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = vmax(mx, sc[mt][i]);
+    if (__builtin_amdgcn_ballot_w64(mx > threshold)) {
+      mx = max_over_rows_swap(mx) * (MODE == 0 ? scale_log2 : 1.f);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {
+        const float m_new = fmaxf(m, mx);
+        const float alpha = fast_exp2(m - (m_new == kNegInf ? 0.f : m_new));  // 0 while the row has seen no key
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+        m = m_new;
+        off = m_new == kNegInf ? 0.f : m_new;
+        threshold = (m_new + kFastRange) * inv_scale_log2;
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < N / 32; ++hf) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = sc[2 * hf + (i >> 2)][i & 3];
+        p[i] = fast_exp2(MODE == 0 ? fmaf(x, scale_log2, -off) : x - off);
+      }
+      if constexpr (MODE == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          l[i & 3] += p[i];
+          p[i] = p[i] == 0.f ? 0.f : p[i] * vs[2 * hf + (i >> 2)][i & 3];  // a hidden key's scale may be anything
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        uint32_t cut[2];
+        float rest[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          cut[x] = __float_as_uint(p[i + x]) & 0xffff0000u;
+          rest[x] = fmaf(p[i + x], 1.f + 0x1p-20f, -__uint_as_float(cut[x]));
+        }
+        hi[hf][i >> 1] = __builtin_amdgcn_perm(cut[1], cut[0], 0x07060302u);
+        lo[hf][i >> 1] = pack_bf16x2(rest[0], rest[1]);
+      }
+      if constexpr (MODE == 0) {  // the sums on the matrix cores, of the values that the product uses
+        l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, hi[hf]), l, 0, 0, 0);
+        l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, lo[hf]), l, 0, 0, 0);
+      }
+    }
+  }
+
+  // O^T += V^T . P^T over N keys whose V stands row-major in LDS.
+  template <int N>
+  __device__ __forceinline__ void product(const uint16_t* sv, int tr_off, int pitch, const u32x4 (&hi)[N / 32],
+                                          const u32x4 (&lo)[N / 32]) {
+#pragma unroll
+    for (int hf = 0; hf < N / 32; ++hf)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const bf16x8 vop = read_v_operand<bf16x8>(sv + 32 * pitch * hf, tr_off, pitch, 16 * dt);
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, hi[hf]), acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, lo[hf]), acc[dt], 0, 0, 0);
+      }
+  }
+
+  __device__ __forceinline__ float sum(int mode) const {
+    return mode == 0 ? l[0] : sum_over_rows_swap(l[0] + l[1] + l[2] + l[3]);
+  }
+};
+
+__device__ __forceinline__ bf16x8 bf16_ones() {
+  bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
+  asm volatile("" : "+v"(ones));  // kept in registers
+  return ones;
+}
+
+template <int D, int KW>
+struct PrefixSmem {
+  static constexpr int KT = 64 * KW, P = D + 16;  // keys of a stage, elements between its rows
+  static constexpr int kTiles = 2 * 2 * KT * P * 2;  // [buffer][K, V][key][P]
+  static constexpr int kOwnPitch = D + 8;
+  static constexpr int kOwnTiles = kPrefixWaves * 32 * kOwnPitch * 2;  // [wave][key][P] of V
+  static constexpr int kOwnMerge = kPrefixWaves * 16 * (D + 4 + 2) * 4;
+  static constexpr int kBytes = kTiles > kOwnTiles ? (kTiles > kOwnMerge ? kTiles : kOwnMerge)
+                                                   : (kOwnTiles > kOwnMerge ? kOwnTiles : kOwnMerge);
+};
+
+// A prefix item: 8 / KW waves side by side over 16 rows each, KW one after the other over the keys, 64 keys each of a stage.
+template <int D, int MODE, int KW, int NPRE>
+__device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, float (*sscale)[2][64 * KW], int* bids) {
+  constexpr int KPW = 64, KT = KW * KPW, MT = KPW / 16, P = D + 16, KS = D / 32, DT = D / 16;
+  constexpr int PT = kPrefixThreads, RW = kPrefixWaves / KW, ROWS = 16 * RW;
+  constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, NCH = KT * CPK;  // 16-byte parts of a key, of a stage
+  constexpr int LPT = (NCH + PT - 1) / PT, SPT = MODE == 0 ? 1 : (2 * KT + PT - 1) / PT;
+  uint16_t(*sm)[2][KT * P] = (uint16_t(*)[2][KT * P]) smem;
+  const int item = blockIdx.x, tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
+  const int4 i0 = *(const int4*)(a.items + 8 * (int64_t)item), i1 = *(const int4*)(a.items + 8 * (int64_t)item + 4);
+  const int table_row = min(max(i0.x, 0), a.S - 1), first_member = max(i0.y, 0), M = max(i0.z, 1), m0 = max(i0.w, 0);
+  const int h = min(max(i1.x, 0), a.Hkv - 1), k_lo = max(i1.y, 0), k_hi = min(min(i1.z, a.max_ctx), k_lo + kPrefixMaxChunk);
+  const int nkeys = k_hi - k_lo, G = a.G;
+  if (nkeys <= 0) return;  // (never in a list of sipa_prefix_plan)
+
+  const int32_t* table = a.bt + (int64_t)table_row * a.bt_ss;
+  const int first_col = k_lo >> a.log_b;
+  for (int i = tid; i << a.log_b < nkeys; i += PT) bids[i] = min(max(table[min(first_col + i, a.bt_w - 1)], 0), a.nb - 1);
+  const int m = m0 + 16 * rw + r, at = min(m, M - 1);
+  const bool valid = m0 + 16 * rw < M;  // wave-uniform: some row of the tile is there
+  bf16x8 qop[KS];
+  {
+    const int i = at / G, s = min(max(a.members[min(first_member + i, a.num_members - 1)], 0), a.S - 1);
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+      qop[j] = __builtin_bit_cast(
+          bf16x8, *(const u32x4*)(a.q + (int64_t)s * a.q_ss + (int64_t)(h * G + at - i * G) * a.q_sh + 32 * j + 8 * q4));
+  }
+  const float inv_scale_log2 = MODE == 0 ? 1.f / a.scale_log2 : 1.f;
+  RowState<D> st;
+  st.clear();
+  const int tr_off = tr16_offset(r, q4, P);
+  const bf16x8 ones = bf16_ones();
+  __syncthreads();  // block ids
+
+  const int ntiles = (nkeys + KT - 1) / KT;
+  u32x4 rk[NPRE][LPT], rv[NPRE][LPT];
+  uint32_t rs[NPRE][SPT];
+  // A thread's parts of a stage keep their place in their blocks from stage to stage (a stage is whole blocks): what changes
+  // is the block id. Keys past the item's end are read too, inside its last block; they are hidden, and their V is zero.
+  const int es = MODE == 0 ? 2 : 1, last_id = (nkeys - 1) >> a.log_b;
+  const uint32_t kv_bytes = (uint32_t)a.kv_sn * es;  // of a block (host-checked)
+  const uint8_t* kbase[LPT];
+  const uint8_t* vbase[LPT];
+  int part_id[LPT];
+#pragma unroll
+  for (int i = 0; i < LPT; ++i) {
+    const int c = tid + PT * i, key = c / CPK;
+    const int64_t e = ((int64_t)h * a.kv_sh + (key & ((1 << a.log_b) - 1)) * D + CH * (c % CPK)) * es;
+    kbase[i] = (const uint8_t*)a.k + e;
+    vbase[i] = (const uint8_t*)a.v + e;
+    part_id[i] = key >> a.log_b;
+  }
+  auto gload = [&](int set, int t) {
+#pragma unroll
+    for (int i = 0; i < LPT; ++i) {
+      if (NCH % PT != 0 && tid + PT * i >= NCH) break;
+      const uint64_t b = (uint64_t)(uint32_t)bids[min((KT * t >> a.log_b) + part_id[i], last_id)] * kv_bytes;
+      rk[set][i] = *(const u32x4*)(kbase[i] + b);
+      rv[set][i] = *(const u32x4*)(vbase[i] + b);
+    }
+    if constexpr (MODE == 1) {
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) {
+        const int c = tid + PT * i;
+        if (2 * KT % PT != 0 && c >= 2 * KT) break;
+        const int key = c % KT, off = key & ((1 << a.log_b) - 1);
+        const int64_t blk = bids[min((KT * t >> a.log_b) + (key >> a.log_b), last_id)];
+        rs[set][i] = c < KT ? scale_bits(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + blk * a.ks_sn + off)
+                            : scale_bits(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + blk * a.vs_sn + off);
+      }
+    }
+  };
+  auto sstore = [&](int set, int t) {
+    const int buf = t & 1;
+#pragma unroll
+    for (int i = 0; i < LPT; ++i) {
+      const int c = tid + PT * i;
+      if (NCH % PT != 0 && c >= NCH) break;
+      const int key = c / CPK, e = key * P + CH * (c % CPK);
+      const u32x4 k = rk[set][i];
+      u32x4 v = rv[set][i];
+      if (KT * t + key >= nkeys) v = u32x4{0, 0, 0, 0};
+      if constexpr (MODE == 0) {
+        *(u32x4*)(&sm[buf][0][e]) = k;
+        *(u32x4*)(&sm[buf][1][e]) = v;
+      } else {
+        // Odd lanes store their second half first at head_dim 64, as 16 bytes of each 32 use half the banks.
+        const int odd = D == 64 ? tid & 1 : 0;
+        *(u32x4*)(&sm[buf][0][e + 8 * odd]) = tree_codes(odd ? k[2] : k[0], odd ? k[3] : k[1]);
+        *(u32x4*)(&sm[buf][0][e + 8 - 8 * odd]) = tree_codes(odd ? k[0] : k[2], odd ? k[1] : k[3]);
+        *(u32x4*)(&sm[buf][1][e + 8 * odd]) = tree_codes(odd ? v[2] : v[0], odd ? v[3] : v[1]);
+        *(u32x4*)(&sm[buf][1][e + 8 - 8 * odd]) = tree_codes(odd ? v[0] : v[2], odd ? v[1] : v[3]);
+      }
+    }
+    if constexpr (MODE == 1) {
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) {
+        const int c = tid + PT * i;
+        if (2 * KT % PT != 0 && c >= 2 * KT) break;
+        sscale[buf][c / KT][c % KT] = c < KT ? scale_value(rs[set][i], a.ks_f32) * a.scale_log2 : scale_value(rs[set][i], a.vs_f32);
+      }
+    }
+  };
+  auto tile = [&](int t) {
+    const int x0 = KT * t + KPW * kw;  // the wave's first key of the item
+    if (x0 >= nkeys || !valid) return;  // wave-uniform
+    const int buf = t & 1;
+    const uint16_t* sk = sm[buf][0] + KPW * kw * P;
+    const uint16_t* sv = sm[buf][1] + KPW * kw * P;
+    f32x4 sc[MT], vs[MT];  // row (mt, q4, i) holds key 16 mt + 4 q4 + i
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const bf16x8 kop = *(const bf16x8*)(sk + (16 * mt + r) * P + 32 * j + 8 * q4);
+        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[j], sc[mt], 0, 0, 0);
+      }
+      if constexpr (MODE == 1) {
+        sc[mt] *= *(const f32x4*)(sscale[buf][0] + KPW * kw + 16 * mt + 4 * q4);  // log2 units
+        vs[mt] = *(const f32x4*)(sscale[buf][1] + KPW * kw + 16 * mt + 4 * q4);
+      }
+    }
+    if (x0 + KPW > nkeys) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (x0 + 16 * mt + 4 * q4 + i >= nkeys) sc[mt][i] = kNegInf;
+    }
+    u32x4 hi[KPW / 32], lo[KPW / 32];
+    st.template add<MODE, KPW>(sc, a.scale_log2, inv_scale_log2, ones, vs, hi, lo);
+    st.template product<KPW>(sv, tr_off, P, hi, lo);
+  };
+#pragma unroll
+  for (int k = 0; k < NPRE; ++k) {
+    gload(k, k);
+    asm volatile("" ::: "memory");  // in this order
+  }
+  sstore(0, 0);
+  __syncthreads();
+  // register set k % NPRE carries stage k to its LDS store; loads past the last stage read its last key again, so that
+  // every wait is for a fixed count, and stages past it compute nothing
+  for (int tb = 0; tb < ntiles; tb += NPRE) {
+#pragma unroll
+    for (int k = 0; k < NPRE; ++k) {
+      const int t = tb + k;
+      gload(k, t + NPRE);
+      tile(t);
+      sstore((k + 1) % NPRE, t + 1);  // that buffer was last read before the last barrier
+      __syncthreads();
+    }
+  }
+  float l = st.sum(MODE);
+  if (l != l) st.m = 0.f;  // NaN scores never raise the max: the merges see the row by its sum
+  if constexpr (KW > 1) {
+    // The key waves' states join in LDS (the tile buffers are free after the last barrier).
+    constexpr int XS = DT * 4 + 4;  // floats of a lane: O, m, l
+    static_assert((KW - 1) * RW * 64 * XS * 4 <= PrefixSmem<D, KW>::kTiles, "the states fit the tile buffers");
+    float* xs = (float*)smem;
+    if (kw > 0) {
+      float* x = xs + (((kw - 1) * RW + rw) * 64 + lane) * XS;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *(f32x4*)(x + 4 * dt) = st.acc[dt];
+      x[4 * DT] = st.m;
+      x[4 * DT + 1] = l;
+    }
+    __syncthreads();
+    if (kw == 0) {
+#pragma unroll
+      for (int k = 1; k < KW; ++k) {
+        const float* x = xs + (((k - 1) * RW + rw) * 64 + lane) * XS;
+        const float m1 = x[4 * DT], l1 = x[4 * DT + 1], top = vmax(st.m, m1);
+        if (top == kNegInf) continue;
+        const float f0 = fast_exp2(st.m - top), f1 = fast_exp2(m1 - top);
+        l = f0 * l + f1 * l1;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) st.acc[dt] = f0 * st.acc[dt] + f1 * *(const f32x4*)(x + 4 * dt);
+        st.m = top;
+      }
+    }
+  }
+  if (kw > 0 || m >= M) return;
+  const int64_t slot = (int64_t)item * ROWS + 16 * rw + r;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.p_o + slot * D + 16 * dt + 4 * q4) = st.acc[dt];
+  if (q4 == 0) a.p_m[slot] = st.m, a.p_l[slot] = l;
+}
+
+// An own item: each wave takes every eighth tile of 32 keys, K straight into the operand's registers, V through LDS of its own.
+template <int D, int MODE>
+__device__ __forceinline__ void own_item(const PrefixArgs& a, char* smem, int index) {
+  constexpr int KS = D / 32, DT = D / 16, P = D + 8, W = kPrefixWaves;
+  constexpr int VCH = MODE == 0 ? 8 : 16, VPK = D / VCH, VL = 32 * VPK / 64;  // 16-byte parts of V: a key's, a lane's
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pairs = a.S * a.Hkv, sp = index / pairs, pair = index - sp * pairs, h = pair / a.S, s = pair - h * a.S;
+  const OwnKeys own = own_keys(a, s);
+  if (sp >= own.splits) return;
+  const int lo_key = own.shared + sp * own.chunk, end = min(lo_key + own.chunk, own.ctx), G = a.G;
+  const int32_t* table = a.bt + (int64_t)s * a.bt_ss;
+  const int last_col = min((end - 1) >> a.log_b, a.bt_w - 1);
+  bf16x8 qop[KS];
+#pragma unroll
+  for (int j = 0; j < KS; ++j)
+    qop[j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(a.q + (int64_t)s * a.q_ss + (int64_t)(h * G + min(r, G - 1)) * a.q_sh +
+                                                        32 * j + 8 * q4));
+  const float inv_scale_log2 = MODE == 0 ? 1.f / a.scale_log2 : 1.f;
+  RowState<D> st;
+  st.clear();
+  uint16_t* sv = (uint16_t*)smem + wave * 32 * P;
+  const int tr_off = tr16_offset(r, q4, P);
+  const bf16x8 ones = bf16_ones();
+  const int ntiles = (end - lo_key + 31) / 32;
+  u32x4 rk[2][2][KS], rv[2][VL];
+  f32x4 rks[2][2], rvs[2][2];
+  // the ids of a tile's two halves of 16 keys, each inside one block; tiles past the end read the last block again
+  auto ids = [&](int t, int (&id)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = min((lo_key + 32 * t + 16 * i) >> a.log_b, last_col);
+      id[i] = __builtin_amdgcn_readfirstlane(min(max(table[col], 0), a.nb - 1));
+    }
+  };
+  auto load = [&](int set, int t, const int (&id)[2]) {
+    const int inside = (1 << a.log_b) - 1;
+    int64_t base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      base[i] = (int64_t)h * a.kv_sh + (int64_t)id[i] * a.kv_sn + ((lo_key + 32 * t + 16 * i) & inside) * D;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const int64_t e = base[mt] + r * D + 32 * j + 8 * q4;
+        if constexpr (MODE == 0) {
+          rk[set][mt][j] = *(const u32x4*)((const uint16_t*)a.k + e);
+        } else {
+          const u32x2 c = *(const u32x2*)((const uint8_t*)a.k + e);
+          rk[set][mt][j] = u32x4{c[0], c[1], 0, 0};
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int c = lane + 64 * i, key = c / VPK;
+      const int64_t e = (key < 16 ? base[0] : base[1]) + (key & 15) * D + VCH * (c % VPK);
+      rv[set][i] = *(const u32x4*)((const uint8_t*)a.v + e * (MODE == 0 ? 2 : 1));
+    }
+    if constexpr (MODE == 1) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const int off = ((lo_key + 32 * t + 16 * mt) & inside) + 4 * q4;
+        rks[set][mt] = four_scales(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + (int64_t)id[mt] * a.ks_sn + off);
+        rvs[set][mt] = four_scales(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + (int64_t)id[mt] * a.vs_sn + off);
+      }
+    }
+  };
+  auto tile = [&](int set, int t) {
+    const int x0 = lo_key + 32 * t;
+    if (t >= ntiles) return;
+    wave_sync();  // the last tile's reads of V
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int c = lane + 64 * i, key = c / VPK;
+      u32x4 v = rv[set][i];
+      if (x0 + key >= end) v = u32x4{0, 0, 0, 0};
+      uint16_t* to = sv + key * P + VCH * (c % VPK);
+      if constexpr (MODE == 0) {
+        *(u32x4*)to = v;
+      } else {
+        *(u32x4*)to = tree_codes(v[0], v[1]);
+        *(u32x4*)(to + 8) = tree_codes(v[2], v[3]);
+      }
+    }
+    f32x4 sc[2], vs[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const u32x4 k = MODE == 0 ? rk[set][mt][j] : tree_codes(rk[set][mt][j][0], rk[set][mt][j][1]);
+        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), qop[j], sc[mt], 0, 0, 0);
+      }
+      if constexpr (MODE == 1) {
+        sc[mt] *= rks[set][mt] * a.scale_log2;
+        vs[mt] = rvs[set][mt];
+      }
+    }
+    if (x0 + 32 > end) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (x0 + 16 * mt + 4 * q4 + i >= end) sc[mt][i] = kNegInf;
+    }
+    u32x4 hi[1], lo[1];
+    st.template add<MODE, 32>(sc, a.scale_log2, inv_scale_log2, ones, vs, hi, lo);
+    wave_sync();  // V has been stored
+    st.template product<32>(sv, tr_off, P, hi, lo);
+  };
+  int id[2];
+  ids(wave, id);
+  load(0, wave, id);
+  ids(wave + W, id);
+  for (int t = wave; t < ntiles; t += 2 * W) {
+    load(1, t + W, id);
+    ids(t + 2 * W, id);
+    tile(0, t);
+    load(0, t + 2 * W, id);
+    ids(t + 3 * W, id);
+    tile(1, t + W);
+  }
+  float l = st.sum(MODE);
+  if (l != l) st.m = 0.f;
+  __syncthreads();  // every wave is done with its V
+  constexpr int MP = D + 4;
+  float2* ml = (float2*)smem;            // [wave][16] (m, l)
+  float* accs = (float*)(ml + W * 16);  // [wave][16][MP]
+  if (q4 == 0) ml[wave * 16 + r] = float2{st.m, l};
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *(f32x4*)(accs + (wave * 16 + r) * MP + 16 * dt + 4 * q4) = st.acc[dt];
+  __syncthreads();
+  const int waves = min(ntiles, W);
+  const int64_t first = ((int64_t)pair * a.nsplit + sp) * G;
+  for (int i = tid; i < G * (D / 4); i += kPrefixThreads) {
+    const int g = i / (D / 4), c = i % (D / 4);
+    float M = kNegInf, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < waves; ++w) M = fmaxf(M, ml[w * 16 + g].x);
+    for (int w = 0; w < waves; ++w) {
+      const float2 x = ml[w * 16 + g];
+      const float e = M == kNegInf ? 0.f : fast_exp2(x.x - M);
+      L += e * x.y;
+      O += e * *(const f32x4*)(accs + (w * 16 + g) * MP + 4 * c);
+    }
+    *(f32x4*)(a.s_o + (first + g) * D + 4 * c) = O;
+    if (c == 0) a.s_m[first + g] = M, a.s_l[first + g] = L;
+  }
+}
+
+template <int D, int MODE, int KW, int NPRE>
+__global__ void __launch_bounds__(kPrefixThreads, 2) prefix_attention_kernel(const PrefixArgs a) {
+  __shared__ __align__(16) char smem[PrefixSmem<D, KW>::kBytes];
+  __shared__ __align__(16) float sscale[MODE == 0 ? 1 : 2][2][64 * KW];
+  __shared__ int bids[kPrefixMaxChunk / 16];
+  if ((int)blockIdx.x < a.num_items) prefix_item<D, MODE, KW, NPRE>(a, smem, sscale, bids);
+  else own_item<D, MODE>(a, smem, (int)blockIdx.x - a.num_items);
+}
+
+// Thread (row, 4 channels): joins the row's parts. A row without any key gets zeros.
+template <int D>
+__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
+  constexpr int Q = D / 4, U = 8;
+  const int at = blockIdx.x * 256 + threadIdx.x, row = at / Q, c = at % Q, Hq = a.Hkv * a.G;
+  if (row >= a.S * Hq) return;
+  const int s = row / Hq, hq = row - s * Hq, h = hq / a.G, g = hq - h * a.G;
+  const OwnKeys own = own_keys(a, s);
+  const int32_t* info = a.rows + 8 * (int64_t)s;
+  const int np = own.shared > 0 ? info[3] : 0, m = info[1] + g, tile = m / a.tile_rows;
+  const int64_t p0 = ((int64_t)info[2] + (int64_t)(h * info[4] + tile) * np) * a.tile_rows + (m - tile * a.tile_rows);
+  const int64_t s0 = (int64_t)(h * a.S + s) * a.nsplit * a.G + g;
+  const int n = np + own.splits;
+  auto part = [&](int j) { return j < np ? p0 + (int64_t)j * a.tile_rows : s0 + (int64_t)(j - np) * a.G; };
+  float M = kNegInf, L = 0.f;
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < n; j0 += U) {
+    float ms[U], ls[U];
+    f32x4 os[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u, n - 1);
+      const int64_t i = part(j);
+      ms[u] = (j < np ? a.p_m : a.s_m)[i];
+      ls[u] = (j < np ? a.p_l : a.s_l)[i];
+      os[u] = *(const f32x4*)((j < np ? a.p_o : a.s_o) + i * D + 4 * c);
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, j0 + u < n ? ms[u] : kNegInf);
+    if (top == kNegInf) continue;
+    const float f = fast_exp2(M - top);
+    L *= f;
+    O *= f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j0 + u >= n || ms[u] == kNegInf) continue;  // a part without a key for the row
+      const float e = fast_exp2(ms[u] - top);
+      L += e * ls[u];
+      O += e * os[u];
+    }
+    M = top;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *(u32x2*)(a.out + (int64_t)s * a.o_ss + (int64_t)hq * a.o_sh + 4 * c) =
+      u32x2{pack_bf16x2(O[0] * inv, O[1] * inv), pack_bf16x2(O[2] * inv, O[3] * inv)};
+}
+
+}  // namespace sipa
+
+using namespace sipa;
+
+static int prefix_check(const sipa_prefix_params* p) {
+  SIPA_CHECK(p != nullptr && p->struct_size == (int32_t)sizeof(sipa_prefix_params), SIPA_EINVAL,
+             "struct_size does not match this library's sipa_prefix_params (%d bytes)", (int)sizeof(sipa_prefix_params));
+  SIPA_CHECK(p->num_seqs >= 0 && p->num_kv_heads > 0 && p->num_q_heads > 0 && p->num_q_heads % p->num_kv_heads == 0, SIPA_EINVAL,
+             "bad sequence or head counts");
+  SIPA_CHECK(p->num_q_heads / p->num_kv_heads <= kMaxGroup, SIPA_EUNSUPPORTED, "GQA group %d > %d",
+             p->num_q_heads / p->num_kv_heads, kMaxGroup);
+  SIPA_CHECK(p->head_dim == 64 || p->head_dim == 128, SIPA_EUNSUPPORTED, "head_dim %d not in {64, 128}", p->head_dim);
+  SIPA_CHECK(p->block_size == 16 || p->block_size == 32 || p->block_size == 64, SIPA_EUNSUPPORTED,
+             "block_size %d not in {16, 32, 64}", p->block_size);
+  SIPA_CHECK(p->max_context > 0 && p->max_context <= 1 << 24, SIPA_EUNSUPPORTED, "max_context %d outside [1, 2^24]", p->max_context);
+  SIPA_CHECK(p->kv_mode == SIPA_KV_PLAIN || p->kv_mode == SIPA_KV_INT8_TOKEN, SIPA_EUNSUPPORTED, "kv_mode %d", p->kv_mode);
+  SIPA_CHECK((int64_t)p->num_seqs * p->num_q_heads * p->head_dim <= 0x3fffffff, SIPA_EUNSUPPORTED, "%d sequences of %d heads",
+             p->num_seqs, p->num_q_heads);
+  return SIPA_OK;
+}
+
+struct PrefixLayout {
+  int64_t p_m, p_l, p_o, s_m, s_l, s_o, total;
+};
+
+static PrefixLayout prefix_workspace(const sipa_prefix_params* p, const sipa_prefix_layout& l) {
+  auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  const int64_t pr = (int64_t)l.num_items * l.tile_rows, sr = (int64_t)p->num_seqs * p->num_q_heads * l.own_splits;
+  PrefixLayout w;
+  w.p_m = 0;
+  w.p_l = w.p_m + up(pr * 4);
+  w.p_o = w.p_l + up(pr * 4);
+  w.s_m = w.p_o + up(pr * p->head_dim * 4);
+  w.s_l = w.s_m + up(sr * 4);
+  w.s_o = w.s_l + up(sr * 4);
+  w.total = w.s_o + up(sr * p->head_dim * 4);
+  return w;
+}
+
+extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_groups, const int32_t* group_starts,
+                                    const int32_t* members, const int32_t* tokens, const int32_t* context_lens,
+                                    int32_t* plan, int64_t capacity, sipa_prefix_layout* layout) {
+  int rc = prefix_check(p);
+  if (rc != SIPA_OK) return rc;
+  SIPA_CHECK(layout != nullptr && num_groups >= 0 && (num_groups == 0 || (group_starts && members && tokens)), SIPA_EINVAL,
+             "NULL pointer or negative group count");
+  const int S = p->num_seqs, G = p->num_q_heads / p->num_kv_heads, H = p->num_kv_heads;
+  SIPA_CHECK(num_groups == 0 || group_starts[0] == 0, SIPA_EINVAL, "group_starts begin at %d", num_groups ? group_starts[0] : 0);
+  // groups that share anything: two members at least, one block
+  auto count_of = [&](int g) { return group_starts[g + 1] - group_starts[g]; };
+  auto shares = [&](int g) { return count_of(g) >= 2 && tokens[g] > 0; };
+  int64_t most_rows = 0, shared_min = p->max_context;
+  int64_t grouped = 0;
+  for (int g = 0; g < num_groups; ++g) {
+    SIPA_CHECK(count_of(g) >= 0 && group_starts[g + 1] <= S, SIPA_EINVAL, "group %d has rows %d .. %d of %d", g, group_starts[g],
+               group_starts[g + 1], S);
+    SIPA_CHECK(tokens[g] >= 0 && tokens[g] <= p->max_context && tokens[g] % p->block_size == 0, SIPA_EINVAL,
+               "group %d shares %d tokens: whole blocks of %d within max_context %d", g, tokens[g], p->block_size, p->max_context);
+    if (!shares(g)) continue;
+    most_rows = std::max<int64_t>(most_rows, (int64_t)count_of(g) * G);
+    shared_min = std::min<int64_t>(shared_min, tokens[g]);
+    grouped += count_of(g);
+  }
+  const int num_members = num_groups ? group_starts[num_groups] : 0;
+  const int cus = sipa_device_cu_count(-1);
+  if (cus < 0) return cus;
+  sipa_prefix_layout l = {};
+  l.tile_rows = most_rows <= 64 ? 64 : 128;
+  const int kt = l.tile_rows == 64 ? 128 : 64;
+  auto tiles_of = [&](int g) { return ((int64_t)count_of(g) * G + l.tile_rows - 1) / l.tile_rows; };
+  int64_t work = 0;  // keys times row tiles
+  for (int g = 0; g < num_groups; ++g)
+    if (shares(g)) work += (int64_t)H * tiles_of(g) * tokens[g];
+  const int64_t share = std::max<int64_t>(256, (work + cus - 1) / cus);
+  auto splits_of = [&](int g) {
+    const int64_t n = std::max<int64_t>((tokens[g] + share - 1) / share, (tokens[g] + kPrefixMaxChunk - 1) / kPrefixMaxChunk);
+    const int64_t chunk = ((tokens[g] + n - 1) / n + kt - 1) / kt * kt;
+    return std::pair<int64_t, int64_t>((tokens[g] + chunk - 1) / chunk, chunk);
+  };
+  int64_t items = 0;
+  for (int g = 0; g < num_groups; ++g)
+    if (shares(g)) items += H * tiles_of(g) * splits_of(g).first;
+  // the sequences' own keys
+  int64_t longest = grouped == S && S > 0 ? p->max_context - shared_min : p->max_context;
+  const int64_t pairs = (int64_t)S * H;
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((longest + 255) / 256, 2 * cus / std::max<int64_t>(pairs, 1)));
+  l.own_chunk = (int)(((longest + n - 1) / n + 63) / 64 * 64);
+  l.own_chunk = std::max(l.own_chunk, 64);
+  l.own_splits = (int)std::max<int64_t>(1, (longest + l.own_chunk - 1) / l.own_chunk);
+  SIPA_CHECK(items + pairs * l.own_splits <= 0x7fffffff && items * l.tile_rows <= 0x7fffffff, SIPA_EUNSUPPORTED,
+             "%lld items exceed the grid limit", (long long)(items + pairs * l.own_splits));
+  l.num_items = (int)items;
+  l.num_members = num_members;
+  l.plan_ints = 8 * items + 8 * (int64_t)S + num_members;
+  l.workspace_bytes = prefix_workspace(p, l).total;
+  *layout = l;
+  if (plan == nullptr) return SIPA_OK;
+  SIPA_CHECK(capacity >= l.plan_ints, SIPA_EINVAL, "the plan takes %lld values, room for %lld", (long long)l.plan_ints,
+             (long long)capacity);
+  int32_t* rows = plan + 8 * items;
+  for (int64_t i = 0; i < 8 * (int64_t)S; ++i) rows[i] = i % 8 == 7 ? -1 : 0;
+  int64_t at = 0;
+  for (int g = 0; g < num_groups; ++g) {
+    const int a0 = group_starts[g], count = count_of(g);
+    for (int i = 0; i < count; ++i) {
+      const int s = members[a0 + i];
+      SIPA_CHECK(s >= 0 && s < S, SIPA_EINVAL, "group %d has row %d of %d", g, s, S);
+      SIPA_CHECK(rows[8 * (int64_t)s + 7] < 0, SIPA_EINVAL, "row %d in two groups, or twice in one", s);
+      rows[8 * (int64_t)s + 7] = g;
+    }
+    if (!shares(g)) continue;
+    const int64_t tiles = tiles_of(g);
+    const auto [np, chunk] = splits_of(g);
+    for (int i = 0; i < count; ++i) {
+      int32_t* r = rows + 8 * (int64_t)members[a0 + i];
+      r[0] = tokens[g], r[1] = i * G, r[2] = (int)at, r[3] = (int)np, r[4] = (int)tiles;
+    }
+    for (int h = 0; h < H; ++h)
+      for (int64_t t = 0; t < tiles; ++t)
+        for (int64_t x = 0; x < np; ++x) {
+          int32_t* it = plan + 8 * at++;
+          it[0] = members[a0], it[1] = a0, it[2] = count * G, it[3] = (int)(t * l.tile_rows);
+          it[4] = h, it[5] = (int)(x * chunk), it[6] = (int)std::min<int64_t>((x + 1) * chunk, tokens[g]), it[7] = 0;
+        }
+  }
+  for (int i = 0; i < num_members; ++i) rows[8 * (int64_t)S + i] = members[i];
+  return SIPA_OK;
+}
+
+template <int D, int MODE>
+static void launch_prefix(int tile_rows, dim3 grid, hipStream_t st, const PrefixArgs& a) {
+  constexpr int NPRE = D == 64 ? 4 : 3;
+  if (tile_rows == 64) hipLaunchKernelGGL((prefix_attention_kernel<D, MODE, 2, NPRE>), grid, dim3(kPrefixThreads), 0, st, a);
+  else hipLaunchKernelGGL((prefix_attention_kernel<D, MODE, 1, NPRE>), grid, dim3(kPrefixThreads), 0, st, a);
+  const int threads = a.S * a.Hkv * a.G * (D / 4);
+  hipLaunchKernelGGL((prefix_merge_kernel<D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+}
+
+extern "C" int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stream) {
+  int rc = prefix_check(p);
+  if (rc != SIPA_OK) return rc;
+  if (p->num_seqs == 0) return SIPA_OK;
+  SIPA_CHECK(p->scale > 0.f && p->scale < __builtin_inff(), SIPA_EINVAL,
+             "scale %g must be positive and finite (the kernel takes maxima of the unscaled scores)", (double)p->scale);
+  SIPA_CHECK(p->bt_width > 0 && (int64_t)p->bt_width * p->block_size >= p->max_context, SIPA_EINVAL,
+             "block_tables rows of %d entries cannot cover max_context %d", p->bt_width, p->max_context);
+  SIPA_CHECK(p->q && p->k_cache && p->v_cache && p->block_tables && p->context_lens && p->out && p->plan && p->num_blocks > 0,
+             SIPA_EINVAL, "NULL pointer or empty pool");
+  SIPA_CHECK(((uintptr_t)p->q & 15) == 0 && p->q_stride_s % 8 == 0 && p->q_stride_h % 8 == 0, SIPA_EINVAL,
+             "q rows must be 16-byte aligned");
+  SIPA_CHECK(((uintptr_t)p->out & 7) == 0 && p->out_stride_s % 4 == 0 && p->out_stride_h % 4 == 0, SIPA_EINVAL,
+             "out rows must be 8-byte aligned");
+  const bool int8 = p->kv_mode == SIPA_KV_INT8_TOKEN;
+  const int per16 = int8 ? 16 : 8;
+  SIPA_CHECK((((uintptr_t)p->k_cache | (uintptr_t)p->v_cache) & 15) == 0 && p->kv_stride_h % per16 == 0 &&
+                 p->kv_stride_n % per16 == 0, SIPA_EINVAL, "K/V pools must be 16-byte aligned");
+  SIPA_CHECK(p->kv_stride_n >= 0 && p->kv_stride_n <= 0x7fffffff, SIPA_EUNSUPPORTED, "blocks %lld elements apart",
+             (long long)p->kv_stride_n);
+  if (int8) {
+    SIPA_CHECK(p->k_scale && p->v_scale, SIPA_EINVAL, "INT8 pools need k_scale and v_scale");
+    SIPA_CHECK((p->k_scale_dtype == SIPA_F16 || p->k_scale_dtype == SIPA_F32) &&
+                   (p->v_scale_dtype == SIPA_F16 || p->v_scale_dtype == SIPA_F32),
+               SIPA_EUNSUPPORTED, "scales must be fp16 or fp32");
+    SIPA_CHECK(((uintptr_t)p->k_scale % (p->k_scale_dtype == SIPA_F32 ? 4 : 2)) == 0 &&
+                   ((uintptr_t)p->v_scale % (p->v_scale_dtype == SIPA_F32 ? 4 : 2)) == 0, SIPA_EINVAL,
+               "scales must be aligned to their element size");
+  }
+  const sipa_prefix_layout& l = p->layout;
+  SIPA_CHECK((l.tile_rows == 64 || l.tile_rows == 128) && l.num_items >= 0 && l.num_members >= 0 && l.own_splits >= 1 &&
+                 l.own_chunk >= 64 && l.own_chunk % 64 == 0 && ((uintptr_t)p->plan & 15) == 0 &&
+                 (int64_t)p->num_seqs * p->num_kv_heads * l.own_splits + l.num_items <= 0x7fffffff,
+             SIPA_EINVAL, "the layout is not one of sipa_prefix_plan");
+  const PrefixLayout w = prefix_workspace(p, l);
+  SIPA_CHECK(p->workspace != nullptr && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= w.total, SIPA_EWORKSPACE,
+             "a 256-byte aligned workspace of %lld bytes is needed (have %lld)", (long long)w.total, (long long)p->workspace_bytes);
+  PrefixArgs a;
+  a.q = (const uint16_t*)p->q;
+  a.q_ss = p->q_stride_s;
+  a.q_sh = p->q_stride_h;
+  a.k = p->k_cache;
+  a.v = p->v_cache;
+  a.kv_sh = p->kv_stride_h;
+  a.kv_sn = p->kv_stride_n;
+  a.bt = p->block_tables;
+  a.bt_ss = p->bt_stride_s;
+  a.bt_w = p->bt_width;
+  a.ctx = p->context_lens;
+  a.out = (uint16_t*)p->out;
+  a.o_ss = p->out_stride_s;
+  a.o_sh = p->out_stride_h;
+  a.ks = p->k_scale;
+  a.vs = p->v_scale;
+  a.ks_f32 = p->k_scale_dtype == SIPA_F32;
+  a.vs_f32 = p->v_scale_dtype == SIPA_F32;
+  a.ks_sh = p->ks_stride_h;
+  a.ks_sn = p->ks_stride_n;
+  a.vs_sh = p->vs_stride_h;
+  a.vs_sn = p->vs_stride_n;
+  a.items = p->plan;
+  a.rows = p->plan + 8 * (int64_t)l.num_items;
+  a.members = a.rows + 8 * (int64_t)p->num_seqs;
+  a.num_items = l.num_items;
+  a.num_members = l.num_members;
+  a.S = p->num_seqs;
+  a.Hkv = p->num_kv_heads;
+  a.G = p->num_q_heads / p->num_kv_heads;
+  a.nb = p->num_blocks;
+  a.max_ctx = p->max_context;
+  a.log_b = p->block_size == 16 ? 4 : p->block_size == 32 ? 5 : 6;
+  a.nsplit = l.own_splits;
+  a.chunk = l.own_chunk;
+  a.tile_rows = l.tile_rows;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  char* ws = (char*)p->workspace;
+  a.p_m = (float*)(ws + w.p_m);
+  a.p_l = (float*)(ws + w.p_l);
+  a.p_o = (float*)(ws + w.p_o);
+  a.s_m = (float*)(ws + w.s_m);
+  a.s_l = (float*)(ws + w.s_l);
+  a.s_o = (float*)(ws + w.s_o);
+  const dim3 grid((unsigned)(l.num_items + (int64_t)p->num_seqs * p->num_kv_heads * l.own_splits));
+  hipStream_t st = (hipStream_t)stream;
+  if (p->head_dim == 64) {
+    if (int8) launch_prefix<64, 1>(l.tile_rows, grid, st, a);
+    else launch_prefix<64, 0>(l.tile_rows, grid, st, a);
+  } else {
+    if (int8) launch_prefix<128, 1>(l.tile_rows, grid, st, a);
+    else launch_prefix<128, 0>(l.tile_rows, grid, st, a);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(SIPA_EHIP, "prefix attention launch failed: %s", hipGetErrorString(e));
+  return SIPA_OK;
+}

@@ -28,8 +28,6 @@
 
 namespace sipa {
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kTreeMaxSplits = 128;
 constexpr int kTreeMaxChunk = 16384;  // block ids of a split in LDS: 4 KB
 constexpr int kTreeMaxGroup = 64;
@@ -64,27 +62,6 @@ struct TreeArgs {
   float* pl;               // the same
   float* part;             // [units][nsplit][rows of a group][D]
 };
-
-// A scale as it lies in memory, and its value: apart, so that the load is waited for only where the value is needed.
-__device__ __forceinline__ uint32_t scale_bits(const void* base, bool f32, int64_t i) {
-  return f32 ? ((const uint32_t*)base)[i] : (uint32_t)((const uint16_t*)base)[i];
-}
-
-__device__ __forceinline__ float scale_value(uint32_t bits, bool f32) {
-  return f32 ? __uint_as_float(bits) : f16_bits_to_f32(bits);
-}
-
-// Eight int8 codes (two words) as bf16, exactly.
-__device__ __forceinline__ u32x4 tree_codes(uint32_t w0, uint32_t w1) {
-  u32x4 x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? w0 : w1;
-    const int b = 16 * (i & 1);
-    x[i] = pack_bf16x2((float)(int8_t)(w >> b), (float)(int8_t)(w >> (b + 8)));
-  }
-  return x;
-}
 
 // MR row tiles of 16 per wave, RW waves side by side over the rows, KW waves one after the other over the keys, each KPW
 // keys of a stage of KW KPW; NPRE stages in flight in registers.

@@ -160,6 +160,47 @@ class LogitsParams(ctypes.Structure):
     ]
 
 
+class PrefixLayout(ctypes.Structure):
+    """Mirror of struct sipa_prefix_layout."""
+    _fields_ = [
+        ("num_items", i32), ("num_members", i32), ("tile_rows", i32), ("own_splits", i32), ("own_chunk", i32),
+        ("plan_ints", i64), ("workspace_bytes", i64),
+    ]
+
+
+class PrefixParams(ctypes.Structure):
+    """Mirror of struct sipa_prefix_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_seqs", i32), ("num_q_heads", i32), ("num_kv_heads", i32), ("head_dim", i32),
+        ("block_size", i32), ("num_blocks", i32), ("max_context", i32), ("kv_mode", i32), ("scale", f32),
+        ("q", vp), ("q_stride_s", i64), ("q_stride_h", i64),
+        ("k_cache", vp), ("v_cache", vp), ("kv_stride_h", i64), ("kv_stride_n", i64),
+        ("block_tables", vp), ("bt_stride_s", i64), ("bt_width", i32), ("context_lens", vp),
+        ("out", vp), ("out_stride_s", i64), ("out_stride_h", i64),
+        ("k_scale", vp), ("k_scale_dtype", i32), ("ks_stride_h", i64), ("ks_stride_n", i64),
+        ("v_scale", vp), ("v_scale_dtype", i32), ("vs_stride_h", i64), ("vs_stride_n", i64),
+        ("layout", PrefixLayout), ("plan", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class BeamParams(ctypes.Structure):
+    """Mirror of struct sipa_beam_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_rows", i32), ("vocab", i32), ("num_groups", i32), ("beams", i32),
+        ("num_candidates", i32), ("dtype", i32), ("logits", vp), ("logits_stride", i64), ("scores", vp), ("starts", vp),
+        ("out_scores", vp), ("out_beams", vp), ("out_tokens", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class CopyParams(ctypes.Structure):
+    """Mirror of struct sipa_copy_params."""
+    _fields_ = [
+        ("struct_size", i32), ("num_layers", i32), ("num_kv_heads", i32), ("num_blocks", i32), ("block_size", i32),
+        ("num_pools", i32), ("pools", vp * 4), ("stride_l", i64 * 4), ("stride_h", i64 * 4), ("row_bytes", i32 * 4),
+        ("copies", vp), ("num_copies", i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "sipa_abi_version": (i32, []),
@@ -203,6 +244,12 @@ SIGNATURES = {
     "sipa_capture_id": (_c.c_uint64, [vp]),
     "sipa_tree_maps": (i32, [vp, vp]),  # a packed or ctypes TreeMapsParams
     "sipa_commit_tokens": (i32, [vp, vp]),  # a packed or ctypes CommitParams
+    "sipa_prefix_plan": (i32, [_c.POINTER(PrefixParams), i32, vp, vp, vp, vp, vp, i64, _c.POINTER(PrefixLayout)]),
+    "sipa_prefix_attention": (i32, [_c.POINTER(PrefixParams), vp]),
+    "sipa_beam_workspace_bytes": (i64, [_c.POINTER(BeamParams)]),
+    "sipa_beam_select": (i32, [_c.POINTER(BeamParams), vp]),
+    "sipa_check_copies": (i32, [vp, i32, i32, i32]),
+    "sipa_copy_blocks": (i32, [_c.POINTER(CopyParams), vp]),
 }
 
 _lib = None

@@ -7,6 +7,9 @@ must be bit-exact with it:
     back in reverse table order, so the next allocation receives them in their old table order, and long-lived
     pools end up with scattered, non-monotonic tables;
   - per-block reference counts (0 or 1 without sharing), free listeners, OutOfBlocks leaves state unchanged.
+
+Sequences that hold the same tokens can share blocks (fork, reorder; the reference never does). Only full blocks are shared, so
+that a sequence's next token always goes to a block of its own: a last block that is not full is copied.
 """
 
 from __future__ import annotations
@@ -29,6 +32,7 @@ class BlockManager:
         # The top of the stack is the end of the list: block 0 is handed out first.
         self._free: list[int] = list(reversed(range(num_blocks)))
         self._ref = [0] * num_blocks
+        self._shared = 0  # blocks that several sequences hold
         self._tables: dict[int, list[int]] = {}
         self._lengths: dict[int, int] = {}
         # int32 mirror of every table (capacity doubles as it grows), so per-forward metadata is built with array
@@ -63,6 +67,20 @@ class BlockManager:
     def ref_count(self, block: int) -> int:
         """Sequences holding `block`."""
         return self._ref[block]
+
+    def num_shared_blocks(self) -> int:
+        """Blocks that several sequences hold."""
+        return self._shared
+
+    def check_own(self, seq_id: int, start: int, n: int) -> None:
+        """ValueError if other sequences hold a block of positions start .. start + n - 1 too: what a forward wrote there
+        would be theirs as well."""
+        if self._shared:
+            B = self.block_size
+            for block in self._tables[seq_id][start // B:(start + n - 1) // B + 1]:
+                if self._ref[block] > 1:
+                    raise ValueError(f"sequence {seq_id}: a forward over positions {start} .. {start + n - 1} would write to block "
+                                     f"{block}, which {self._ref[block]} sequences hold")
 
     def block_table(self, seq_id: int) -> list[int]:
         """The sequence's blocks in token order (a copy)."""
@@ -167,11 +185,15 @@ class BlockManager:
     def truncate(self, seq_id: int, n_tokens: int) -> None:
         """Keep the first n_tokens of seq_id (drafted tokens that were not accepted are given up); the blocks past them
         return to the stack, last block first, and free listeners hear of them. An int8-kchannel cache refuses to keep part of
-        a block that it has quantized. No counterpart in the reference."""
+        a block that it has quantized; no part of a block that other sequences hold can be kept. No counterpart in the
+        reference."""
         if not 0 <= n_tokens <= self._lengths[seq_id]:
             raise ValueError(f"sequence {seq_id} holds {self._lengths[seq_id]} tokens, {n_tokens} to keep")
         table, keep = self._tables[seq_id], self.blocks_for(n_tokens)
         if n_tokens % self.block_size and n_tokens < self._lengths[seq_id]:
+            if self._ref[table[keep - 1]] > 1:
+                raise ValueError(f"sequence {seq_id}: {n_tokens} tokens end inside block {table[keep - 1]}, which "
+                                 f"{self._ref[table[keep - 1]]} sequences hold; truncate to a multiple of the block size")
             for fn in self._truncate_checks:
                 fn(table[keep - 1])
         self._lengths[seq_id] = n_tokens
@@ -186,6 +208,7 @@ class BlockManager:
             self._ref[b] -= 1
             if self._ref[b] < 0:
                 raise AssertionError(f"block {b} released more often than it was taken")
+            self._shared -= self._ref[b] == 1
             if self._ref[b] == 0:
                 self._free.append(b)
                 released.append(b)
@@ -200,6 +223,91 @@ class BlockManager:
         self._release(table[::-1])  # last block first, so the stack hands the blocks out again in table order
         for fn in self._table_listeners:
             fn(seq_id, -1)
+
+    # ---- sharing -------------------------------------------------------------------------------------------------
+
+    def _take(self, blocks: list[int]) -> None:
+        """One more holder for each block."""
+        for b in blocks:
+            self._ref[b] += 1
+            self._shared += self._ref[b] == 2
+
+    def _set_table(self, seq_id: int, table: list[int], n_tokens: int) -> None:
+        """Give a sequence another table (an array of its own: metadata built before keeps the old one)."""
+        old = self._tables.get(seq_id)
+        first = 0
+        if old is not None:
+            while first < min(len(old), len(table)) and old[first] == table[first]:
+                first += 1
+        self._tables[seq_id], self._lengths[seq_id] = table, n_tokens
+        arr = self._arrays[seq_id] = np.empty(max(16, 2 * len(table)), dtype=np.int32)
+        arr[:len(table)] = table
+        if old is None or first < len(table):
+            for fn in self._table_listeners:
+                fn(seq_id, first)
+
+    def fork(self, seq_id: int, new_ids: list[int]) -> list[tuple[int, int, int]]:
+        """Create new_ids, each holding the tokens of seq_id: its full blocks are shared, its last one, if it is not full, is
+        a block of their own for each. Returns the copies to make, (from block, to block, tokens), before anything is
+        written to or read from the new sequences (PagedKVCache.copy_blocks)."""
+        table, n = self._tables[seq_id], self._lengths[seq_id]
+        if len(set(new_ids)) != len(new_ids) or any(i in self._tables for i in new_ids):
+            raise ValueError(f"new sequences {new_ids} must be distinct and not live yet")
+        full, rest = divmod(n, self.block_size)
+        need = len(new_ids) if rest else 0
+        if need > len(self._free):
+            raise OutOfBlocks(f"{len(new_ids)} forks of sequence {seq_id} take {need} blocks; the pool has {len(self._free)} free")
+        own = self._pop_blocks(need)
+        for i, new in enumerate(new_ids):
+            self._take(table[:full])
+            self._set_table(new, table[:full] + own[i:i + 1], n)
+        return [(table[full], b, rest) for b in own]
+
+    def reorder(self, seq_ids: list[int], parents: list[int]) -> list[tuple[int, int, int]]:
+        """Sequence seq_ids[i] goes on from what seq_ids[parents[i]] holds (beams after a selection): it gives up its own
+        blocks and shares that one's full ones; a last block that is not full stays with one of them, and the others get
+        copies. Returns the copies to make, as fork does. No more blocks are held afterwards than len(seq_ids) tables of the
+        longest would take; OutOfBlocks and ValueError leave everything as it was."""
+        if len(set(seq_ids)) != len(seq_ids) or len(parents) != len(seq_ids):
+            raise ValueError(f"{len(parents)} parents of {len(seq_ids)} sequences, which must be distinct")
+        if any(not 0 <= p < len(seq_ids) for p in parents):
+            raise ValueError(f"parents {parents} of {len(seq_ids)} sequences")
+        tables, lengths = [self._tables[s] for s in seq_ids], [self._lengths[s] for s in seq_ids]
+        # who keeps the last block: the sequence itself if it goes on, else the first that goes on from it
+        keeper: dict[int, int] = {}
+        for i, p in enumerate(parents):
+            if i == p or p not in keeper:
+                keeper[p] = i
+        moved = [i for i, p in enumerate(parents) if i != p]
+        taken, copied = [], []
+        for i in moved:
+            p = parents[i]
+            full, rest = divmod(lengths[p], self.block_size)
+            taken.append(tables[p][:full] if rest and keeper[p] != i else tables[p][:])
+            if rest and keeper[p] != i:
+                copied.append(i)
+        change: dict[int, int] = {}
+        for i, blocks in zip(moved, taken):
+            for b in tables[i]:
+                change[b] = change.get(b, 0) - 1
+            for b in blocks:
+                change[b] = change.get(b, 0) + 1
+        room = len(self._free) + sum(self._ref[b] + c == 0 for b, c in change.items())
+        if len(copied) > room:
+            raise OutOfBlocks(f"{len(copied)} copies of last blocks; the pool has {room} blocks for them")
+        for blocks in taken:
+            self._take(blocks)
+        for i in moved:
+            self._release(tables[i][::-1])
+        own = dict(zip(copied, self._pop_blocks(len(copied))))
+        copies = []
+        for i, blocks in zip(moved, taken):
+            p = parents[i]
+            if i in own:
+                copies.append((tables[p][-1], own[i], lengths[p] % self.block_size))
+                blocks = [*blocks, own[i]]
+            self._set_table(seq_ids[i], blocks, lengths[p])
+        return copies
 
     # ---- checking ------------------------------------------------------------------------------------------------
 
@@ -220,6 +328,10 @@ class BlockManager:
             if self._arrays[seq_id][:len(table)].tolist() != table:
                 fail(f"the int32 mirror of sequence {seq_id} is out of date")
             np.add.at(owners, np.asarray(table, dtype=np.int64), 1)
+            if self._lengths[seq_id] % self.block_size and self._ref[table[-1]] > 1:
+                fail(f"sequence {seq_id}'s last block {table[-1]} is not full, and shared")
+        if self._shared != int((owners > 1).sum()):
+            fail(f"{self._shared} blocks are counted as shared, {int((owners > 1).sum())} are")
         for b in range(self.num_blocks):
             n = int(owners[b])
             if n != self._ref[b]:

@@ -20,7 +20,7 @@ import torch
 from . import _hip
 from .block_manager import BlockManager
 from .hip_tree import tree_maps
-from .paged_cache import PagedMetadata, PerSequence, TreeMetadata, check_trees
+from .paged_cache import PagedMetadata, PerSequence, TreeMetadata, check_trees, decode_groups
 
 
 class _LazyList(Sequence):
@@ -127,6 +127,8 @@ class DeviceBlockTables:
             i = int(np.argmax(ctx))
             raise ValueError(f"sequence {seqs[i]}: context {ctx[i]} exceeds the device tables' "
                              f"{self.max_blocks * B} tokens")
+        for seq, start, n in batch:
+            m.check_own(seq, start, n)
         return seqs, starts, counts, ctx
 
     def build_tree(self, batch: list[tuple[int, int, list[int]]]) -> TreeMetadata:
@@ -163,6 +165,7 @@ class DeviceBlockTables:
             return out
 
         return dict(
+            shared=decode_groups(m, tables, ctx.tolist(), counts.tolist()),
             slots_cpu=_LazyList(int(counts.sum()), slot_list),
             block_ids=PerSequence(S, lambda i: torch.from_numpy(tables[i][:nbs[i]].astype(np.int64)).to(self.device)),
             block_ids_cpu=PerSequence(S, lambda i: tables[i][:nbs[i]].tolist()))

@@ -132,6 +132,8 @@ class DecodeGraphRunner:
         if bad.size:
             i = int(bad[0])
             raise ValueError(f"sequence {seq_ids[i]}: context {lens[i]} outside 1 .. {self.max_context}")
+        for s, n in zip(seq_ids, lens.tolist()):
+            m.check_own(s, n - 1, 1)
         self._copied.synchronize()  # the previous step's copy has left the pinned buffer
         info = self._ninfo
         info[:b] = np.fromiter((self.tables.row(s) for s in seq_ids), dtype=np.int64, count=b)

@@ -1,0 +1,152 @@
+"""Beam search on MI355X through libsmallinf_hip.so: the best continuations over the beams and the vocabulary of every
+request, and the copies of blocks of beams that go on from the same one. The reference decodes greedily and has no
+counterpart.
+
+A step over the beams of a batch, which share their blocks (engine.block_manager.BlockManager.fork):
+
+  logits = model.forward(...)                      # rows: the beams, one request after the other
+  choice = beam_select(logits, scores, beams, n)   # n best (score, beam, token) of each request
+  copies = manager.reorder(ids, parents)           # each sequence goes on from the one that was chosen
+  cache.copy_blocks(copies)                        # their blocks that are not full yet
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Sequence
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import _hip
+
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+MAX_CANDIDATES = 64
+MAX_BEAMS = 1024
+
+
+class BeamChoice(NamedTuple):
+    """The best continuations of each request, in descending order; score -inf, beam and token -1 behind the last one."""
+    scores: torch.Tensor  # [groups, n] fp32
+    beams: torch.Tensor   # [groups, n] int64 row within the group
+    tokens: torch.Tensor  # [groups, n] int64
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int | torch.Tensor, candidates: int) -> BeamChoice:
+    """The `candidates` (1 .. 64) best continuations over the beams and the vocabulary of each request, in two launches
+    (sipa_beam_select): of row r and token v the score is scores[r] + log_softmax(logits[r])[v], equal ones in the order of
+    their rows, then tokens. The scores decide in 64 bits and are returned in 32.
+
+    logits [R, V] bf16, fp16 or fp32 with a contiguous last dim (R the beams of all requests); scores [R] fp32; beams: how
+    many rows each request has (1 to 1024, dividing R; 1 for the first step, when there is one row a request), or int32
+    starts [groups + 1] of requests of different numbers of rows (up to 1024 each). Tokens of logit -inf are never taken,
+    nor is any of a row whose score is not finite (a beam that has ended: -inf) or whose logits hold NaN or +inf, or -inf
+    alone. CPU tensors are computed by torch operations."""
+    if logits.dim() != 2 or logits.dtype not in DTYPES or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] in bf16, fp16 or fp32 with a contiguous last dim")
+    R, V = logits.shape
+    if scores.dtype is not torch.float32 or scores.shape != (R,) or not scores.is_contiguous():
+        raise ValueError(f"scores must be a contiguous fp32 vector of {R}")
+    if not 1 <= candidates <= MAX_CANDIDATES:
+        raise ValueError(f"{candidates} candidates (1 to {MAX_CANDIDATES})")
+    starts = beams if isinstance(beams, torch.Tensor) else None
+    if starts is not None:
+        if starts.dtype is not torch.int32 or starts.dim() != 1 or starts.shape[0] < 1 or not starts.is_contiguous():
+            raise ValueError("starts of requests must be a contiguous int32 vector")
+        groups, beams = starts.shape[0] - 1, 0
+    else:
+        if not 1 <= beams <= MAX_BEAMS or R % beams:
+            raise ValueError(f"{beams} beams a request (1 to {MAX_BEAMS}) in {R} rows")
+        groups = R // beams
+    devices = {t.device for t in (logits, scores, starts) if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"logits, scores and starts must be on one device, got {sorted(map(str, devices))}")
+    if not logits.is_cuda:
+        return _select_torch(logits, scores, starts, beams, groups, candidates)
+    dev = logits.device
+    out = BeamChoice(torch.empty(groups, candidates, dtype=torch.float32, device=dev),
+                     *(torch.empty(groups, candidates, dtype=torch.int64, device=dev) for _ in range(2)))
+    if groups == 0:
+        return out
+    p = _hip.BeamParams(struct_size=ctypes.sizeof(_hip.BeamParams), num_rows=R, vocab=V, num_groups=groups, beams=beams,
+                        num_candidates=candidates, dtype=_hip.dtype_code(logits.dtype), logits=logits.data_ptr(),
+                        logits_stride=logits.stride(0), scores=scores.data_ptr(), starts=_hip.ptr(starts),
+                        out_scores=out.scores.data_ptr(), out_beams=out.beams.data_ptr(), out_tokens=out.tokens.data_ptr())
+    lib, ref = _hip.lib(), ctypes.byref(p)
+    n = lib.sipa_beam_workspace_bytes(ref)
+    if n < 0:
+        _hip.check(n, "beam_select")
+    with _hip.on_device(dev):
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), n
+        rc = lib.sipa_beam_select(ref, _hip.stream_of(logits))
+    if rc:
+        _hip.check(rc, "beam_select")
+    return out
+
+
+def _select_torch(logits, scores, starts, beams: int, groups: int, candidates: int) -> BeamChoice:
+    """beam_select() on CPU tensors, group by group."""
+    R, V = logits.shape
+    bounds = [g * beams for g in range(groups + 1)] if starts is None else starts.clamp(0, R).tolist()
+    out = BeamChoice(torch.full((groups, candidates), float("-inf")),
+                     *(torch.full((groups, candidates), -1, dtype=torch.int64) for _ in range(2)))
+    n = min(candidates, V)
+    for g, (a, b) in enumerate(zip(bounds, bounds[1:])):
+        b = min(b, a + MAX_BEAMS)
+        if a >= b:
+            continue
+        l = logits[a:b].double()
+        value, token = torch.sort(l, dim=-1, descending=True, stable=True)
+        value, token = value[:, :n], token[:, :n]
+        off = scores[a:b].double() - torch.logsumexp(l, -1)
+        score = off[:, None] + value
+        score = torch.where(off.isfinite()[:, None] & (value > float("-inf")), score, float("-inf")).reshape(-1)
+        best, at = torch.sort(score, descending=True, stable=True)
+        k = min(candidates, int((best > float("-inf")).sum()))
+        out.scores[g, :k] = best[:k].float()
+        out.beams[g, :k], out.tokens[g, :k] = at[:k] // n, token.reshape(-1)[at[:k]]
+    return out
+
+
+def copy_blocks(pools: Sequence[torch.Tensor], copies: Sequence[tuple[int, int, int]]) -> None:
+    """For each (src, dst, tokens) of copies, the first `tokens` tokens of block src become those of block dst, in every layer
+    and head of the pools, in place (sipa_copy_blocks; one launch for 256 copies). No block may be the destination of two
+    copies, or of one and the source of another.
+
+    pools: one to four tensors [L, Hkv, N, B, ...], a cache's K, V and their per-token scales, each head's blocks contiguous.
+    The copies are the host's: a graph captures the ones it was given. CPU pools are copied by torch operations."""
+    if not 1 <= len(pools) <= 4:
+        raise ValueError(f"{len(pools)} pools (1 to 4)")
+    L, H, N, B = pools[0].shape[:4]
+    for t in pools:
+        if t.dim() < 4 or t.shape[:4] != (L, H, N, B) or t.device != pools[0].device:
+            raise ValueError(f"the pools must be {(L, H, N, B, '...')} on one device")
+        if t.numel() and not t[0, 0].is_contiguous():
+            raise ValueError("each head's blocks must be contiguous")
+    n = len(copies)
+    if not n:
+        return
+    flat = np.fromiter((x for c in copies for x in c), dtype=np.int64)
+    if flat.size != 3 * n or any(len(c) != 3 for c in copies):
+        raise ValueError("copies must be (src, dst, tokens)")
+    if flat.min() < 0 or flat.max() >= 1 << 31:
+        raise ValueError(f"copies past the {N} blocks of {B} tokens")
+    flat = flat.astype(np.int32)
+    if not pools[0].is_cuda:
+        _hip.check(_hip.lib().sipa_check_copies(flat.ctypes.data, n, N, B), "copy_blocks")
+        for t in pools:
+            for s, d, rows in copies:
+                t[:, :, d, :rows] = t[:, :, s, :rows]
+        return
+    p = _hip.CopyParams(struct_size=ctypes.sizeof(_hip.CopyParams), num_layers=L, num_kv_heads=H, num_blocks=N, block_size=B,
+                        num_pools=len(pools), copies=flat.ctypes.data, num_copies=n)
+    for i, t in enumerate(pools):
+        size = t.element_size()
+        p.pools[i], p.stride_l[i], p.stride_h[i] = t.data_ptr(), t.stride(0) * size, t.stride(1) * size
+        p.row_bytes[i] = t[0, 0, 0, 0].numel() * size if t.numel() else size
+    with _hip.on_device(pools[0].device):
+        rc = _hip.lib().sipa_copy_blocks(ctypes.byref(p), _hip.stream_of(pools[0]))
+    if rc:
+        _hip.check(rc, "copy_blocks")

@@ -18,7 +18,7 @@ On a GPU pool, write() scatters K and V with one HIP store launch; a CPU pool us
 from __future__ import annotations
 
 from collections.abc import Callable, Sequence
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -27,8 +27,10 @@ from ._hip import layer_ptr
 from .attention import attention
 from .block_manager import BlockManager
 from .config import ModelConfig
+from .hip_beam import copy_blocks
 from .hip_decode import DecodePlan
 from .hip_prefill import paged_prefill_attention, prefill_splits, prefill_supported
+from .hip_prefix import PrefixPlan, prefix_supported, shared_groups
 from .hip_quant import store_layer
 from .hip_tree import MAX_NODES, TreePlan, commit_tokens, mask_words, tree_supported
 
@@ -82,11 +84,23 @@ class PagedMetadata:
     block_tables: torch.Tensor  # [num_seqs, max_blocks] int32, padded with -1 (the kernel-facing form)
     context_lens_t: torch.Tensor  # [num_seqs] int32 on the device
     last_token_indices: torch.Tensor  # [num_seqs] row of each sequence's last new token
+    # which sequences of one new token share their first blocks: [(sequences, tokens)] (engine.hip_prefix.shared_groups)
+    shared: list[tuple[list[int], int]] = field(default_factory=list, kw_only=True)
 
     @property
     def num_seqs(self) -> int:
         """Sequences in this forward."""
         return len(self.context_lens)
+
+
+def decode_groups(manager: BlockManager, tables: list[np.ndarray], context_lens: list[int],
+                  new_tokens: list[int]) -> list[tuple[list[int], int]]:
+    """The groups of a forward's sequences of one new token whose tables share blocks ([] for managers that share none)."""
+    if not getattr(manager, "num_shared_blocks", int)():
+        return []
+    dec = [i for i, n in enumerate(new_tokens) if n == 1]
+    found = shared_groups([tables[i] for i in dec], [context_lens[i] for i in dec], manager.block_size)
+    return [([dec[r] for r in rows], tokens) for rows, tokens in found]
 
 
 def build_metadata(manager: BlockManager, batch: list[tuple[int, int, int]],
@@ -107,6 +121,7 @@ def build_metadata(manager: BlockManager, batch: list[tuple[int, int, int]],
     if table_of is None:
         def table_of(seq_id: int) -> np.ndarray:
             return np.asarray(manager.block_table(seq_id), dtype=np.int32)
+    check_own = getattr(manager, "check_own", None)
     starts, lens, tables = [0], [], []
     positions: list[int] = []
     slot_list: list[int] = []
@@ -119,6 +134,8 @@ def build_metadata(manager: BlockManager, batch: list[tuple[int, int, int]],
             raise ValueError(f"sequence {seq_id} holds {held} tokens, forward needs {ctx}")
         if start < 0:
             raise ValueError(f"sequence {seq_id}: negative start {start}")
+        if check_own is not None:
+            check_own(seq_id, start, n)
         table = table_of(seq_id)[:(ctx + B - 1) // B]
         if n == 1:  # a decode row: one slot, no array work
             positions.append(start)
@@ -158,6 +175,7 @@ def build_metadata(manager: BlockManager, batch: list[tuple[int, int, int]],
         block_tables=d32[:S * width].view(S, width),
         context_lens_t=d32[S * width:],
         last_token_indices=d64[4 * T:],
+        shared=decode_groups(manager, tables, lens, [n for _, _, n in batch]),
     )
 
 
@@ -312,6 +330,8 @@ class PagedKVCache:
                 rows, bt, ctx = meta.last_token_indices[idx], meta.block_tables[idx], meta.context_lens_t[idx]
             self._decode = (rows, bt, ctx, [meta.context_lens[i] for i in dec])
             self._decode_seqs = dec
+            place = {seq: i for i, seq in enumerate(dec)}
+            self._shared = [([place[i] for i in seqs], tokens) for seqs, tokens in meta.shared]
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Scatter this forward's k, v [T, H_kv, d] into their slots."""
@@ -377,6 +397,13 @@ class PagedKVCache:
         return prefill_supported(self.dtype, self.k.dtype, self.block_size, cfg.head_dim,
                                  cfg.num_q_heads // cfg.num_kv_heads, max_context)
 
+    def _prefix_kernel_ok(self, q: torch.Tensor, max_context: int) -> bool:
+        """Whether the forward's decode rows go to the shared-prefix kernel, which reads a group's keys once."""
+        S, Hq, d = q.shape
+        if not prefix_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads, max_context):
+            return False
+        return sum((len(rows) - 1) * tokens for rows, tokens in self._shared) > 0
+
     def _attend_prefill(self, layer: int, q: torch.Tensor, scale: float, out: torch.Tensor) -> None:
         """Multi-token rows of the forward, written into their rows of out [T, Hq, d] by the prefill kernel."""
         bt, ctx, qs, ql, max_ctx, max_q, splits = self._prefill_launch
@@ -413,11 +440,16 @@ class PagedKVCache:
         dec_out = out[rows].view(-1, Hq, d) if in_place else None
         if self._plan is None or self._plan_scale != scale:  # first layer of the forward: validate once
             # The host-side lengths let a ragged batch run from a work list (built once, used by every layer).
-            self._plan = DecodePlan(q_dec, self.k[layer], self.v[layer], bt, ctx, scale, max(lens),
-                                    quant=self._kernel_quant(layer), host_context_lens=lens)
+            if self._shared and self._prefix_kernel_ok(q_dec, max(lens)):
+                self._plan = PrefixPlan(q_dec, self.k[layer], self.v[layer], bt, ctx, self._shared, scale, max(lens),
+                                        quant=self._kernel_quant(layer), host_context_lens=lens)
+                dec = self._plan(q_dec, self.k[layer], self.v[layer], out=dec_out)
+            else:
+                self._plan = DecodePlan(q_dec, self.k[layer], self.v[layer], bt, ctx, scale, max(lens),
+                                        quant=self._kernel_quant(layer), host_context_lens=lens)
+                dec = self._plan(out=dec_out)
             self._plan_scale = scale
             self._quant_pools = self._all_quant()
-            dec = self._plan(out=dec_out)
         else:
             dec = self._plan.run_layer(layer, q_dec, self.k, self.v, self._quant_pools, dec_out)
         if rows is None:
@@ -443,6 +475,11 @@ class PagedKVCache:
                 max(m.context_lens), m.max_nodes, quant=self._kernel_quant(layer)), scale
             return self._tree_plan(q, self.k[layer], self.v[layer]).view(T, Hq * d)
         return plan.run_layer(layer, q, self.k, self.v, self._all_quant()).view(T, Hq * d)
+
+    def copy_blocks(self, copies: list[tuple[int, int, int]]) -> None:
+        """Make the copies that BlockManager.fork or reorder returned: the first tokens of blocks, in every layer. No
+        counterpart in the reference, whose sequences share nothing."""
+        copy_blocks([t for t in self._commit_pools() if t is not None], copies)
 
     def _commit_pools(self) -> tuple:
         """(K, V, K scales, V scales): what a token's row of every layer consists of; scales None without any."""

@@ -26,6 +26,7 @@ import torch
 
 from .block_manager import BlockManager
 from .config import ModelConfig
+from .hip_beam import copy_blocks
 from .hip_decode import QuantKV
 from .hip_quant import (kchan_write_rows, quantize_store_block_rows, quantize_store_blocks, quantize_store_layer,
                         quantize_store_tokens, store_tokens)
@@ -348,6 +349,20 @@ class QuantPagedKVCache(PagedKVCache):
         if self.fmt == "int8":
             return QuantKV(1, self.k_scale[layer], self.v_scale[layer])
         return QuantKV(2, self.k_scale[layer], self.v_scale[layer], self.stage[layer], self._tails_dec)
+
+    def _prefix_kernel_ok(self, q: torch.Tensor, max_context: int) -> bool:
+        return self.fmt == "int8" and super()._prefix_kernel_ok(q, max_context)
+
+    def copy_blocks(self, copies: list[tuple[int, int, int]]) -> None:
+        """As the base's; format B's last blocks hold K in their staging slots, which the copies get of their own."""
+        if self.fmt == "int8":
+            super().copy_blocks(copies)
+            return
+        copy_blocks((self.v, self.v_scale), copies)
+        # (a block without a slot: none of its tokens has been written yet)
+        staged = [(src, dst, n) for src, dst, n in copies if src in self._stage_of]
+        self._book.assign([dst for _, dst, _ in staged if dst not in self._stage_of])
+        copy_blocks((self.stage,), [(self._stage_of[src], self._stage_of[dst], n) for src, dst, n in staged])
 
     def _commit_pools(self) -> tuple:
         if self.fmt != "int8":
