@@ -6,8 +6,9 @@
 //   beam_rows   a workgroup holds a piece of a row in registers, takes its maximum, the sum of exponentials below it, and
 //               its N largest logits: those above a threshold that at least N pass (the least of the maxima of at least N
 //               parts of the workgroup's lanes) are collected in LDS and put into order by counting.
-//   beam_merge  a workgroup a group joins the pieces' sums in 64 bits and puts the candidates in order in the same way.
-// It reads every logit once; no sum depends on the order in which workgroups or atomics run.
+//   beam_merge  a workgroup a group, a wave a row: joins the pieces' sums in 64 bits and puts a row's candidates, then the
+//               group's, in order in the same way.
+// It reads every logit once; no sum depends on the order in which workgroups or waves run, so equal rows get equal sums.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -16,24 +17,26 @@
 
 namespace sipa {
 
-constexpr int kBeamThreads = 256, kBeamMaxN = 64, kBeamMaxRows = 1024, kBeamCap = 1024, kBeamMergeCap = 512;
+constexpr int kBeamThreads = 256, kBeamMaxN = 64, kBeamMaxRows = 1024;
+constexpr int kBeamCap = 256;  // collected logits of a wave
 
 struct BeamArgs {
   const void* logits;
   int64_t l_st;
   const float* cum;
   const int32_t* starts;
-  int32_t R, V, beams, N, ns;  // ns pieces of a row
-  float* p_max;                // [R][ns]
-  double* p_sum;               // [R][ns] sum of exp(l - p_max)
-  float* c_val;                // [R][ns][N] a piece's largest logits in order, -inf behind them
-  int32_t* c_tok;
+  int32_t R, V, beams, N;
+  int32_t ns, piece;  // pieces of a row, logits of a piece
+  int32_t log_parts;  // 1 << log_parts >= N classes of lanes
+  float* p_max;       // [R][ns]
+  double* p_sum;      // [R][ns] sum of exp(l - p_max)
+  uint64_t* p_key;    // [R][N][ns] the pieces' largest logits in order (beam_key), 0 behind them
   float* out_scores;
   int64_t* out_beams;
   int64_t* out_tokens;
 };
 
-// fp32 as an integer of the same order; of equal values the lower index is the larger key.
+// fp32 as an integer of the same order; of equal values the lower index is the larger key. No value but NaN gives 0.
 __device__ __forceinline__ uint64_t beam_key(float x, uint32_t index) {
   const uint32_t b = __float_as_uint(x + 0.f);  // -0 as 0
   return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~index;
@@ -44,22 +47,70 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t x, int o) {
-  return (uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), o) << 32 | (uint32_t)__shfl_xor((int)x, o);
+// fp64 as an integer of the same order, 0 for none.
+__device__ __forceinline__ uint64_t score_key(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.);
+  return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double x, int o) {
-  return __builtin_bit_cast(double, shfl_xor_u64(__builtin_bit_cast(uint64_t, x), o));
+__device__ __forceinline__ double score_value(uint64_t b) {
+  return __builtin_bit_cast(double, b >> 63 ? b & ~(1ull << 63) : ~b);
 }
 
-// exp(d) for d <= 0 to about an ulp: the product with log2 e is carried in two terms, since an ulp of d log2 e = 20 alone is
-// 1e-6 of the result.
-__device__ __forceinline__ float beam_exp(float d) {
-  constexpr float kL = 1.44269502162933349609f, kLo = 1.92596299112661746887e-8f, kLn2 = 0.69314718055994530942f;
-  const float y = d * kL;
-  const float rest = fmaf(d, kLo, fmaf(d, kL, -y));
-  const float e = fast_exp2(y);
-  return y < -126.f ? 0.f : fmaf(e * kLn2, rest, e);
+// Step K = 0 .. 5 of a butterfly over a wave: the value of a lane that the steps before have not brought together with this one.
+// Cross-lane moves of the vector unit, without LDS. After K steps the lanes that hold one value are spread evenly over the wave:
+// every 32nd, 16th, 8th, then pairs of those.
+template <int K>
+__device__ __forceinline__ uint32_t other_lane(uint32_t x) {
+  if constexpr (K == 0) {
+    const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? p[0] : p[1];
+  } else if constexpr (K == 1) {
+    const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? p[0] : p[1];
+  }
+  else if constexpr (K == 2) return __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, true);  // 8 further of 16
+  else if constexpr (K == 3) return __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, true);  // 7 - i of 8
+  else if constexpr (K == 4) return __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xf, 0xf, true);   // 2 3 0 1 of 4
+  else return __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xf, 0xf, true);                         // 1 0 3 2
+}
+
+template <int K>
+__device__ __forceinline__ float other_lane(float x) {
+  return __uint_as_float(other_lane<K>(__float_as_uint(x)));
+}
+
+template <int K>
+__device__ __forceinline__ uint64_t other_lane(uint64_t x) {
+  return (uint64_t)other_lane<K>((uint32_t)(x >> 32)) << 32 | other_lane<K>((uint32_t)x);
+}
+
+template <int K>
+__device__ __forceinline__ double other_lane(double x) {
+  return __builtin_bit_cast(double, other_lane<K>(__builtin_bit_cast(uint64_t, x)));
+}
+
+template <int K = 0, typename T, typename F>
+__device__ __forceinline__ T butterfly(T x, F f) {  // f(K, own, other); every lane gets the result
+  if constexpr (K == 6) return x;
+  else return butterfly<K + 1>(f(K, x, other_lane<K>(x)), f);
+}
+
+__device__ __forceinline__ double wave_sum_f64(double x) {  // a + b and b + a are the same bits
+  return butterfly(x, [](int, double a, double b) { return a + b; });
+}
+
+// How many of the keys of a list in LDS (in fours, with 0 behind the last) are over `key`.
+__device__ __forceinline__ int keys_over(const uint64_t* list, int n, uint64_t key) {
+  int over = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 4) {
+    const ulonglong2 a = *(const ulonglong2*)(list + j), b = *(const ulonglong2*)(list + j + 2);
+    const uint64_t k[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) over += k[x] > key;
+  }
+  return over;
 }
 
 template <int DT>
@@ -80,49 +131,52 @@ struct BeamType<SIPA_F16> {
   static constexpr int E = 8;
 };
 
+template <int DT>
+__device__ __forceinline__ float logit(uint32_t bits) {
+  return DT == SIPA_F32 ? __uint_as_float(bits) : DT == SIPA_BF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits);
+}
+
 // PARTS 16-byte parts of a row a thread (aligned to an element only: rows of an odd vocabulary start anywhere).
 template <int DT, int PARTS>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs a) {
   typedef typename BeamType<DT>::T T;
-  constexpr int THR = kBeamThreads, E = BeamType<DT>::E, BITS = 8 * sizeof(T), PIECE = THR * E * PARTS;
+  constexpr int THR = kBeamThreads, E = BeamType<DT>::E, BITS = 8 * sizeof(T);
   struct __attribute__((packed, aligned(sizeof(T)))) Part {
     uint32_t w[4];
   };
-  __shared__ uint64_t found[kBeamCap];
-  __shared__ float w_max[4], w_low[4];
+  __shared__ __align__(16) uint64_t found[4][kBeamCap + 4];
+  __shared__ float w_max[4][64];
   __shared__ double w_sum[4];
+  __shared__ int w_count[4];
   __shared__ uint64_t w_key[4];
-  __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r = blockIdx.x / a.ns, piece = blockIdx.x - r * a.ns, v0 = piece * PIECE;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = blockIdx.x / a.ns, piece = blockIdx.x - r * a.ns, v0 = piece * a.piece;
   const T* row = (const T*)a.logits + (int64_t)r * a.l_st + v0;
-  const int n = min(PIECE, a.V - v0);
+  const int n = min(a.piece, a.V - v0);
   Part x[PARTS];
-  const uint32_t kNone = DT == SIPA_F32 ? 0xff800000u : DT == SIPA_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  constexpr uint32_t kNone = DT == SIPA_F32 ? 0xff800000u : DT == SIPA_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
     const int at = E * (tid + THR * i);
-    if (at + E <= n) {
-      x[i] = *(const Part*)(row + at);
-    } else {
+    if (at + E <= n) x[i] = *(const Part*)(row + at);
+    else x[i] = Part{{kNone, kNone, kNone, kNone}};
+  }
+  if (const int last = n / E; n % E != 0 && last % THR == tid) {  // the row's last few logits
+    Part y = {{kNone, kNone, kNone, kNone}};
+    for (int e = 0; e < n % E; ++e) {
+      const uint32_t bits = row[last * E + e], shift = BITS * e & 31, mask = BITS == 32 ? ~0u : 0xffffu << shift;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) x[i].w[w] = kNone;
-      for (int e = 0; e < E && at + e < n; ++e) {
-        const uint32_t bits = row[at + e];
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (BITS * e >> 5 == w) {
-            if constexpr (BITS == 32) x[i].w[w] = bits;
-            else x[i].w[w] = e & 1 ? (x[i].w[w] & 0xffffu) | bits << 16 : (x[i].w[w] & 0xffff0000u) | bits;
-          }
-      }
+      for (int w = 0; w < 4; ++w)
+        if (BITS * e >> 5 == w) y.w[w] = (y.w[w] & ~mask) | bits << shift;
     }
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+      if (last / THR == i) x[i] = y;
   }
   auto value = [&](int i, int e) {
-    if constexpr (DT == SIPA_F32) return __uint_as_float(x[i].w[e]);
-    const uint32_t w = x[i].w[e >> 1];
+    const uint32_t w = x[i].w[BITS * e >> 5];
     if constexpr (DT == SIPA_BF16) return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
-    return f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
+    return logit<DT>(BITS == 32 ? w : e & 1 ? w >> 16 : w & 0xffffu);
   };
   auto index = [&](int i, int e) { return (uint32_t)(v0 + E * (tid + THR * i) + e); };
   float mine = kNegInf;
@@ -130,86 +184,84 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
   for (int i = 0; i < PARTS; ++i)
 #pragma unroll
     for (int e = 0; e < E; ++e) mine = fmaxf(mine, value(i, e));
-  // The maxima of parts of `part` lanes each, as many parts as candidates at least, and the least of them.
-  int parts = 4;
-  while (parts < a.N) parts *= 2;
-  const int part = THR / parts;
-  float top = mine, low = mine;
+  // Kept as they came: the compiler would otherwise hold every logit in fp32, or its key (244 registers for 64 logits).
+  auto keep = [&]() {
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    top = fmaxf(top, __shfl_xor(top, o));
-    const float other = __shfl_xor(low, o);
-    low = o < part ? fmaxf(low, other) : fminf(low, other);
-  }
-  if (lane == 0) w_max[wave] = top, w_low[wave] = low;
-  if (tid == 0) count = 0;
+    for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(x[i].w[w]));
+  };
+  keep();
+  // The maxima of classes of lanes, as many classes as candidates at least, and the least of them. (A class's lanes are spread
+  // over the workgroup: a short piece has some of each.)
+  const int within = 6 - a.log_parts;  // steps within a class
+  float best = mine;
+  best = butterfly(best, [&](int k, float p, float q) { return k < within ? fmaxf(p, q) : p; });
+  w_max[wave][lane] = best;
   __syncthreads();
-  top = fmaxf(fmaxf(w_max[0], w_max[1]), fmaxf(w_max[2], w_max[3]));
-  low = fminf(fminf(w_low[0], w_low[1]), fminf(w_low[2], w_low[3]));
+  best = fmaxf(fmaxf(w_max[0][lane], w_max[1][lane]), fmaxf(w_max[2][lane], w_max[3][lane]));
+  const float top = butterfly(best, [](int, float p, float q) { return fmaxf(p, q); });
+  float low = butterfly(best, [](int, float p, float q) { return fminf(p, q); });
+  // exp(l - top) as exp2((l - top) log2 e): its argument is rounded, 2^-20 of the term at most where the term matters.
   const float off = top == kNegInf ? 0.f : top;
+  low = fmaxf(low, -__FLT_MAX__);  // never -inf
   double sum = 0.;
+  int count = 0;
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += beam_exp(value(i, e) - off);
+    for (int e = 0; e < E; ++e) {
+      const float v = value(i, e);
+      s += fast_exp2((v - off) * 1.44269504088896340736f);
+      const uint64_t hits = __builtin_amdgcn_ballot_w64(v >= low);
+      if (hits) {
+        const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0u));
+        if (v >= low && to < kBeamCap) found[wave][to] = beam_key(v, index(i, e));
+        count += __builtin_popcountll(hits);
+      }
+    }
     sum += (double)s;
   }
-  if (mine >= low && mine > kNegInf) {
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float v = value(i, e);
-        if (v >= low && v > kNegInf) {
-          const int to = atomicAdd(&count, 1);
-          if (to < kBeamCap) found[to] = beam_key(v, index(i, e));
-        }
-      }
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_f64(sum, o);
-  if (lane == 0) w_sum[wave] = sum;
+  sum = wave_sum_f64(sum);
+  if (lane < 4 && count <= kBeamCap) found[wave][count + lane] = 0;
+  if (lane == 0) w_sum[wave] = sum, w_count[wave] = count;
   __syncthreads();
   const int64_t at = (int64_t)r * a.ns + piece;
   if (tid == 0) {
     a.p_max[at] = top;
     a.p_sum[at] = (w_sum[0] + w_sum[1]) + (w_sum[2] + w_sum[3]);
   }
-  int got = count;
-  float* c_val = a.c_val + at * a.N;
-  int32_t* c_tok = a.c_tok + at * a.N;
-  if (got <= kBeamCap) {
-    for (int i = tid; i < got; i += THR) {
-      const uint64_t key = found[i];
+  uint64_t* out = a.p_key + (int64_t)r * a.ns * a.N + piece;  // rank i at i ns
+  const int all[4] = {w_count[0], w_count[1], w_count[2], w_count[3]};
+  int got = 0;
+  if (max(max(all[0], all[1]), max(all[2], all[3])) <= kBeamCap) {
+    got = all[0] + all[1] + all[2] + all[3];
+    for (int i = lane; i < count; i += 64) {
+      const uint64_t key = found[wave][i];  // no two are equal
       int rank = 0;
-      for (int j = 0; j < got; ++j) rank += found[j] > key;
-      if (rank < a.N) c_val[rank] = key_value(key), c_tok[rank] = (int32_t)~(uint32_t)key;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) rank += keys_over(found[w], all[w], key);
+      if (rank < a.N) out[(int64_t)rank * a.ns] = key;
     }
   } else {
     // Most of the piece ties or rises: the largest key under the last one, N times. Only the thread that had it looks for
     // its next.
     auto best_below = [&](uint64_t limit) {
       uint64_t best = 0;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < PARTS; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float v = value(i, e);
+#pragma unroll 1
+        for (int e = 0; e < E && E * (tid + THR * i) + e < n; ++e) {
+          const float v = logit<DT>(row[E * (tid + THR * i) + e]);
           const uint64_t key = v > kNegInf ? beam_key(v, index(i, e)) : 0;
           best = key < limit && key > best ? key : best;
         }
       return best;
     };
     uint64_t own = best_below(~0ull);
-    got = 0;
-    for (int k = 0; k < a.N; ++k) {
-      uint64_t best = own;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) {
-        const uint64_t other = shfl_xor_u64(best, o);
-        best = other > best ? other : best;
-      }
+    for (; got < a.N; ++got) {
+      uint64_t best = butterfly(own, [](int, uint64_t p, uint64_t q) { return p > q ? p : q; });
       if (lane == 0) w_key[wave] = best;
       __syncthreads();
 #pragma unroll
@@ -217,154 +269,143 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
       __syncthreads();
       if (best == 0) break;  // uniform
       if (own == best) {
-        c_val[k] = key_value(best), c_tok[k] = (int32_t)~(uint32_t)best;
+        out[(int64_t)got * a.ns] = best;
         own = best_below(best);
       }
-      ++got;
     }
   }
-  for (int i = got + tid; i < a.N; i += THR) c_val[i] = kNegInf, c_tok[i] = -1;
+  for (int i = got + tid; i < a.N; i += THR) out[(int64_t)i * a.ns] = 0;
 }
 
-// A candidate of a group: its score's bits in order, its row within the group, its logit and token (beam_key). Equal scores go
-// by row, then as the row orders its tokens: logits so small that they leave no trace in the score still do that.
-struct BeamCandidate {
-  uint64_t score, key;
-  uint32_t row;
-  __device__ __forceinline__ bool over(const BeamCandidate& o) const {
-    return score != o.score ? score > o.score : row != o.row ? row < o.row : key > o.key;
+// The N largest of a wave's keys (no two equal, 0: none), SLOTS a lane, in order, to best[0 ..] in LDS. list: room for
+// 64 SLOTS + 4 keys.
+template <int SLOTS>
+__device__ __forceinline__ void wave_select(const uint64_t (&key)[SLOTS], int N, int log_parts, uint64_t* list, uint64_t* best) {
+  const int lane = threadIdx.x & 63;
+  uint64_t low = 0;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) low = key[i] > low ? key[i] : low;
+  low = butterfly(low, [&](int k, uint64_t p, uint64_t q) { return (k < 6 - log_parts) == (p > q) ? p : q; });
+  low = low == 0 ? 1 : low;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const uint64_t hits = __builtin_amdgcn_ballot_w64(key[i] >= low);
+    if (hits) {
+      const int to = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0u));
+      if (key[i] >= low) list[to] = key[i];
+      n += __builtin_popcountll(hits);
+    }
   }
-};
-
-__device__ __forceinline__ uint64_t f64_order(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.);
-  return b >> 63 ? ~b : b | 1ull << 63;
+  if (lane < 4) list[n + lane] = 0;
+  wave_sync();
+  for (int i = lane; i < n; i += 64) {
+    const int rank = keys_over(list, n, list[i]);
+    if (rank < N) best[rank] = list[i];
+  }
 }
 
-__device__ __forceinline__ double order_f64(uint64_t b) {
-  return __builtin_bit_cast(double, b >> 63 ? b & ~(1ull << 63) : ~b);
-}
+constexpr int kMergeWaves = 8, kMergeSlots = 8;
 
-__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamArgs a) {
-  constexpr int THR = kBeamThreads;
-  __shared__ double offset[kBeamMaxRows];  // cum - log sum exp, NaN for a row without candidates
-  __shared__ BeamCandidate found[kBeamMergeCap];
-  __shared__ uint64_t w_low[4];
-  __shared__ BeamCandidate w_best[4];
-  __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x;
+// Eight rows at a time: each wave finds its row's candidates among those of the row's pieces, then where they stand among the
+// other rows' and the group's so far (lists in order, searched by halving; of equal scores the earlier row's go first).
+__global__ void __launch_bounds__(64 * kMergeWaves) beam_merge_kernel(const BeamArgs a) {
+  constexpr int W = kMergeWaves, SLOTS = kMergeSlots + 1;
+  __shared__ __align__(16) uint64_t list[W][64 * SLOTS + 4];
+  __shared__ uint64_t row_best[W][kBeamMaxN];             // a row's candidates in order (beam_key)
+  __shared__ uint64_t score[2][W + 1][kBeamMaxN];         // in turn: the group's so far, then the rows' (score_key)
+  __shared__ uint64_t from[2][kBeamMaxN];                 // the group's so far: row << 32 | token
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = blockIdx.x, N = a.N;
   const int r0 = a.starts == nullptr ? g * a.beams : min(max(a.starts[g], 0), a.R);
   const int r1 = a.starts == nullptr ? r0 + a.beams : min(max(a.starts[g + 1], r0), a.R);
   const int rows = min(r1 - r0, kBeamMaxRows);
-  for (int b = wave; b < rows; b += 4) {  // a wave a row
-    const int64_t first = (int64_t)(r0 + b) * a.ns;
-    float top = kNegInf;
-    for (int i = lane; i < a.ns; i += 64) top = fmaxf(top, a.p_max[first + i]);
-    top = wave_max(top);
-    double sum = 0.;
-    for (int i = lane; i < a.ns; i += 64) {
-      const float m = a.p_max[first + i];
-      const double s = a.p_sum[first + i];
-      sum += m == kNegInf ? s : s * exp((double)m - (double)top);
-    }
+  if (wave == 0) score[0][0][lane] = 0;
+  int turn = 0;
+  for (int b0 = 0; b0 < rows; b0 += W, turn ^= 1) {
+    const int b = b0 + wave;
+    uint64_t mine = 0;  // lane i: the row's candidate i
+    double off = __builtin_nan("");
+    if (b < rows) {
+      const int64_t first = (int64_t)(r0 + b) * a.ns;
+      const uint64_t* keys = a.p_key + first * N;
+      const int total = a.ns * N;
+      uint64_t key[SLOTS];
+      auto load = [&](int i0) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_f64(sum, o);
-    const double lse = (double)top + log(sum), cum = (double)a.cum[r0 + b];
-    const double off = cum - lse;
-    if (lane == 0) offset[b] = fabs(off) < __builtin_huge_val() ? off : __builtin_nan("");
-  }
-  if (tid == 0) count = 0;
-  __syncthreads();
-  const int per = a.ns * a.N, total = rows * per;  // (host-checked)
-  const int64_t first = (int64_t)r0 * per;
-  auto candidate = [&](int i) {
-    const int b = i / per;
-    const float v = a.c_val[first + i];
-    const double s = offset[b] + (double)v;
-    BeamCandidate c;
-    c.score = s > -__builtin_huge_val() ? f64_order(s) : 0;  // 0: none (-inf, NaN)
-    c.key = beam_key(v, (uint32_t)a.c_tok[first + i]);
-    c.row = (uint32_t)b;
-    return c;
-  };
-  // The threshold, as in beam_rows.
-  uint64_t mine = 0;
-  for (int i = tid; i < total; i += THR) {
-    const uint64_t s = candidate(i).score;
-    mine = s > mine ? s : mine;
-  }
-  int parts = 4;
-  while (parts < a.N) parts *= 2;
-  const int part = THR / parts;
-  uint64_t low = mine;
+        for (int i = 0; i < kMergeSlots; ++i) key[i + 1] = keys[min(i0 + 64 * i + lane, total - 1)];
+      };
+      load(0);
+      // the row's sum
+      float top = kNegInf;
+      for (int i = lane; i < a.ns; i += 64) top = fmaxf(top, a.p_max[first + i]);
+      top = butterfly(top, [](int, float p, float q) { return fmaxf(p, q); });
+      double sum = 0.;
+      for (int i = lane; i < a.ns; i += 64) {
+        const float m = a.p_max[first + i];
+        const double s = a.p_sum[first + i];
+        sum += m == kNegInf ? s : s * exp((double)m - (double)top);
+      }
+      sum = wave_sum_f64(sum);
+      off = (double)a.cum[r0 + b] - ((double)top + log(sum));
+      for (int i0 = 0; i0 < total; i0 += 64 * kMergeSlots) {
+        if (i0 > 0) load(i0);
+        key[0] = mine;
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const uint64_t other = shfl_xor_u64(low, o);
-    low = (o < part) == (other > low) ? other : low;
-  }
-  if (lane == 0) w_low[wave] = low;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) low = w_low[w] < low ? w_low[w] : low;
-  if (mine >= low && mine > 0)
-    for (int i = tid; i < total; i += THR) {
-      const BeamCandidate c = candidate(i);
-      if (c.score >= low && c.score > 0) {
-        const int to = atomicAdd(&count, 1);
-        if (to < kBeamMergeCap) found[to] = c;
+        for (int i = 0; i < kMergeSlots; ++i)
+          if (i0 + 64 * i + lane >= total) key[i + 1] = 0;
+        row_best[wave][lane] = 0;
+        wave_sync();
+        wave_select<SLOTS>(key, N, a.log_parts, list[wave], row_best[wave]);
+        wave_sync();
+        mine = row_best[wave][lane];
       }
     }
-  __syncthreads();
-  int got = count;
-  const int64_t out = (int64_t)g * a.N;
-  auto store = [&](int k, const BeamCandidate& c) {
-    a.out_scores[out + k] = (float)order_f64(c.score);
-    a.out_beams[out + k] = (int64_t)c.row;
-    a.out_tokens[out + k] = (int64_t)(uint32_t)~(uint32_t)c.key;
-  };
-  if (got <= kBeamMergeCap) {
-    for (int i = tid; i < got; i += THR) {
-      const BeamCandidate c = found[i];
-      int rank = 0;
-      for (int j = 0; j < got; ++j) rank += found[j].over(c);
-      if (rank < a.N) store(rank, c);
-    }
-  } else {
-    const BeamCandidate kNone = {0, 0, ~0u};
-    auto best_below = [&](const BeamCandidate& limit, bool all) {
-      BeamCandidate best = kNone;
-      for (int i = tid; i < total; i += THR) {
-        const BeamCandidate c = candidate(i);
-        if (c.score > 0 && (all || limit.over(c)) && c.over(best)) best = c;
+    const bool live = fabs(off) < __builtin_huge_val();  // else no candidate is the row's
+    const uint64_t own = mine != 0 && live ? score_key(off + (double)key_value(mine)) : 0;
+    score[turn][wave + 1][lane] = own;
+    if (wave == 0) score[turn ^ 1][0][lane] = 0;
+    __syncthreads();
+    auto place = [&](int of, uint64_t k) {  // candidates before the lane's: of earlier lists those not under it, of later ones those over it
+      int at[W + 1];
+#pragma unroll
+      for (int w = 0; w <= W; ++w) at[w] = 0;
+#pragma unroll
+      for (int step = 32; step > 0; step >>= 1)
+#pragma unroll
+        for (int w = 0; w <= W; ++w) {
+          const uint64_t x = score[turn][w][at[w] + step - 1];
+          at[w] += x > k || (x == k && w < of) ? step : 0;
+        }
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w <= W; ++w) {  // (63 of the 64 places so far)
+        const uint64_t x = score[turn][w][at[w]];
+        sum += w == of ? 0 : at[w] + (x > k || (x == k && w < of));
       }
-      return best;
+      return sum;
     };
-    BeamCandidate own = best_below(kNone, true);
-    got = 0;
-    for (int k = 0; k < a.N; ++k) {
-      BeamCandidate best = own;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) {
-        const BeamCandidate other = {shfl_xor_u64(best.score, o), shfl_xor_u64(best.key, o), (uint32_t)__shfl_xor((int)best.row, o)};
-        if (other.over(best)) best = other;
+    if (own != 0) {
+      const int at = place(wave + 1, own) + lane;
+      if (at < N) {
+        score[turn ^ 1][0][at] = own;
+        from[turn ^ 1][at] = (uint64_t)b << 32 | (uint32_t)~(uint32_t)mine;
       }
-      if (lane == 0) w_best[wave] = best;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (w_best[w].over(best)) best = w_best[w];
-      __syncthreads();
-      if (best.score == 0) break;  // uniform
-      if (own.score == best.score && own.key == best.key && own.row == best.row) {
-        store(k, best);
-        own = best_below(best, false);
-      }
-      ++got;
     }
+    if (wave == W - 1 && b0 > 0 && score[turn][0][lane] != 0) {
+      const int at = place(0, score[turn][0][lane]) + lane;
+      if (at < N) {
+        score[turn ^ 1][0][at] = score[turn][0][lane];
+        from[turn ^ 1][at] = from[turn][lane];
+      }
+    }
+    __syncthreads();
   }
-  for (int i = got + tid; i < a.N; i += THR) {
-    a.out_scores[out + i] = kNegInf;
-    a.out_beams[out + i] = a.out_tokens[out + i] = -1;
+  __syncthreads();
+  if (wave == 0 && lane < N) {
+    const uint64_t k = score[turn][0][lane], of = from[turn][lane];
+    a.out_scores[(int64_t)g * N + lane] = k != 0 ? (float)score_value(k) : kNegInf;
+    a.out_beams[(int64_t)g * N + lane] = k != 0 ? (int64_t)(of >> 32) : -1;
+    a.out_tokens[(int64_t)g * N + lane] = k != 0 ? (int64_t)(uint32_t)of : -1;
   }
 }
 
@@ -426,8 +467,8 @@ static int beam_parts(const sipa_beam_params* p) {
 }
 
 struct BeamLayout {
-  int parts, ns;
-  int64_t sum, val, tok, total;
+  int parts, ns, piece;
+  int64_t sum, key, total;
 };
 
 static int beam_layout(const sipa_beam_params* p, BeamLayout* l) {
@@ -439,16 +480,16 @@ static int beam_layout(const sipa_beam_params* p, BeamLayout* l) {
              p->num_candidates, kBeamMaxN);
   SIPA_CHECK(p->dtype == SIPA_F32 || p->dtype == SIPA_BF16 || p->dtype == SIPA_F16, SIPA_EUNSUPPORTED, "logits of type %d", p->dtype);
   l->parts = beam_parts(p);
-  const int piece = kBeamThreads * (p->dtype == SIPA_F32 ? 4 : 8) * l->parts;
-  l->ns = (p->vocab + piece - 1) / piece;
+  const int e = p->dtype == SIPA_F32 ? 4 : 8, most = kBeamThreads * e * l->parts;
+  l->ns = (p->vocab + most - 1) / most;
+  l->piece = ((p->vocab + l->ns - 1) / l->ns + e - 1) / e * e;  // alike, whole parts
+  l->ns = (p->vocab + l->piece - 1) / l->piece;
   const int64_t pieces = (int64_t)p->num_rows * l->ns;
-  SIPA_CHECK(pieces <= 0x7fffffff && (int64_t)std::min(p->num_rows, kBeamMaxRows) * l->ns * p->num_candidates <= 0x7fffffff,
-             SIPA_EUNSUPPORTED, "%d rows of %d pieces exceed the grid limit", p->num_rows, l->ns);
+  SIPA_CHECK(pieces <= 0x7fffffff, SIPA_EUNSUPPORTED, "%d rows of %d pieces exceed the grid limit", p->num_rows, l->ns);
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   l->sum = up(pieces * 4);
-  l->val = l->sum + up(pieces * 8);
-  l->tok = l->val + up(pieces * p->num_candidates * 4);
-  l->total = l->tok + up(pieces * p->num_candidates * 4);
+  l->key = l->sum + up(pieces * 8);
+  l->total = l->key + up(pieces * p->num_candidates * 8);
   return SIPA_OK;
 }
 
@@ -489,11 +530,13 @@ extern "C" int32_t sipa_beam_select(const sipa_beam_params* p, void* stream) {
   a.beams = p->beams;
   a.N = p->num_candidates;
   a.ns = l.ns;
+  a.piece = l.piece;
   char* ws = (char*)p->workspace;
   a.p_max = (float*)ws;
   a.p_sum = (double*)(ws + l.sum);
-  a.c_val = (float*)(ws + l.val);
-  a.c_tok = (int32_t*)(ws + l.tok);
+  a.p_key = (uint64_t*)(ws + l.key);
+  a.log_parts = 2;
+  while (1 << a.log_parts < a.N) ++a.log_parts;
   a.out_scores = p->out_scores;
   a.out_beams = p->out_beams;
   a.out_tokens = p->out_tokens;
@@ -504,7 +547,7 @@ extern "C" int32_t sipa_beam_select(const sipa_beam_params* p, void* stream) {
     else if (p->dtype == SIPA_BF16) launch_beam_rows<SIPA_BF16>(l.parts, grid, st, a);
     else launch_beam_rows<SIPA_F16>(l.parts, grid, st, a);
   }
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)p->num_groups), dim3(kBeamThreads), 0, st, a);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)p->num_groups), dim3(64 * kMergeWaves), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(SIPA_EHIP, "beam selection launch failed: %s", hipGetErrorString(e));
   return SIPA_OK;
