@@ -832,7 +832,7 @@ int64_t sipa_beam_workspace_bytes(const sipa_beam_params* p);
  * for i < num_copies, rows 0 .. tokens - 1 of block src become those of block dst, (src, dst, tokens) = copies[3 i ..]. Beams
  * that go on from the same one share its full blocks; its last block, where it is not full, is copied for all but one.
  * copies is HOST memory, read during the call (a captured call copies the same blocks at every replay). No block may be the
- * destination of two copies, or of one and the source of another (SIPA_EINVAL).
+ * destination of two copies, or of one and the source of another (SIPA_EINVAL). Blocks of up to 255 tokens.
  */
 typedef struct sipa_copy_params {
   int32_t struct_size; /* sizeof(sipa_copy_params) */

@@ -4,8 +4,8 @@
 // Selection, for row r (a beam) and token v:  score = cum[r] + l[r, v] - log sum_v exp(l[r, v]).  Within a row the logits
 // decide the order, so that one pass over them finds a row's best tokens and its sum together:
 //   beam_rows   a workgroup holds a piece of a row in registers, takes its maximum, the sum of exponentials below it, and
-//               its N largest logits: those above a threshold that at least N pass (the least of the maxima of at least N
-//               parts of the workgroup's lanes) are collected in LDS and put into order by counting.
+//               its N largest logits: those above a threshold that at least N pass (the N-th largest of the threads' maxima)
+//               are collected in LDS and put into order by counting.
 //   beam_merge  a workgroup a group, a wave a row: joins the pieces' sums in 64 bits and puts a row's candidates, then the
 //               group's, in order in the same way.
 // It reads every logit once; no sum depends on the order in which workgroups or waves run, so equal rows get equal sums.
@@ -27,7 +27,6 @@ struct BeamArgs {
   const int32_t* starts;
   int32_t R, V, beams, N;
   int32_t ns, piece;  // pieces of a row, logits of a piece
-  int32_t log_parts;  // 1 << log_parts >= N classes of lanes
   float* p_max;       // [R][ns]
   double* p_sum;      // [R][ns] sum of exp(l - p_max)
   uint64_t* p_key;    // [R][N][ns] the pieces' largest logits in order (beam_key), 0 behind them
@@ -58,8 +57,7 @@ __device__ __forceinline__ double score_value(uint64_t b) {
 }
 
 // Step K = 0 .. 5 of a butterfly over a wave: the value of a lane that the steps before have not brought together with this one.
-// Cross-lane moves of the vector unit, without LDS. After K steps the lanes that hold one value are spread evenly over the wave:
-// every 32nd, 16th, 8th, then pairs of those.
+// Cross-lane moves of the vector unit, without LDS.
 template <int K>
 __device__ __forceinline__ uint32_t other_lane(uint32_t x) {
   if constexpr (K == 0) {
@@ -96,6 +94,30 @@ __device__ __forceinline__ T butterfly(T x, F f) {  // f(K, own, other); every l
   else return butterfly<K + 1>(f(K, x, other_lane<K>(x)), f);
 }
 
+// fp32's upper 16 bits in order, and the least value that has them.
+__device__ __forceinline__ uint32_t upper_key(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (b & 0x80000000u ? ~b : b | 0x80000000u) >> 16;
+}
+
+__device__ __forceinline__ float upper_value(uint32_t key) {
+  return __uint_as_float(key & 0x8000u ? (key & 0x7fffu) << 16 : ~(key << 16));
+}
+
+// The N-th largest of a wave's 64 C 16-bit keys, C a lane (0 if there are fewer): a bit at a time, by counting.
+template <int C>
+__device__ __forceinline__ uint32_t nth_key(const uint32_t (&key)[C], int N) {
+  uint32_t t = 0;
+#pragma unroll
+  for (uint32_t bit = 0x8000u; bit > 0; bit >>= 1) {
+    int over = 0;
+#pragma unroll
+    for (int i = 0; i < C; ++i) over += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= (t | bit)));
+    t = over >= N ? t | bit : t;
+  }
+  return t;
+}
+
 __device__ __forceinline__ double wave_sum_f64(double x) {  // a + b and b + a are the same bits
   return butterfly(x, [](int, double a, double b) { return a + b; });
 }
@@ -106,29 +128,43 @@ __device__ __forceinline__ int keys_over(const uint64_t* list, int n, uint64_t k
 #pragma unroll 1
   for (int j = 0; j < n; j += 4) {
     const ulonglong2 a = *(const ulonglong2*)(list + j), b = *(const ulonglong2*)(list + j + 2);
-    const uint64_t k[4] = {a.x, a.y, b.x, b.y};
-#pragma unroll
-    for (int x = 0; x < 4; ++x) over += k[x] > key;
+    over += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key);
   }
   return over;
 }
 
+__device__ __forceinline__ int keys_over(const uint32_t* list, int n, uint32_t key) {
+  int over = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 4) {
+    const uint4 a = *(const uint4*)(list + j);
+    over += (a.x > key) + (a.y > key) + (a.z > key) + (a.w > key);
+  }
+  return over;
+}
+
+// A row's element: bits, how many make 16 bytes, and the key that orders those of a piece. Of 16-bit types it has 32 bits, the
+// value's 16 and the place's within the piece: half the LDS reads and comparisons.
 template <int DT>
-struct BeamType;
+struct BeamType {
+  typedef uint16_t T;
+  typedef uint32_t Key;
+  static constexpr int E = 8;
+  static __device__ __forceinline__ Key key(uint32_t bits, uint32_t at) {
+    bits = bits == 0x8000u ? 0u : bits;  // -0 as 0
+    return (bits & 0x8000u ? ~bits & 0xffffu : bits | 0x8000u) << 16 | (0xffffu - at);
+  }
+  static __device__ __forceinline__ uint32_t bits(Key key) { return key >> 31 ? key >> 16 & 0x7fffu : ~(key >> 16) & 0xffffu; }
+  static __device__ __forceinline__ uint32_t place(Key key) { return 0xffffu - (key & 0xffffu); }
+};
 template <>
 struct BeamType<SIPA_F32> {
   typedef uint32_t T;
+  typedef uint64_t Key;
   static constexpr int E = 4;
-};
-template <>
-struct BeamType<SIPA_BF16> {
-  typedef uint16_t T;
-  static constexpr int E = 8;
-};
-template <>
-struct BeamType<SIPA_F16> {
-  typedef uint16_t T;
-  static constexpr int E = 8;
+  static __device__ __forceinline__ Key key(uint32_t bits, uint32_t at) { return beam_key(__uint_as_float(bits), at); }
+  static __device__ __forceinline__ uint32_t bits(Key key) { return __float_as_uint(key_value(key)); }
+  static __device__ __forceinline__ uint32_t place(Key key) { return ~(uint32_t)key; }
 };
 
 template <int DT>
@@ -140,15 +176,16 @@ __device__ __forceinline__ float logit(uint32_t bits) {
 template <int DT, int PARTS>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs a) {
   typedef typename BeamType<DT>::T T;
+  typedef typename BeamType<DT>::Key Key;
   constexpr int THR = kBeamThreads, E = BeamType<DT>::E, BITS = 8 * sizeof(T);
   struct __attribute__((packed, aligned(sizeof(T)))) Part {
     uint32_t w[4];
   };
-  __shared__ __align__(16) uint64_t found[4][kBeamCap + 4];
+  __shared__ __align__(16) Key found[4][kBeamCap + 4];
   __shared__ float w_max[4][64];
   __shared__ double w_sum[4];
   __shared__ int w_count[4];
-  __shared__ uint64_t w_key[4];
+  __shared__ Key w_key[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = blockIdx.x / a.ns, piece = blockIdx.x - r * a.ns, v0 = piece * a.piece;
   const T* row = (const T*)a.logits + (int64_t)r * a.l_st + v0;
@@ -173,12 +210,16 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
     for (int i = 0; i < PARTS; ++i)
       if (last / THR == i) x[i] = y;
   }
+  auto bits = [&](int i, int e) {
+    const uint32_t w = x[i].w[BITS * e >> 5];
+    return BITS == 32 ? w : e & 1 ? w >> 16 : w & 0xffffu;
+  };
   auto value = [&](int i, int e) {
     const uint32_t w = x[i].w[BITS * e >> 5];
     if constexpr (DT == SIPA_BF16) return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
-    return logit<DT>(BITS == 32 ? w : e & 1 ? w >> 16 : w & 0xffffu);
+    return logit<DT>(bits(i, e));
   };
-  auto index = [&](int i, int e) { return (uint32_t)(v0 + E * (tid + THR * i) + e); };
+  auto place = [&](int i, int e) { return (uint32_t)(E * (tid + THR * i) + e); };
   float mine = kNegInf;
 #pragma unroll
   for (int i = 0; i < PARTS; ++i)
@@ -192,19 +233,25 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
       for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(x[i].w[w]));
   };
   keep();
-  // The maxima of classes of lanes, as many classes as candidates at least, and the least of them. (A class's lanes are spread
-  // over the workgroup: a short piece has some of each.)
-  const int within = 6 - a.log_parts;  // steps within a class
-  float best = mine;
-  best = butterfly(best, [&](int k, float p, float q) { return k < within ? fmaxf(p, q) : p; });
-  w_max[wave][lane] = best;
+  // Of the threads' maxima, or those of four threads each, the N-th largest is a threshold that N logits pass at least, and few
+  // more do (N = 16: 18 of a piece of 16384; the least maximum of 16 classes of threads let 53 pass, whose collection took a
+  // third of the time).
+  w_max[wave][lane] = mine;
   __syncthreads();
-  best = fmaxf(fmaxf(w_max[0][lane], w_max[1][lane]), fmaxf(w_max[2][lane], w_max[3][lane]));
+  const float of[4] = {w_max[0][lane], w_max[1][lane], w_max[2][lane], w_max[3][lane]};
+  const float best = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
   const float top = butterfly(best, [](int, float p, float q) { return fmaxf(p, q); });
-  float low = butterfly(best, [](int, float p, float q) { return fminf(p, q); });
+  float low;
+  if (a.N <= 32) {
+    const uint32_t key[1] = {upper_key(best)};
+    low = upper_value(nth_key(key, a.N));
+  } else {
+    const uint32_t key[4] = {upper_key(of[0]), upper_key(of[1]), upper_key(of[2]), upper_key(of[3])};
+    low = upper_value(nth_key(key, a.N));
+  }
   // exp(l - top) as exp2((l - top) log2 e): its argument is rounded, 2^-20 of the term at most where the term matters.
   const float off = top == kNegInf ? 0.f : top;
-  low = fmaxf(low, -__FLT_MAX__);  // never -inf
+  low = fmaxf(low, -__FLT_MAX__);  // never -inf (or NaN, which the key 0 stands for)
   double sum = 0.;
   int count = 0;
 #pragma unroll
@@ -217,7 +264,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
       const uint64_t hits = __builtin_amdgcn_ballot_w64(v >= low);
       if (hits) {
         const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0u));
-        if (v >= low && to < kBeamCap) found[wave][to] = beam_key(v, index(i, e));
+        if (v >= low && to < kBeamCap) found[wave][to] = BeamType<DT>::key(bits(i, e), place(i, e));
         count += __builtin_popcountll(hits);
       }
     }
@@ -232,36 +279,39 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
     a.p_max[at] = top;
     a.p_sum[at] = (w_sum[0] + w_sum[1]) + (w_sum[2] + w_sum[3]);
   }
-  uint64_t* out = a.p_key + (int64_t)r * a.ns * a.N + piece;  // rank i at i ns
+  auto store = [&](int rank, Key key) {
+    a.p_key[((int64_t)r * a.N + rank) * a.ns + piece] =
+        beam_key(logit<DT>(BeamType<DT>::bits(key)), (uint32_t)v0 + BeamType<DT>::place(key));
+  };
   const int all[4] = {w_count[0], w_count[1], w_count[2], w_count[3]};
   int got = 0;
   if (max(max(all[0], all[1]), max(all[2], all[3])) <= kBeamCap) {
     got = all[0] + all[1] + all[2] + all[3];
     for (int i = lane; i < count; i += 64) {
-      const uint64_t key = found[wave][i];  // no two are equal
+      const Key key = found[wave][i];  // no two are equal
       int rank = 0;
 #pragma unroll
       for (int w = 0; w < 4; ++w) rank += keys_over(found[w], all[w], key);
-      if (rank < a.N) out[(int64_t)rank * a.ns] = key;
+      if (rank < a.N) store(rank, key);
     }
   } else {
     // Most of the piece ties or rises: the largest key under the last one, N times. Only the thread that had it looks for
     // its next.
-    auto best_below = [&](uint64_t limit) {
-      uint64_t best = 0;
+    auto best_below = [&](Key limit) {
+      Key best = 0;
 #pragma unroll 1
       for (int i = 0; i < PARTS; ++i)
 #pragma unroll 1
-        for (int e = 0; e < E && E * (tid + THR * i) + e < n; ++e) {
-          const float v = logit<DT>(row[E * (tid + THR * i) + e]);
-          const uint64_t key = v > kNegInf ? beam_key(v, index(i, e)) : 0;
+        for (int e = 0; e < E && (int)place(i, e) < n; ++e) {
+          const uint32_t b = row[place(i, e)];
+          const Key key = logit<DT>(b) > kNegInf ? BeamType<DT>::key(b, place(i, e)) : 0;
           best = key < limit && key > best ? key : best;
         }
       return best;
     };
-    uint64_t own = best_below(~0ull);
+    Key own = best_below(~(Key)0);
     for (; got < a.N; ++got) {
-      uint64_t best = butterfly(own, [](int, uint64_t p, uint64_t q) { return p > q ? p : q; });
+      Key best = butterfly(own, [](int, Key p, Key q) { return p > q ? p : q; });
       if (lane == 0) w_key[wave] = best;
       __syncthreads();
 #pragma unroll
@@ -269,24 +319,24 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
       __syncthreads();
       if (best == 0) break;  // uniform
       if (own == best) {
-        out[(int64_t)got * a.ns] = best;
+        store(got, best);
         own = best_below(best);
       }
     }
   }
-  for (int i = got + tid; i < a.N; i += THR) out[(int64_t)i * a.ns] = 0;
+  for (int i = got + tid; i < a.N; i += THR) a.p_key[((int64_t)r * a.N + i) * a.ns + piece] = 0;
 }
 
 // The N largest of a wave's keys (no two equal, 0: none), SLOTS a lane, in order, to best[0 ..] in LDS. list: room for
 // 64 SLOTS + 4 keys.
 template <int SLOTS>
-__device__ __forceinline__ void wave_select(const uint64_t (&key)[SLOTS], int N, int log_parts, uint64_t* list, uint64_t* best) {
+__device__ __forceinline__ void wave_select(const uint64_t (&key)[SLOTS], int N, uint64_t* list, uint64_t* best) {
   const int lane = threadIdx.x & 63;
-  uint64_t low = 0;
+  uint64_t most = 0;
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) low = key[i] > low ? key[i] : low;
-  low = butterfly(low, [&](int k, uint64_t p, uint64_t q) { return (k < 6 - log_parts) == (p > q) ? p : q; });
-  low = low == 0 ? 1 : low;
+  for (int i = 0; i < SLOTS; ++i) most = key[i] > most ? key[i] : most;
+  const uint32_t upper[1] = {(uint32_t)(most >> 48)};
+  const uint64_t low = max((uint64_t)nth_key(upper, N) << 48, (uint64_t)1);
   int n = 0;
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
@@ -336,14 +386,15 @@ __global__ void __launch_bounds__(64 * kMergeWaves) beam_merge_kernel(const Beam
       };
       load(0);
       // the row's sum
-      float top = kNegInf;
-      for (int i = lane; i < a.ns; i += 64) top = fmaxf(top, a.p_max[first + i]);
+      float m = lane < a.ns ? a.p_max[first + lane] : kNegInf, top = m;
+      double s = lane < a.ns ? a.p_sum[first + lane] : 0.;
+      for (int i = lane + 64; i < a.ns; i += 64) top = fmaxf(top, a.p_max[first + i]);
       top = butterfly(top, [](int, float p, float q) { return fmaxf(p, q); });
       double sum = 0.;
-      for (int i = lane; i < a.ns; i += 64) {
-        const float m = a.p_max[first + i];
-        const double s = a.p_sum[first + i];
+      for (int i = lane;;) {
         sum += m == kNegInf ? s : s * exp((double)m - (double)top);
+        if ((i += 64) >= a.ns) break;
+        m = a.p_max[first + i], s = a.p_sum[first + i];
       }
       sum = wave_sum_f64(sum);
       off = (double)a.cum[r0 + b] - ((double)top + log(sum));
@@ -355,7 +406,7 @@ __global__ void __launch_bounds__(64 * kMergeWaves) beam_merge_kernel(const Beam
           if (i0 + 64 * i + lane >= total) key[i + 1] = 0;
         row_best[wave][lane] = 0;
         wave_sync();
-        wave_select<SLOTS>(key, N, a.log_parts, list[wave], row_best[wave]);
+        wave_select<SLOTS>(key, N, list[wave], row_best[wave]);
         wave_sync();
         mine = row_best[wave][lane];
       }
@@ -411,7 +462,7 @@ __global__ void __launch_bounds__(64 * kMergeWaves) beam_merge_kernel(const Beam
 
 // ---- copies of blocks --------------------------------------------------------------------------------------------------
 
-constexpr int kCopiesPerLaunch = 256, kCopyPools = 4, kCopyUnroll = 4;
+constexpr int kCopiesPerLaunch = 424, kCopyPools = 4, kCopyUnroll = 8;  // (as many as kernel arguments hold, 4 KB)
 
 struct CopyArgs {
   char* pool[kCopyPools];
@@ -421,35 +472,47 @@ struct CopyArgs {
   int32_t log_lanes[kCopyPools];   // lanes of a (layer, head)
   int32_t L, H, B;
   int32_t src[kCopiesPerLaunch], dst[kCopiesPerLaunch];
-  uint16_t tokens[kCopiesPerLaunch];
+  uint8_t tokens[kCopiesPerLaunch];
 };
+static_assert(sizeof(CopyArgs) <= 4096, "kernel arguments");
 
-// Workgroup (copy, y, pool): (layer, head) segments of one block, 1 << log_lanes lanes side by side on each.
+// Workgroup (copy, y, pool): (layer, head) segments of one block, 1 << log_lanes lanes side by side on each, kCopyUnroll segments
+// a thread with all their loads ahead of the stores, which go past the caches: 384 copies in 28 layers of INT8 pools, 128 MB read
+// and written, 24 us (5.2 TB/s; with ordinary stores 41, with loads past the caches too 28).
 template <typename U>
 __device__ __forceinline__ void copy_segments(const CopyArgs& a, int pool, int c) {
-  const int lanes = 1 << a.log_lanes[pool], per = (256 >> a.log_lanes[pool]), lane = threadIdx.x & (lanes - 1);
-  const int units = (int)((int64_t)a.tokens[c] * a.row[pool] / (int)sizeof(U)), all = a.L * a.H;
-  const int64_t block = (int64_t)a.B * a.row[pool];
-  const int first = blockIdx.y * per * kCopyUnroll + (threadIdx.x >> a.log_lanes[pool]);
-  if (first >= all) return;
-  for (int u = lane; u < units; u += lanes) {
+  const int log_lanes = a.log_lanes[pool], per = 256 >> log_lanes, lane = threadIdx.x & ((1 << log_lanes) - 1);
+  const int row = a.row[pool], units = a.tokens[c] * row / (int)sizeof(U), all = a.L * a.H;
+  const int64_t block = (int64_t)a.B * row, to = (a.dst[c] - a.src[c]) * block, st_l = a.st_l[pool], st_h = a.st_h[pool];
+  const int first = blockIdx.y * per * kCopyUnroll + (threadIdx.x >> log_lanes);
+  if (first >= all || lane >= units) return;
+  const int dl = per / a.H, dh = per - dl * a.H;  // uniform
+  const int64_t step = dl * st_l + dh * st_h, wrap = st_l - a.H * st_h;
+  const int l0 = first / a.H, h0 = first - l0 * a.H;
+  char* base = a.pool[pool] + a.src[c] * block + l0 * st_l + h0 * st_h;
+  for (int u = lane; u < units; u += 1 << log_lanes) {
     U x[kCopyUnroll];
-    char* at[kCopyUnroll];
+    char* at = base + u * (int)sizeof(U);
+    auto each = [&](auto f) {
+      char* p = at;
+      int h = h0;
 #pragma unroll
-    for (int i = 0; i < kCopyUnroll; ++i) {
-      const int seg = min(first + per * i, all - 1), l = seg / a.H;
-      at[i] = a.pool[pool] + l * a.st_l[pool] + (seg - l * a.H) * a.st_h[pool];
-      x[i] = *((const U*)(at[i] + a.src[c] * block) + u);
-    }
-#pragma unroll
-    for (int i = 0; i < kCopyUnroll; ++i)
-      if (first + per * i < all) *((U*)(at[i] + a.dst[c] * block) + u) = x[i];
+      for (int i = 0; i < kCopyUnroll; ++i) {
+        if (i == 0 || first + per * i < all) f(i, p);
+        p += step;
+        h += dh;
+        p += h >= a.H ? wrap : 0;
+        h -= h >= a.H ? a.H : 0;
+      }
+    };
+    each([&](int i, char* p) { x[i] = *(const U*)p; });
+    each([&](int i, char* p) { __builtin_nontemporal_store(x[i], (U*)(p + to)); });
   }
 }
 
 __global__ void __launch_bounds__(256) copy_blocks_kernel(const CopyArgs a) {
   const int pool = blockIdx.z, c = blockIdx.x;
-  if (a.unit[pool] == 16) copy_segments<uint4>(a, pool, c);
+  if (a.unit[pool] == 16) copy_segments<u32x4>(a, pool, c);
   else if (a.unit[pool] == 2) copy_segments<uint16_t>(a, pool, c);
   else copy_segments<uint8_t>(a, pool, c);
 }
@@ -458,12 +521,14 @@ __global__ void __launch_bounds__(256) copy_blocks_kernel(const CopyArgs a) {
 
 using namespace sipa;
 
-// Pieces of a row: parts of a thread, by type.
+// Parts of a thread: the most, up to 8, that leave two workgroups a CU; 2 at least, from 32 candidates on 4, as the merge pays for
+// each piece. Times in us with 2 / 4 / 8 parts, 16-bit logits of 151936 tokens: 4 rows, 8 candidates 10.8 / 11.6 / 12.4; 32 rows
+// 13.5 / 13.2 / 14.4; 128 rows, 16 candidates 25.3 / 20.6 / 20.6; 512 rows 61 / 45 / 42.5; 1 row, 64 candidates 28 / 20.5 / 19.3.
+// (16 parts, 137 registers: 512 rows 50.)
 static int beam_parts(const sipa_beam_params* p) {
-  const int e = p->dtype == SIPA_F32 ? 4 : 8;
-  for (int parts = 8; parts > 1; parts /= 2)
-    if ((int64_t)p->num_rows * ((p->vocab + kBeamThreads * e * parts - 1) / (kBeamThreads * e * parts)) >= 512) return parts;
-  return 1;
+  const int piece = kBeamThreads * (p->dtype == SIPA_F32 ? 4 : 8);
+  const auto workgroups = [&](int parts) { return (int64_t)p->num_rows * ((p->vocab + piece * parts - 1) / (piece * parts)); };
+  return workgroups(8) >= 512 ? 8 : workgroups(4) >= 512 || p->num_candidates >= 32 ? 4 : 2;
 }
 
 struct BeamLayout {
@@ -503,8 +568,7 @@ template <int DT>
 static void launch_beam_rows(int parts, unsigned grid, hipStream_t st, const BeamArgs& a) {
   if (parts == 8) hipLaunchKernelGGL((beam_rows_kernel<DT, 8>), dim3(grid), dim3(kBeamThreads), 0, st, a);
   else if (parts == 4) hipLaunchKernelGGL((beam_rows_kernel<DT, 4>), dim3(grid), dim3(kBeamThreads), 0, st, a);
-  else if (parts == 2) hipLaunchKernelGGL((beam_rows_kernel<DT, 2>), dim3(grid), dim3(kBeamThreads), 0, st, a);
-  else hipLaunchKernelGGL((beam_rows_kernel<DT, 1>), dim3(grid), dim3(kBeamThreads), 0, st, a);
+  else hipLaunchKernelGGL((beam_rows_kernel<DT, 2>), dim3(grid), dim3(kBeamThreads), 0, st, a);
 }
 
 extern "C" int32_t sipa_beam_select(const sipa_beam_params* p, void* stream) {
@@ -535,8 +599,6 @@ extern "C" int32_t sipa_beam_select(const sipa_beam_params* p, void* stream) {
   a.p_max = (float*)ws;
   a.p_sum = (double*)(ws + l.sum);
   a.p_key = (uint64_t*)(ws + l.key);
-  a.log_parts = 2;
-  while (1 << a.log_parts < a.N) ++a.log_parts;
   a.out_scores = p->out_scores;
   a.out_beams = p->out_beams;
   a.out_tokens = p->out_tokens;
@@ -558,39 +620,52 @@ extern "C" int32_t sipa_check_copies(const int32_t* copies, int32_t num_copies, 
              num_blocks, block_size);
   if (num_copies == 0) return SIPA_OK;
   SIPA_CHECK(copies != nullptr, SIPA_EINVAL, "NULL pointer");
-  // every block with 1 where it is a destination, in order: equal neighbours that are not both sources collide
-  constexpr int kHere = 256;
-  uint64_t here[2 * kHere];
-  std::unique_ptr<uint64_t[]> more;
-  uint64_t* of = here;
-  if (num_copies > kHere) {
-    more.reset(new (std::nothrow) uint64_t[2 * (size_t)num_copies]);
-    SIPA_CHECK(more != nullptr, SIPA_EINVAL, "no memory for %d copies", num_copies);
-    of = more.get();
-  }
   for (int i = 0; i < num_copies; ++i) {
     const int32_t* c = copies + 3 * (int64_t)i;
     SIPA_CHECK(c[0] >= 0 && c[0] < num_blocks && c[1] >= 0 && c[1] < num_blocks && c[2] >= 0 && c[2] <= block_size,
                SIPA_EINVAL, "copy %d: %d tokens of block %d to block %d (%d blocks of %d tokens)", i, c[2], c[0], c[1],
                num_blocks, block_size);
-    of[2 * (int64_t)i] = 2 * (uint64_t)c[0], of[2 * (int64_t)i + 1] = 2 * (uint64_t)c[1] + 1;
   }
-  std::sort(of, of + 2 * (int64_t)num_copies);
-  for (int64_t i = 1; i < 2 * (int64_t)num_copies; ++i)
-    SIPA_CHECK(of[i] >> 1 != of[i - 1] >> 1 || of[i] % 2 == 0, SIPA_EINVAL,
-               "block %lld is the destination of two copies, or of one and the source of another", (long long)(of[i] >> 1));
+  // The destinations in a hash table at most half full (block + 1, 0 for free), then the sources looked up in it.
+  constexpr int kHere = 1024;
+  uint32_t here[kHere];
+  std::unique_ptr<uint32_t[]> more;
+  uint32_t* table = here;
+  int64_t size = kHere;
+  while (size < 2 * (int64_t)num_copies) size *= 2;
+  if (size > kHere) {
+    more.reset(new (std::nothrow) uint32_t[size]);
+    SIPA_CHECK(more != nullptr, SIPA_EINVAL, "no memory for %d copies", num_copies);
+    table = more.get();
+  }
+  std::fill(table, table + size, 0u);
+  const auto slot = [&](int32_t block) {  // of the block, or the free one where it would stand
+    int64_t i = ((uint32_t)block * 2654435761u) & (size - 1);
+    while (table[i] != 0 && table[i] != (uint32_t)block + 1) i = (i + 1) & (size - 1);
+    return i;
+  };
+  for (int i = 0; i < num_copies; ++i) {
+    const int32_t d = copies[3 * (int64_t)i + 1];
+    const int64_t at = slot(d);
+    SIPA_CHECK(table[at] == 0, SIPA_EINVAL, "block %d is the destination of two copies", d);
+    table[at] = (uint32_t)d + 1;
+  }
+  for (int i = 0; i < num_copies; ++i)
+    SIPA_CHECK(table[slot(copies[3 * (int64_t)i])] == 0, SIPA_EINVAL,
+               "block %d is the destination of one copy and the source of another", copies[3 * (int64_t)i]);
   return SIPA_OK;
 }
 
 extern "C" int32_t sipa_copy_blocks(const sipa_copy_params* p, void* stream) {
   SIPA_CHECK(p != nullptr && p->struct_size == (int32_t)sizeof(sipa_copy_params), SIPA_EINVAL,
              "struct_size does not match this library's sipa_copy_params (%d bytes)", (int)sizeof(sipa_copy_params));
-  SIPA_CHECK(p->num_layers >= 0 && p->num_kv_heads >= 0 && p->num_blocks >= 0 && p->block_size > 0 && p->block_size <= 65535 &&
+  SIPA_CHECK(p->num_layers >= 0 && p->num_kv_heads >= 0 && p->num_blocks >= 0 && p->block_size > 0 &&
                  p->num_copies >= 0 && p->num_pools >= 1 && p->num_pools <= kCopyPools &&
                  (int64_t)p->num_layers * p->num_kv_heads <= 1 << 24, SIPA_EINVAL,
              "%d layers of %d heads, %d blocks of %d tokens, %d pools, %d copies", p->num_layers, p->num_kv_heads, p->num_blocks,
              p->block_size, p->num_pools, p->num_copies);
   if (p->num_copies == 0 || p->num_layers == 0 || p->num_kv_heads == 0) return SIPA_OK;
+  SIPA_CHECK(p->block_size <= 255, SIPA_EUNSUPPORTED, "blocks of %d tokens (up to 255)", p->block_size);
   const int rc = sipa_check_copies(p->copies, p->num_copies, p->num_blocks, p->block_size);
   if (rc != SIPA_OK) return rc;
   CopyArgs a;
@@ -607,8 +682,8 @@ extern "C" int32_t sipa_copy_blocks(const sipa_copy_params* p, void* stream) {
     a.st_h[i] = p->stride_h[i];
     a.row[i] = (int32_t)row;
     a.unit[i] = (of & 15) == 0 ? 16 : (of & 1) == 0 ? 2 : 1;
-    int log = 0;  // lanes for a whole block, a wave at most
-    while (log < 6 && (int64_t)a.unit[i] << log < row * p->block_size) ++log;
+    int log = 0;  // lanes for a whole block, a workgroup at most
+    while (log < 8 && (int64_t)a.unit[i] << log < row * p->block_size) ++log;
     a.log_lanes[i] = log;
     const int per = (256 >> log) * kCopyUnroll;
     most = std::max(most, (a.L * a.H + per - 1) / per);
@@ -618,7 +693,7 @@ extern "C" int32_t sipa_copy_blocks(const sipa_copy_params* p, void* stream) {
     const int n = std::min(kCopiesPerLaunch, p->num_copies - first);
     for (int i = 0; i < n; ++i) {
       const int32_t* c = p->copies + 3 * ((int64_t)first + i);
-      a.src[i] = c[0], a.dst[i] = c[1], a.tokens[i] = (uint16_t)c[2];
+      a.src[i] = c[0], a.dst[i] = c[1], a.tokens[i] = (uint8_t)c[2];
     }
     hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)n, (unsigned)most, (unsigned)p->num_pools), dim3(256), 0,
                        (hipStream_t)stream, a);

@@ -246,10 +246,10 @@ SIGNATURES = {
     "sipa_commit_tokens": (i32, [vp, vp]),  # a packed or ctypes CommitParams
     "sipa_prefix_plan": (i32, [_c.POINTER(PrefixParams), i32, vp, vp, vp, vp, vp, i64, _c.POINTER(PrefixLayout)]),
     "sipa_prefix_attention": (i32, [_c.POINTER(PrefixParams), vp]),
-    "sipa_beam_workspace_bytes": (i64, [_c.POINTER(BeamParams)]),
-    "sipa_beam_select": (i32, [_c.POINTER(BeamParams), vp]),
+    "sipa_beam_workspace_bytes": (i64, [vp]),  # a packed or ctypes BeamParams
+    "sipa_beam_select": (i32, [vp, vp]),
     "sipa_check_copies": (i32, [vp, i32, i32, i32]),
-    "sipa_copy_blocks": (i32, [_c.POINTER(CopyParams), vp]),
+    "sipa_copy_blocks": (i32, [vp, vp]),  # a packed or ctypes CopyParams
 }
 
 _lib = None

@@ -13,10 +13,13 @@ A step over the beams of a batch, which share their blocks (engine.block_manager
 from __future__ import annotations
 
 import ctypes
+import functools
+import itertools
+import struct
+from array import array
 from collections.abc import Sequence
 from typing import NamedTuple
 
-import numpy as np
 import torch
 
 from . import _hip
@@ -24,6 +27,10 @@ from . import _hip
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 MAX_CANDIDATES = 64
 MAX_BEAMS = 1024
+# sipa_beam_params and sipa_copy_params as bytes (native alignment), as engine.hip_tree packs its own
+_SELECT = struct.Struct("7iPq6Pq")
+_COPY = struct.Struct("6i4P4q4q4iPi4x")
+assert _SELECT.size == ctypes.sizeof(_hip.BeamParams) and _COPY.size == ctypes.sizeof(_hip.CopyParams)
 
 
 class BeamChoice(NamedTuple):
@@ -64,26 +71,32 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int | torch.T
         raise ValueError(f"logits, scores and starts must be on one device, got {sorted(map(str, devices))}")
     if not logits.is_cuda:
         return _select_torch(logits, scores, starts, beams, groups, candidates)
-    dev = logits.device
-    out = BeamChoice(torch.empty(groups, candidates, dtype=torch.float32, device=dev),
-                     *(torch.empty(groups, candidates, dtype=torch.int64, device=dev) for _ in range(2)))
+    dev, code, n = logits.device, _hip.dtype_code(logits.dtype), candidates
+    both = torch.empty(2, groups, n, dtype=torch.int64, device=dev)
+    out = BeamChoice(torch.empty(groups, n, dtype=torch.float32, device=dev), both[0], both[1])
     if groups == 0:
         return out
-    p = _hip.BeamParams(struct_size=ctypes.sizeof(_hip.BeamParams), num_rows=R, vocab=V, num_groups=groups, beams=beams,
-                        num_candidates=candidates, dtype=_hip.dtype_code(logits.dtype), logits=logits.data_ptr(),
-                        logits_stride=logits.stride(0), scores=scores.data_ptr(), starts=_hip.ptr(starts),
-                        out_scores=out.scores.data_ptr(), out_beams=out.beams.data_ptr(), out_tokens=out.tokens.data_ptr())
-    lib, ref = _hip.lib(), ctypes.byref(p)
-    n = lib.sipa_beam_workspace_bytes(ref)
-    if n < 0:
-        _hip.check(n, "beam_select")
+    size = _select_bytes(R, V, groups, beams, n, code)
+    at = both.data_ptr()
     with _hip.on_device(dev):
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), n
-        rc = lib.sipa_beam_select(ref, _hip.stream_of(logits))
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        p = _SELECT.pack(_SELECT.size, R, V, groups, beams, n, code, logits.data_ptr(), logits.stride(0), scores.data_ptr(),
+                         0 if starts is None else starts.data_ptr(), out.scores.data_ptr(), at, at + 8 * groups * n,
+                         ws.data_ptr(), size)
+        rc = _hip.lib().sipa_beam_select(p, _hip.stream_of(logits))
     if rc:
         _hip.check(rc, "beam_select")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _select_bytes(rows: int, vocab: int, groups: int, beams: int, candidates: int, dtype: int) -> int:
+    """Workspace bytes of a selection of these sizes."""
+    n = _hip.lib().sipa_beam_workspace_bytes(_SELECT.pack(_SELECT.size, rows, vocab, groups, beams, candidates, dtype, 0, 0, 0, 0,
+                                                          0, 0, 0, 0, 0))
+    if n < 0:
+        _hip.check(n, "beam_select")
+    return n
 
 
 def _select_torch(logits, scores, starts, beams: int, groups: int, candidates: int) -> BeamChoice:
@@ -112,41 +125,46 @@ def _select_torch(logits, scores, starts, beams: int, groups: int, candidates: i
 
 def copy_blocks(pools: Sequence[torch.Tensor], copies: Sequence[tuple[int, int, int]]) -> None:
     """For each (src, dst, tokens) of copies, the first `tokens` tokens of block src become those of block dst, in every layer
-    and head of the pools, in place (sipa_copy_blocks; one launch for 256 copies). No block may be the destination of two
+    and head of the pools, in place (sipa_copy_blocks; one launch for 424 copies). No block may be the destination of two
     copies, or of one and the source of another.
 
     pools: one to four tensors [L, Hkv, N, B, ...], a cache's K, V and their per-token scales, each head's blocks contiguous.
-    The copies are the host's: a graph captures the ones it was given. CPU pools are copied by torch operations."""
-    if not 1 <= len(pools) <= 4:
-        raise ValueError(f"{len(pools)} pools (1 to 4)")
-    L, H, N, B = pools[0].shape[:4]
-    for t in pools:
-        if t.dim() < 4 or t.shape[:4] != (L, H, N, B) or t.device != pools[0].device:
+    Blocks of up to 255 tokens on the GPU. The copies are the host's: a graph captures the ones it was given. CPU pools are copied by torch operations."""
+    P, n = len(pools), len(copies)
+    if not 1 <= P <= 4:
+        raise ValueError(f"{P} pools (1 to 4)")
+    first = pools[0]
+    L, H, N, B = lead = first.shape[:4]
+    dev, ptrs, st_l, st_h, row_bytes = first.device, [0] * 4, [0] * 4, [0] * 4, [0] * 4
+    for i, t in enumerate(pools):
+        if t.shape[:4] != lead or t.device != dev:
             raise ValueError(f"the pools must be {(L, H, N, B, '...')} on one device")
-        if t.numel() and not t[0, 0].is_contiguous():
+        size, st = t.element_size(), t.stride()
+        row = 1
+        for x, y in zip(t.shape[:3:-1], st[:3:-1]):
+            if x > 1 and y != row:
+                raise ValueError("each head's blocks must be contiguous")
+            row *= x
+        if (B > 1 and st[3] != row) or (N > 1 and st[2] != B * row):
             raise ValueError("each head's blocks must be contiguous")
-    n = len(copies)
+        ptrs[i], st_l[i], st_h[i], row_bytes[i] = t.data_ptr(), st[0] * size, st[1] * size, row * size
     if not n:
         return
-    flat = np.fromiter((x for c in copies for x in c), dtype=np.int64)
-    if flat.size != 3 * n or any(len(c) != 3 for c in copies):
+    try:
+        flat = array("i", itertools.chain.from_iterable(copies))
+    except OverflowError:
+        raise ValueError(f"copies past the {N} blocks of {B} tokens") from None
+    if len(flat) != 3 * n or set(map(len, copies)) != {3}:
         raise ValueError("copies must be (src, dst, tokens)")
-    if flat.min() < 0 or flat.max() >= 1 << 31:
-        raise ValueError(f"copies past the {N} blocks of {B} tokens")
-    flat = flat.astype(np.int32)
-    if not pools[0].is_cuda:
-        _hip.check(_hip.lib().sipa_check_copies(flat.ctypes.data, n, N, B), "copy_blocks")
+    at = flat.buffer_info()[0]
+    if not first.is_cuda:
+        _hip.check(_hip.lib().sipa_check_copies(at, n, N, B), "copy_blocks")
         for t in pools:
             for s, d, rows in copies:
                 t[:, :, d, :rows] = t[:, :, s, :rows]
         return
-    p = _hip.CopyParams(struct_size=ctypes.sizeof(_hip.CopyParams), num_layers=L, num_kv_heads=H, num_blocks=N, block_size=B,
-                        num_pools=len(pools), copies=flat.ctypes.data, num_copies=n)
-    for i, t in enumerate(pools):
-        size = t.element_size()
-        p.pools[i], p.stride_l[i], p.stride_h[i] = t.data_ptr(), t.stride(0) * size, t.stride(1) * size
-        p.row_bytes[i] = t[0, 0, 0, 0].numel() * size if t.numel() else size
-    with _hip.on_device(pools[0].device):
-        rc = _hip.lib().sipa_copy_blocks(ctypes.byref(p), _hip.stream_of(pools[0]))
+    p = _COPY.pack(_COPY.size, L, H, N, B, P, *ptrs, *st_l, *st_h, *row_bytes, at, n)
+    with _hip.on_device(dev):
+        rc = _hip.lib().sipa_copy_blocks(p, _hip.stream_of(first))
     if rc:
         _hip.check(rc, "copy_blocks")
