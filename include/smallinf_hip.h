@@ -753,7 +753,7 @@ uint64_t sipa_capture_id(void* stream);
  * same sizes, any tensors and any context lengths up to max_context.
  */
 typedef struct sipa_prefix_layout {
-  int32_t num_items, num_members, tile_rows, own_splits, own_chunk;
+  int32_t num_items, num_pieces, num_members, tile_rows, reserved;
   int64_t plan_ints, workspace_bytes;
 } sipa_prefix_layout;
 

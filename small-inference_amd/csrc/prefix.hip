@@ -4,9 +4,10 @@
 // One token a sequence. A row (sequence, query head) splits its softmax over the keys of its group's prefix and those of its
 // own: (m, l, O) of each part, m the part's largest score, l = sum 2^(s - m), O = sum 2^(s - m) v, joined as
 //   M = max m,  out = sum 2^(m - M) O / sum 2^(m - M) l.
-// Prefix items: (group, KV head, up to ROWS of the group's rows, keys): the members' G query heads make one matrix of rows
-// that see every key, so the product has full tiles whatever G is. Own items: (sequence, KV head, keys), G rows of 16.
-// Both kinds are workgroups of one launch; a second, small one joins a row's parts.
+// Prefix items: (group, KV head, up to ROWS of the group's rows, keys), a workgroup each: the members' G query heads make one
+// matrix of rows that see every key, so the product has full tiles whatever G is. Own pieces: (sequence, KV head, keys), G rows
+// of 16, a wave each, eight to a workgroup: most are short, and a wave needs no other. Both kinds are in one launch, so that the
+// pieces' loads run beside the items' products; a second, small one joins a row's parts.
 #include <algorithm>
 
 #include "decode_common.h"
@@ -15,6 +16,7 @@ namespace sipa {
 
 constexpr int kPrefixMaxChunk = 16384;  // keys of a prefix item: its block ids stand in LDS
 constexpr int kPrefixThreads = 512, kPrefixWaves = 8;
+constexpr int kPrefixStage = 64;  // keys in LDS at a time
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -32,54 +34,67 @@ struct PrefixArgs {
   const void* vs;
   bool ks_f32, vs_f32;
   int64_t ks_sh, ks_sn, vs_sh, vs_sn;
-  const int32_t* items;    // [num_items][8]: table row, first member, rows, first row, KV head, first key, end, -
-  const int32_t* rows;     // [S][8]: prefix tokens, first row in the group, first state, splits, row tiles, -
-  const int32_t* members;  // batch rows of the groups, one group after the other
-  int32_t num_items, num_members, S, Hkv, G, nb, max_ctx;
+  // The plan. Items: table row, first member, rows, first row, KV head, first key, end, state. Pieces: batch row, KV head, which
+  // of the row's, how many those are, prefix tokens, state, -, -. Rows: prefix tokens, first row in the group, first state,
+  // splits, row tiles, first piece's state, pieces of a KV head, -. Members: batch rows of the groups, one group after the other.
+  const int32_t* items;    // [num_items][8]
+  const int32_t* pieces;   // [num_pieces][8]
+  const int32_t* rows;     // [S][8]
+  const int32_t* members;  // [num_members]
+  int32_t num_items, num_pieces, num_members, S, Hkv, G, nb, max_ctx;
   int32_t log_b;           // blocks of 1 << log_b tokens
-  int32_t nsplit, chunk;   // of the sequences' own keys
   int32_t tile_rows;       // rows of a prefix item
   float scale_log2;
-  float* p_m;              // [num_items][tile_rows]
-  float* p_l;
-  float* p_o;              // [num_items][tile_rows][D]
-  float* s_m;              // [S Hkv][nsplit][G]
-  float* s_l;
-  float* s_o;              // [S Hkv][nsplit][G][D]
+  // States, of the items' rows, then of the pieces': O, and (m, l).
+  float* st_o;             // [num_items tile_rows + num_pieces G][D]
+  float2* st_ml;
 };
 
-// A sequence's keys: the prefix's `shared` (read with its group, or 0), then splits of `chunk` keys of its own. A context that
-// is shorter than its group's prefix is read by itself, from its first key on.
+// Stores of states, in device memory: the two paths' would else be joined into flat ones, which also look for LDS.
+typedef __attribute__((address_space(1))) f32x4 GlobalF32x4;
+typedef __attribute__((address_space(1))) uint64_t GlobalU64;
+
+// A sequence's keys: the prefix's `shared` (read with its group, or 0), then up to `planned` pieces of `chunk` keys of its own. A
+// context that is shorter than its group's prefix is read by itself, from its first key on.
 struct OwnKeys {
-  int shared, ctx, chunk, splits;
+  int shared, ctx, chunk, pieces;
 };
 
-__device__ __forceinline__ OwnKeys own_keys(const PrefixArgs& a, int s) {
+__device__ __forceinline__ OwnKeys own_keys(const PrefixArgs& a, int s, int tokens, int planned) {
   OwnKeys k;
-  const int tokens = a.rows[8 * (int64_t)s];
   k.ctx = min(max(a.ctx[s], 0), a.max_ctx);
   k.shared = k.ctx >= tokens ? tokens : 0;
   const int own = k.ctx - k.shared;
-  k.chunk = max(a.chunk, ((own + a.nsplit - 1) / a.nsplit + 63) & ~63);
-  k.splits = (own + k.chunk - 1) / k.chunk;
+  k.chunk = max(((own + planned - 1) / planned + 31) & ~31, 32);
+  k.pieces = (own + k.chunk - 1) / k.chunk;
   return k;
 }
 
-// The four scales of consecutive keys, at any alignment, as fp32.
-__device__ __forceinline__ f32x4 four_scales(const void* base, bool f32, int64_t i) {
-  struct __attribute__((packed, aligned(4))) Four {
-    float x[4];
-  };
-  struct __attribute__((packed, aligned(2))) Halves {
+// The four scales of consecutive keys, at any alignment, as they lie in memory, and their values: apart, so that the loads are
+// waited for only where the values are needed. (fp16 scales: both halves are the same eight bytes.)
+__device__ __forceinline__ u32x4 load_scales(const void* base, bool f32, int64_t i) {
+  struct __attribute__((packed, aligned(2))) Eight {
     uint32_t w[2];
   };
-  if (f32) {
-    const Four s = *(const Four*)((const float*)base + i);
-    return f32x4{s.x[0], s.x[1], s.x[2], s.x[3]};
-  }
-  const Halves s = *(const Halves*)((const uint16_t*)base + i);
-  return f32x4{f16_bits_to_f32(s.w[0] & 0xffff), f16_bits_to_f32(s.w[0] >> 16), f16_bits_to_f32(s.w[1] & 0xffff),
-               f16_bits_to_f32(s.w[1] >> 16)};
+  const char* at = (const char*)base + i * (f32 ? 4 : 2);
+  const Eight lo = *(const Eight*)at, hi = *(const Eight*)(at + (f32 ? 8 : 0));
+  return u32x4{lo.w[0], lo.w[1], hi.w[0], hi.w[1]};
+}
+
+__device__ __forceinline__ f32x4 four_scales(u32x4 s, bool f32) {
+  const f32x4 half = {f16_bits_to_f32(s[0] & 0xffff), f16_bits_to_f32(s[0] >> 16), f16_bits_to_f32(s[1] & 0xffff),
+                      f16_bits_to_f32(s[1] >> 16)};
+  return f32 ? __builtin_bit_cast(f32x4, s) : half;
+}
+
+// One scale, by halves (of fp16 both are the same): loads under a branch of the type would be waited for at its end.
+__device__ __forceinline__ u32x2 load_scale(const void* base, bool f32, int64_t i) {
+  const uint16_t* at = (const uint16_t*)base + (f32 ? 2 * i : i);
+  return u32x2{at[0], at[f32 ? 1 : 0]};
+}
+
+__device__ __forceinline__ float one_scale(u32x2 s, bool f32) {
+  return f32 ? __uint_as_float(s[0] | s[1] << 16) : f16_bits_to_f32(s[0]);
 }
 
 // The softmax state of 16 rows in a wave, lane (r, q4) holding row r: O^T in the accumulators' layout (channels 16 dt + 4 q4 + i).
@@ -182,26 +197,26 @@ __device__ __forceinline__ bf16x8 bf16_ones() {
   return ones;
 }
 
-template <int D, int KW>
+template <int D>
 struct PrefixSmem {
-  static constexpr int KT = 64 * KW, P = D + 16;  // keys of a stage, elements between its rows
+  static constexpr int KT = kPrefixStage, P = D + 16;  // keys of a stage, elements between its rows
   static constexpr int kTiles = 2 * 2 * KT * P * 2;  // [buffer][K, V][key][P]
   static constexpr int kOwnPitch = D + 8;
   static constexpr int kOwnTiles = kPrefixWaves * 32 * kOwnPitch * 2;  // [wave][key][P] of V
-  static constexpr int kOwnMerge = kPrefixWaves * 16 * (D + 4 + 2) * 4;
-  static constexpr int kBytes = kTiles > kOwnTiles ? (kTiles > kOwnMerge ? kTiles : kOwnMerge)
-                                                   : (kOwnTiles > kOwnMerge ? kOwnTiles : kOwnMerge);
+  static constexpr int kBytes = kTiles > kOwnTiles ? kTiles : kOwnTiles;
 };
 
-// A prefix item: 8 / KW waves side by side over 16 rows each, KW one after the other over the keys, 64 keys each of a stage.
+// A prefix item: 8 / KW waves side by side over 16 rows each, KW one after the other over a stage's keys.
 template <int D, int MODE, int KW, int NPRE>
-__device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, float (*sscale)[2][64 * KW], int* bids) {
-  constexpr int KPW = 64, KT = KW * KPW, MT = KPW / 16, P = D + 16, KS = D / 32, DT = D / 16;
+__device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, float (*sscale)[2][kPrefixStage], int* bids, int index) {
+  const float scale_log2 = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, a.scale_log2)));
+  const bool k_f32 = a.ks_f32, v_f32 = a.vs_f32;
+  constexpr int KT = kPrefixStage, KPW = KT / KW, P = D + 16, KS = D / 32, DT = D / 16;
   constexpr int PT = kPrefixThreads, RW = kPrefixWaves / KW, ROWS = 16 * RW;
   constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, NCH = KT * CPK;  // 16-byte parts of a key, of a stage
   constexpr int LPT = (NCH + PT - 1) / PT, SPT = MODE == 0 ? 1 : (2 * KT + PT - 1) / PT;
   uint16_t(*sm)[2][KT * P] = (uint16_t(*)[2][KT * P]) smem;
-  const int item = blockIdx.x, tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+  const int item = index, tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
   const int4 i0 = *(const int4*)(a.items + 8 * (int64_t)item), i1 = *(const int4*)(a.items + 8 * (int64_t)item + 4);
   const int table_row = min(max(i0.x, 0), a.S - 1), first_member = max(i0.y, 0), M = max(i0.z, 1), m0 = max(i0.w, 0);
@@ -222,7 +237,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
       qop[j] = __builtin_bit_cast(
           bf16x8, *(const u32x4*)(a.q + (int64_t)s * a.q_ss + (int64_t)(h * G + at - i * G) * a.q_sh + 32 * j + 8 * q4));
   }
-  const float inv_scale_log2 = MODE == 0 ? 1.f / a.scale_log2 : 1.f;
+  const float inv_scale_log2 = MODE == 0 ? 1.f / scale_log2 : 1.f;
   RowState<D> st;
   st.clear();
   const int tr_off = tr16_offset(r, q4, P);
@@ -231,29 +246,32 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
 
   const int ntiles = (nkeys + KT - 1) / KT;
   u32x4 rk[NPRE][LPT], rv[NPRE][LPT];
-  uint32_t rs[NPRE][SPT];
+  u32x2 rs[NPRE][SPT];
   // A thread's parts of a stage keep their place in their blocks from stage to stage (a stage is whole blocks): what changes
   // is the block id. Keys past the item's end are read too, inside its last block; they are hidden, and their V is zero.
   const int es = MODE == 0 ? 2 : 1, last_id = (nkeys - 1) >> a.log_b;
   const uint32_t kv_bytes = (uint32_t)a.kv_sn * es;  // of a block (host-checked)
   const uint8_t* kbase[LPT];
-  const uint8_t* vbase[LPT];
+  const int64_t v_from_k = (const uint8_t*)a.v - (const uint8_t*)a.k;
   int part_id[LPT];
 #pragma unroll
   for (int i = 0; i < LPT; ++i) {
     const int c = tid + PT * i, key = c / CPK;
     const int64_t e = ((int64_t)h * a.kv_sh + (key & ((1 << a.log_b) - 1)) * D + CH * (c % CPK)) * es;
     kbase[i] = (const uint8_t*)a.k + e;
-    vbase[i] = (const uint8_t*)a.v + e;
     part_id[i] = key >> a.log_b;
   }
+  // The scales' thread-wise choice among copies: a choice among the arguments' addresses puts them into memory, whose own
+  // address comes from the launch's packet on the host, at 50 ns a workgroup (128 sequences of 500 tokens 25 -> 12 us).
+  const void *k_scales = a.ks, *v_scales = a.vs;
+  const int64_t ks_head = (int64_t)h * a.ks_sh, vs_head = (int64_t)h * a.vs_sh, ks_sn = a.ks_sn, vs_sn = a.vs_sn;
   auto gload = [&](int set, int t) {
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
       if (NCH % PT != 0 && tid + PT * i >= NCH) break;
       const uint64_t b = (uint64_t)(uint32_t)bids[min((KT * t >> a.log_b) + part_id[i], last_id)] * kv_bytes;
       rk[set][i] = *(const u32x4*)(kbase[i] + b);
-      rv[set][i] = *(const u32x4*)(vbase[i] + b);
+      rv[set][i] = *(const u32x4*)(kbase[i] + b + v_from_k);
     }
     if constexpr (MODE == 1) {
 #pragma unroll
@@ -262,8 +280,9 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
         if (2 * KT % PT != 0 && c >= 2 * KT) break;
         const int key = c % KT, off = key & ((1 << a.log_b) - 1);
         const int64_t blk = bids[min((KT * t >> a.log_b) + (key >> a.log_b), last_id)];
-        rs[set][i] = c < KT ? scale_bits(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + blk * a.ks_sn + off)
-                            : scale_bits(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + blk * a.vs_sn + off);
+        const bool of_k = c < KT;
+        rs[set][i] = load_scale(of_k ? k_scales : v_scales, of_k ? k_f32 : v_f32,
+                                (of_k ? ks_head : vs_head) + blk * (of_k ? ks_sn : vs_sn) + off);
       }
     }
   };
@@ -281,12 +300,17 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
         *(u32x4*)(&sm[buf][0][e]) = k;
         *(u32x4*)(&sm[buf][1][e]) = v;
       } else {
-        // Odd lanes store their second half first at head_dim 64, as 16 bytes of each 32 use half the banks.
+        // Odd lanes store their second half first at head_dim 64, as 16 bytes of each 32 use half the banks. The halves change
+        // places by their differing bits.
         const int odd = D == 64 ? tid & 1 : 0;
-        *(u32x4*)(&sm[buf][0][e + 8 * odd]) = tree_codes(odd ? k[2] : k[0], odd ? k[3] : k[1]);
-        *(u32x4*)(&sm[buf][0][e + 8 - 8 * odd]) = tree_codes(odd ? k[0] : k[2], odd ? k[1] : k[3]);
-        *(u32x4*)(&sm[buf][1][e + 8 * odd]) = tree_codes(odd ? v[2] : v[0], odd ? v[3] : v[1]);
-        *(u32x4*)(&sm[buf][1][e + 8 - 8 * odd]) = tree_codes(odd ? v[0] : v[2], odd ? v[1] : v[3]);
+        const uint32_t swap = -(uint32_t)odd;
+        auto store = [&](uint16_t* to, u32x4 x) {
+          const uint32_t d0 = (x[0] ^ x[2]) & swap, d1 = (x[1] ^ x[3]) & swap;
+          *(u32x4*)(to + 8 * odd) = tree_codes(x[0] ^ d0, x[1] ^ d1);
+          *(u32x4*)(to + 8 - 8 * odd) = tree_codes(x[2] ^ d0, x[3] ^ d1);
+        };
+        store(&sm[buf][0][e], k);
+        store(&sm[buf][1][e], v);
       }
     }
     if constexpr (MODE == 1) {
@@ -294,40 +318,45 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
       for (int i = 0; i < SPT; ++i) {
         const int c = tid + PT * i;
         if (2 * KT % PT != 0 && c >= 2 * KT) break;
-        sscale[buf][c / KT][c % KT] = c < KT ? scale_value(rs[set][i], a.ks_f32) * a.scale_log2 : scale_value(rs[set][i], a.vs_f32);
+        sscale[buf][c / KT][c % KT] = one_scale(rs[set][i], c < KT ? k_f32 : v_f32) * (c < KT ? scale_log2 : 1.f);
       }
     }
   };
+  // At head_dim 128 half of the wave's keys at a time: the scores of 64 would not fit the registers of two workgroups a CU.
+  constexpr int SUB = D == 64 ? KPW : 32, SMT = SUB / 16;
   auto tile = [&](int t) {
-    const int x0 = KT * t + KPW * kw;  // the wave's first key of the item
-    if (x0 >= nkeys || !valid) return;  // wave-uniform
     const int buf = t & 1;
-    const uint16_t* sk = sm[buf][0] + KPW * kw * P;
-    const uint16_t* sv = sm[buf][1] + KPW * kw * P;
-    f32x4 sc[MT], vs[MT];  // row (mt, q4, i) holds key 16 mt + 4 q4 + i
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int part = 0; part < KPW / SUB; ++part) {
+      const int first = KPW * kw + SUB * part, x0 = KT * t + first;  // the keys' place in the stage, in the item
+      if (x0 >= nkeys || !valid) return;  // wave-uniform
+      const uint16_t* sk = sm[buf][0] + first * P;
+      const uint16_t* sv = sm[buf][1] + first * P;
+      f32x4 sc[SMT], vs[SMT];  // row (mt, q4, i) holds key 16 mt + 4 q4 + i
 #pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const bf16x8 kop = *(const bf16x8*)(sk + (16 * mt + r) * P + 32 * j + 8 * q4);
-        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[j], sc[mt], 0, 0, 0);
+      for (int mt = 0; mt < SMT; ++mt) {
+        sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          const bf16x8 kop = *(const bf16x8*)(sk + (16 * mt + r) * P + 32 * j + 8 * q4);
+          sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[j], sc[mt], 0, 0, 0);
+        }
+        if constexpr (MODE == 1) {
+          sc[mt] *= *(const f32x4*)(sscale[buf][0] + first + 16 * mt + 4 * q4);  // log2 units
+          vs[mt] = *(const f32x4*)(sscale[buf][1] + first + 16 * mt + 4 * q4);
+        }
       }
-      if constexpr (MODE == 1) {
-        sc[mt] *= *(const f32x4*)(sscale[buf][0] + KPW * kw + 16 * mt + 4 * q4);  // log2 units
-        vs[mt] = *(const f32x4*)(sscale[buf][1] + KPW * kw + 16 * mt + 4 * q4);
+      if (x0 + SUB > nkeys) {
+#pragma unroll
+        for (int mt = 0; mt < SMT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (x0 + 16 * mt + 4 * q4 + i >= nkeys) sc[mt][i] = kNegInf;
       }
+      u32x4 hi[SUB / 32], lo[SUB / 32];
+      st.template add<MODE, SUB>(sc, scale_log2, inv_scale_log2, ones, vs, hi, lo);
+      st.template product<SUB>(sv, tr_off, P, hi, lo);
     }
-    if (x0 + KPW > nkeys) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (x0 + 16 * mt + 4 * q4 + i >= nkeys) sc[mt][i] = kNegInf;
-    }
-    u32x4 hi[KPW / 32], lo[KPW / 32];
-    st.template add<MODE, KPW>(sc, a.scale_log2, inv_scale_log2, ones, vs, hi, lo);
-    st.template product<KPW>(sv, tr_off, P, hi, lo);
   };
 #pragma unroll
   for (int k = 0; k < NPRE; ++k) {
@@ -353,7 +382,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
   if constexpr (KW > 1) {
     // The key waves' states join in LDS (the tile buffers are free after the last barrier).
     constexpr int XS = DT * 4 + 4;  // floats of a lane: O, m, l
-    static_assert((KW - 1) * RW * 64 * XS * 4 <= PrefixSmem<D, KW>::kTiles, "the states fit the tile buffers");
+    static_assert((KW - 1) * RW * 64 * XS * 4 <= PrefixSmem<D>::kTiles, "the states fit the tile buffers");
     float* xs = (float*)smem;
     if (kw > 0) {
       float* x = xs + (((kw - 1) * RW + rw) * 64 + lane) * XS;
@@ -378,215 +407,199 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
     }
   }
   if (kw > 0 || m >= M) return;
-  const int64_t slot = (int64_t)item * ROWS + 16 * rw + r;
+  const int64_t slot = (int64_t)min(max(i1.w, 0), a.num_items - 1) * ROWS + 16 * rw + r;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.p_o + slot * D + 16 * dt + 4 * q4) = st.acc[dt];
-  if (q4 == 0) a.p_m[slot] = st.m, a.p_l[slot] = l;
+  for (int dt = 0; dt < DT; ++dt) *(GlobalF32x4*)(a.st_o + slot * D + 16 * dt + 4 * q4) = st.acc[dt];
+  if (q4 == 0) *(GlobalU64*)(a.st_ml + slot) = __builtin_bit_cast(uint64_t, float2{st.m, l});
 }
 
-// An own item: each wave takes every eighth tile of 32 keys, K straight into the operand's registers, V through LDS of its own.
-template <int D, int MODE>
-__device__ __forceinline__ void own_item(const PrefixArgs& a, char* smem, int index) {
-  constexpr int KS = D / 32, DT = D / 16, P = D + 8, W = kPrefixWaves;
-  constexpr int VCH = MODE == 0 ? 8 : 16, VPK = D / VCH, VL = 32 * VPK / 64;  // 16-byte parts of V: a key's, a lane's
+// An own piece, a wave: 32 keys at a time in two halves, K straight into the operand's registers, V through LDS of the wave's own.
+// Registers hold NH halves: a half's are loaded again for a later one as soon as its K is in the scores and its V in LDS.
+template <int D, int MODE, int NH>
+__device__ __forceinline__ void own_piece(const PrefixArgs& a, char* smem, int index) {
+  const float scale_log2 = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, a.scale_log2)));
+  const bool k_f32 = a.ks_f32, v_f32 = a.vs_f32;
+  constexpr int KS = D / 32, DT = D / 16, P = D + 8;
+  constexpr int VCH = MODE == 0 ? 8 : 16, VPK = D / VCH, VL = (16 * VPK + 63) / 64;  // 16-byte parts of V: a key's, a lane's of a half
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int pairs = a.S * a.Hkv, sp = index / pairs, pair = index - sp * pairs, h = pair / a.S, s = pair - h * a.S;
-  const OwnKeys own = own_keys(a, s);
-  if (sp >= own.splits) return;
-  const int lo_key = own.shared + sp * own.chunk, end = min(lo_key + own.chunk, own.ctx), G = a.G;
-  const int32_t* table = a.bt + (int64_t)s * a.bt_ss;
-  const int last_col = min((end - 1) >> a.log_b, a.bt_w - 1);
+  const int piece = __builtin_amdgcn_readfirstlane(index * kPrefixWaves + wave);
+  if (piece >= a.num_pieces) return;
+  const int4 i0 = *(const int4*)(a.pieces + 8 * (int64_t)piece), i1 = *(const int4*)(a.pieces + 8 * (int64_t)piece + 4);
+  const int s = min(max(__builtin_amdgcn_readfirstlane(i0.x), 0), a.S - 1), h = min(max(__builtin_amdgcn_readfirstlane(i0.y), 0), a.Hkv - 1);
+  const int sp = max(__builtin_amdgcn_readfirstlane(i0.z), 0), planned = max(__builtin_amdgcn_readfirstlane(i0.w), 1);
+  const int tokens = max(__builtin_amdgcn_readfirstlane(i1.x), 0), G = a.G;
   bf16x8 qop[KS];
 #pragma unroll
   for (int j = 0; j < KS; ++j)
     qop[j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(a.q + (int64_t)s * a.q_ss + (int64_t)(h * G + min(r, G - 1)) * a.q_sh +
                                                         32 * j + 8 * q4));
-  const float inv_scale_log2 = MODE == 0 ? 1.f / a.scale_log2 : 1.f;
+  const OwnKeys own = own_keys(a, s, tokens, planned);
+  if (sp >= own.pieces) return;
+  const int lo_key = own.shared + sp * own.chunk, end = min(lo_key + own.chunk, own.ctx);
+  const int32_t* table = a.bt + (int64_t)s * a.bt_ss;
+  const int last_col = min((end - 1) >> a.log_b, a.bt_w - 1);
+  const float inv_scale_log2 = MODE == 0 ? 1.f / scale_log2 : 1.f;
   RowState<D> st;
   st.clear();
   uint16_t* sv = (uint16_t*)smem + wave * 32 * P;
   const int tr_off = tr16_offset(r, q4, P);
   const bf16x8 ones = bf16_ones();
-  const int ntiles = (end - lo_key + 31) / 32;
-  u32x4 rk[2][2][KS], rv[2][VL];
-  f32x4 rks[2][2], rvs[2][2];
-  // the ids of a tile's two halves of 16 keys, each inside one block; tiles past the end read the last block again
-  auto ids = [&](int t, int (&id)[2]) {
+  const int halves = 2 * ((end - lo_key + 31) / 32);
+  u32x4 rk[NH][KS], rv[NH][VL];
+  u32x4 rks[NH], rvs[NH];
+  // the id of the block that half i, 16 keys, is inside; halves past the end read the last block again
+  auto id_of = [&](int i) { return table[min((lo_key + 16 * i) >> a.log_b, last_col)]; };
+  const int k_off = r * D + 8 * q4;
+  auto load = [&](int set, int i, int entry) {
+    const int id = __builtin_amdgcn_readfirstlane(min(max(entry, 0), a.nb - 1));
+    const int off = (lo_key + 16 * i) & ((1 << a.log_b) - 1);
+    const int64_t base = (int64_t)h * a.kv_sh + (int64_t)id * a.kv_sn + off * D;
+    const uint8_t* k = (const uint8_t*)a.k + base * (MODE == 0 ? 2 : 1);
+    const uint8_t* v = (const uint8_t*)a.v + base * (MODE == 0 ? 2 : 1);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = min((lo_key + 32 * t + 16 * i) >> a.log_b, last_col);
-      id[i] = __builtin_amdgcn_readfirstlane(min(max(table[col], 0), a.nb - 1));
-    }
-  };
-  auto load = [&](int set, int t, const int (&id)[2]) {
-    const int inside = (1 << a.log_b) - 1;
-    int64_t base[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      base[i] = (int64_t)h * a.kv_sh + (int64_t)id[i] * a.kv_sn + ((lo_key + 32 * t + 16 * i) & inside) * D;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const int64_t e = base[mt] + r * D + 32 * j + 8 * q4;
-        if constexpr (MODE == 0) {
-          rk[set][mt][j] = *(const u32x4*)((const uint16_t*)a.k + e);
-        } else {
-          const u32x2 c = *(const u32x2*)((const uint8_t*)a.k + e);
-          rk[set][mt][j] = u32x4{c[0], c[1], 0, 0};
-        }
+    for (int j = 0; j < KS; ++j) {
+      if constexpr (MODE == 0) {
+        rk[set][j] = *(const u32x4*)(k + 2 * (k_off + 32 * j));
+      } else {
+        const u32x2 c = *(const u32x2*)(k + k_off + 32 * j);
+        rk[set][j] = u32x4{c[0], c[1], 0, 0};
       }
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int c = lane + 64 * i, key = c / VPK;
-      const int64_t e = (key < 16 ? base[0] : base[1]) + (key & 15) * D + VCH * (c % VPK);
-      rv[set][i] = *(const u32x4*)((const uint8_t*)a.v + e * (MODE == 0 ? 2 : 1));
     }
+#pragma unroll
+    for (int x = 0; x < VL; ++x)
+      if (16 * VPK % 64 == 0 || lane + 64 * x < 16 * VPK) rv[set][x] = *(const u32x4*)(v + 16 * (lane + 64 * x));
     if constexpr (MODE == 1) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int off = ((lo_key + 32 * t + 16 * mt) & inside) + 4 * q4;
-        rks[set][mt] = four_scales(a.ks, a.ks_f32, (int64_t)h * a.ks_sh + (int64_t)id[mt] * a.ks_sn + off);
-        rvs[set][mt] = four_scales(a.vs, a.vs_f32, (int64_t)h * a.vs_sh + (int64_t)id[mt] * a.vs_sn + off);
-      }
+      rks[set] = load_scales(a.ks, k_f32, (int64_t)h * a.ks_sh + (int64_t)id * a.ks_sn + off + 4 * q4);
+      rvs[set] = load_scales(a.vs, v_f32, (int64_t)h * a.vs_sh + (int64_t)id * a.vs_sn + off + 4 * q4);
     }
   };
-  auto tile = [&](int set, int t) {
-    const int x0 = lo_key + 32 * t;
-    if (t >= ntiles) return;
+  // Table entries are loaded a half ahead of the keys they are for, and before those of the half between: a wait for one is then
+  // no wait for keys that are still to come.
+  int first[NH + 1];
+#pragma unroll
+  for (int i = 0; i <= NH; ++i) first[i] = id_of(i);
+#pragma unroll
+  for (int i = 0; i < NH; ++i) load(i, i, first[i]);
+  int id = first[NH];
+  for (int i0 = 0; i0 < halves; i0 += 2) {
+    f32x4 sc[2], vs[2];
     wave_sync();  // the last tile's reads of V
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int c = lane + 64 * i, key = c / VPK;
-      u32x4 v = rv[set][i];
-      if (x0 + key >= end) v = u32x4{0, 0, 0, 0};
-      uint16_t* to = sv + key * P + VCH * (c % VPK);
-      if constexpr (MODE == 0) {
-        *(u32x4*)to = v;
-      } else {
-        *(u32x4*)to = tree_codes(v[0], v[1]);
-        *(u32x4*)(to + 8) = tree_codes(v[2], v[3]);
-      }
-    }
-    f32x4 sc[2], vs[2];
+    for (int half = 0; half < 2; ++half) {
+      const int set = half % NH, i = i0 + half, x0 = lo_key + 16 * i;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      sc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < VL; ++x) {
+        const int c = lane + 64 * x, key = c / VPK;
+        if (16 * VPK % 64 != 0 && c >= 16 * VPK) break;
+        u32x4 v = rv[set][x];
+        if (x0 + key >= end) v = u32x4{0, 0, 0, 0};
+        uint16_t* to = sv + (16 * half + key) * P + VCH * (c % VPK);
+        if constexpr (MODE == 0) {
+          *(u32x4*)to = v;
+        } else {
+          *(u32x4*)to = tree_codes(v[0], v[1]);
+          *(u32x4*)(to + 8) = tree_codes(v[2], v[3]);
+        }
+      }
+      sc[half] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        const u32x4 k = MODE == 0 ? rk[set][mt][j] : tree_codes(rk[set][mt][j][0], rk[set][mt][j][1]);
-        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), qop[j], sc[mt], 0, 0, 0);
+        const u32x4 k = MODE == 0 ? rk[set][j] : tree_codes(rk[set][j][0], rk[set][j][1]);
+        sc[half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), qop[j], sc[half], 0, 0, 0);
       }
       if constexpr (MODE == 1) {
-        sc[mt] *= rks[set][mt] * a.scale_log2;
-        vs[mt] = rvs[set][mt];
+        sc[half] *= four_scales(rks[set], k_f32) * scale_log2;
+        vs[half] = four_scales(rvs[set], v_f32);
+        asm volatile("" : "+v"(vs[half]));  // now: the registers are loaded again below
       }
-    }
-    if (x0 + 32 > end) {
+      if (x0 + 16 > end) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (x0 + 16 * mt + 4 * q4 + i >= end) sc[mt][i] = kNegInf;
+        for (int x = 0; x < 4; ++x)
+          if (x0 + 4 * q4 + x >= end) sc[half][x] = kNegInf;
+      }
+      const int next = id_of(i + NH + 1);
+      load(set, i + NH, id);
+      id = next;
     }
     u32x4 hi[1], lo[1];
-    st.template add<MODE, 32>(sc, a.scale_log2, inv_scale_log2, ones, vs, hi, lo);
+    st.template add<MODE, 32>(sc, scale_log2, inv_scale_log2, ones, vs, hi, lo);
     wave_sync();  // V has been stored
     st.template product<32>(sv, tr_off, P, hi, lo);
-  };
-  int id[2];
-  ids(wave, id);
-  load(0, wave, id);
-  ids(wave + W, id);
-  for (int t = wave; t < ntiles; t += 2 * W) {
-    load(1, t + W, id);
-    ids(t + 2 * W, id);
-    tile(0, t);
-    load(0, t + 2 * W, id);
-    ids(t + 3 * W, id);
-    tile(1, t + W);
   }
   float l = st.sum(MODE);
-  if (l != l) st.m = 0.f;
-  __syncthreads();  // every wave is done with its V
-  constexpr int MP = D + 4;
-  float2* ml = (float2*)smem;            // [wave][16] (m, l)
-  float* accs = (float*)(ml + W * 16);  // [wave][16][MP]
-  if (q4 == 0) ml[wave * 16 + r] = float2{st.m, l};
+  if (l != l) st.m = 0.f;  // NaN scores never raise the max: the merge sees the row by its sum
+  if (r >= G) return;
+  const int64_t slot = (int64_t)a.num_items * a.tile_rows + (int64_t)min(max(__builtin_amdgcn_readfirstlane(i1.y), 0), a.num_pieces - 1) * G + r;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) *(f32x4*)(accs + (wave * 16 + r) * MP + 16 * dt + 4 * q4) = st.acc[dt];
-  __syncthreads();
-  const int waves = min(ntiles, W);
-  const int64_t first = ((int64_t)pair * a.nsplit + sp) * G;
-  for (int i = tid; i < G * (D / 4); i += kPrefixThreads) {
-    const int g = i / (D / 4), c = i % (D / 4);
-    float M = kNegInf, L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < waves; ++w) M = fmaxf(M, ml[w * 16 + g].x);
-    for (int w = 0; w < waves; ++w) {
-      const float2 x = ml[w * 16 + g];
-      const float e = M == kNegInf ? 0.f : fast_exp2(x.x - M);
-      L += e * x.y;
-      O += e * *(const f32x4*)(accs + (w * 16 + g) * MP + 4 * c);
-    }
-    *(f32x4*)(a.s_o + (first + g) * D + 4 * c) = O;
-    if (c == 0) a.s_m[first + g] = M, a.s_l[first + g] = L;
-  }
+  for (int dt = 0; dt < DT; ++dt) *(GlobalF32x4*)(a.st_o + slot * D + 16 * dt + 4 * q4) = st.acc[dt];
+  if (q4 == 0) *(GlobalU64*)(a.st_ml + slot) = __builtin_bit_cast(uint64_t, float2{st.m, l});
 }
 
 template <int D, int MODE, int KW, int NPRE>
-__global__ void __launch_bounds__(kPrefixThreads, 2) prefix_attention_kernel(const PrefixArgs a) {
-  __shared__ __align__(16) char smem[PrefixSmem<D, KW>::kBytes];
-  __shared__ __align__(16) float sscale[MODE == 0 ? 1 : 2][2][64 * KW];
+__global__ void __launch_bounds__(kPrefixThreads, 4) prefix_attention_kernel(const PrefixArgs a) {
+  __shared__ __align__(16) char smem[PrefixSmem<D>::kBytes];
+  __shared__ __align__(16) float sscale[MODE == 0 ? 1 : 2][2][kPrefixStage];
   __shared__ int bids[kPrefixMaxChunk / 16];
-  if ((int)blockIdx.x < a.num_items) prefix_item<D, MODE, KW, NPRE>(a, smem, sscale, bids);
-  else own_item<D, MODE>(a, smem, (int)blockIdx.x - a.num_items);
+  if ((int)blockIdx.x < a.num_items) prefix_item<D, MODE, KW, NPRE>(a, smem, sscale, bids, blockIdx.x);
+  else own_piece<D, MODE, D == 64 ? 2 : 1>(a, smem, (int)blockIdx.x - a.num_items);
 }
 
-// Thread (row, 4 channels): joins the row's parts. A row without any key gets zeros.
+// Joins the parts of a row, a wave: lane (part, 4 channels), 256 / D parts side by side. A row without any key gets zeros.
 template <int D>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
-  constexpr int Q = D / 4, U = 8;
-  const int at = blockIdx.x * 256 + threadIdx.x, row = at / Q, c = at % Q, Hq = a.Hkv * a.G;
+  constexpr int Q = D / 4, ROWS = 64 / Q, U = 8;  // parts side by side, of which a lane takes U at a time
+  const int lane = threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), Hq = a.Hkv * a.G;
   if (row >= a.S * Hq) return;
-  const int s = row / Hq, hq = row - s * Hq, h = hq / a.G, g = hq - h * a.G;
-  const OwnKeys own = own_keys(a, s);
-  const int32_t* info = a.rows + 8 * (int64_t)s;
-  const int np = own.shared > 0 ? info[3] : 0, m = info[1] + g, tile = m / a.tile_rows;
-  const int64_t p0 = ((int64_t)info[2] + (int64_t)(h * info[4] + tile) * np) * a.tile_rows + (m - tile * a.tile_rows);
-  const int64_t s0 = (int64_t)(h * a.S + s) * a.nsplit * a.G + g;
-  const int n = np + own.splits;
-  auto part = [&](int j) { return j < np ? p0 + (int64_t)j * a.tile_rows : s0 + (int64_t)(j - np) * a.G; };
+  const int s = row / Hq, hq = row - s * Hq, h = hq / a.G, g = hq - h * a.G, c = lane % Q, side = lane / Q;
+  const int4 i0 = *(const int4*)(a.rows + 8 * (int64_t)s), i1 = *(const int4*)(a.rows + 8 * (int64_t)s + 4);
+  const OwnKeys own = own_keys(a, s, i0.x, max(i1.z, 1));
+  const int np = own.shared > 0 ? i0.w : 0, m = i0.y + g, tile = m / a.tile_rows, n = np + own.pieces;
+  const int64_t p0 = ((int64_t)i0.z + (int64_t)(h * i1.x + tile) * np) * a.tile_rows + (m - tile * a.tile_rows);
+  const int64_t s0 = (int64_t)a.num_items * a.tile_rows + ((int64_t)i1.y + (int64_t)h * i1.z) * a.G + g;
   float M = kNegInf, L = 0.f;
   f32x4 O = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < n; j0 += U) {
+  for (int j0 = side; j0 < n; j0 += ROWS * U) {
     float ms[U], ls[U];
     f32x4 os[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = min(j0 + u, n - 1);
-      const int64_t i = part(j);
-      ms[u] = (j < np ? a.p_m : a.s_m)[i];
-      ls[u] = (j < np ? a.p_l : a.s_l)[i];
-      os[u] = *(const f32x4*)((j < np ? a.p_o : a.s_o) + i * D + 4 * c);
+      const int j = min(j0 + ROWS * u, n - 1);
+      const int64_t i = j < np ? p0 + (int64_t)j * a.tile_rows : s0 + (int64_t)(j - np) * a.G;
+      const float2 ml = a.st_ml[i];
+      ms[u] = ml.x, ls[u] = ml.y;
+      os[u] = *(const f32x4*)(a.st_o + i * D + 4 * c);
     }
     float top = M;
 #pragma unroll
-    for (int u = 0; u < U; ++u) top = fmaxf(top, j0 + u < n ? ms[u] : kNegInf);
+    for (int u = 0; u < U; ++u) top = fmaxf(top, j0 + ROWS * u < n ? ms[u] : kNegInf);
     if (top == kNegInf) continue;
     const float f = fast_exp2(M - top);
     L *= f;
     O *= f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (j0 + u >= n || ms[u] == kNegInf) continue;  // a part without a key for the row
+      if (j0 + ROWS * u >= n || ms[u] == kNegInf) continue;  // a part without a key for the row
       const float e = fast_exp2(ms[u] - top);
       L += e * ls[u];
       O += e * os[u];
     }
     M = top;
   }
+  auto join = [&](int o) {
+    const float m1 = __shfl_xor(M, o), l1 = __shfl_xor(L, o), top = fmaxf(M, m1);
+    f32x4 o1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o1[i] = __shfl_xor(O[i], o);
+    // (an empty side's O is 0, but its factor would be NaN)
+    const float f0 = M == kNegInf ? 0.f : fast_exp2(M - top), f1 = m1 == kNegInf ? 0.f : fast_exp2(m1 - top);
+    L = f0 * L + f1 * l1;
+    O = f0 * O + f1 * o1;
+    M = top;
+  };
+#pragma unroll
+  for (int o = Q; o < 64; o *= 2) join(o);
+  if (side > 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   *(u32x2*)(a.out + (int64_t)s * a.o_ss + (int64_t)hq * a.o_sh + 4 * c) =
       u32x2{pack_bf16x2(O[0] * inv, O[1] * inv), pack_bf16x2(O[2] * inv, O[3] * inv)};
@@ -596,6 +609,13 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
 
 using namespace sipa;
 
+#ifndef PREFIX_MIN
+#define PREFIX_MIN 128
+#define PREFIX_WGS 2
+#define OWN_MIN 64
+#define OWN_MAX 512
+#define OWN_WGS 2
+#endif
 static int prefix_check(const sipa_prefix_params* p) {
   SIPA_CHECK(p != nullptr && p->struct_size == (int32_t)sizeof(sipa_prefix_params), SIPA_EINVAL,
              "struct_size does not match this library's sipa_prefix_params (%d bytes)", (int)sizeof(sipa_prefix_params));
@@ -613,22 +633,15 @@ static int prefix_check(const sipa_prefix_params* p) {
   return SIPA_OK;
 }
 
-struct PrefixLayout {
-  int64_t p_m, p_l, p_o, s_m, s_l, s_o, total;
+struct PrefixStates {
+  int64_t ml, total;  // byte offsets into the workspace
 };
 
-static PrefixLayout prefix_workspace(const sipa_prefix_params* p, const sipa_prefix_layout& l) {
+static PrefixStates prefix_workspace(const sipa_prefix_params* p, const sipa_prefix_layout& l) {
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  const int64_t pr = (int64_t)l.num_items * l.tile_rows, sr = (int64_t)p->num_seqs * p->num_q_heads * l.own_splits;
-  PrefixLayout w;
-  w.p_m = 0;
-  w.p_l = w.p_m + up(pr * 4);
-  w.p_o = w.p_l + up(pr * 4);
-  w.s_m = w.p_o + up(pr * p->head_dim * 4);
-  w.s_l = w.s_m + up(sr * 4);
-  w.s_o = w.s_l + up(sr * 4);
-  w.total = w.s_o + up(sr * p->head_dim * 4);
-  return w;
+  const int64_t n = (int64_t)l.num_items * l.tile_rows + (int64_t)l.num_pieces * (p->num_q_heads / p->num_kv_heads);
+  const int64_t ml = up(n * p->head_dim * 4);
+  return PrefixStates{ml, ml + up(n * 8)};
 }
 
 extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_groups, const int32_t* group_starts,
@@ -640,82 +653,108 @@ extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_gro
              "NULL pointer or negative group count");
   const int S = p->num_seqs, G = p->num_q_heads / p->num_kv_heads, H = p->num_kv_heads;
   SIPA_CHECK(num_groups == 0 || group_starts[0] == 0, SIPA_EINVAL, "group_starts begin at %d", num_groups ? group_starts[0] : 0);
+  const int num_members = num_groups ? group_starts[num_groups] : 0;
   // groups that share anything: two members at least, one block
   auto count_of = [&](int g) { return group_starts[g + 1] - group_starts[g]; };
   auto shares = [&](int g) { return count_of(g) >= 2 && tokens[g] > 0; };
-  int64_t most_rows = 0, shared_min = p->max_context;
-  int64_t grouped = 0;
+  auto length = [&](int s) { return context_lens == nullptr ? p->max_context : std::min(std::max(context_lens[s], 0), p->max_context); };
+  int64_t most_rows = 0, own = 0;  // own: keys that are read for one sequence
+  for (int s = 0; s < S; ++s) own += length(s);
   for (int g = 0; g < num_groups; ++g) {
     SIPA_CHECK(count_of(g) >= 0 && group_starts[g + 1] <= S, SIPA_EINVAL, "group %d has rows %d .. %d of %d", g, group_starts[g],
                group_starts[g + 1], S);
     SIPA_CHECK(tokens[g] >= 0 && tokens[g] <= p->max_context && tokens[g] % p->block_size == 0, SIPA_EINVAL,
                "group %d shares %d tokens: whole blocks of %d within max_context %d", g, tokens[g], p->block_size, p->max_context);
-    if (!shares(g)) continue;
-    most_rows = std::max<int64_t>(most_rows, (int64_t)count_of(g) * G);
-    shared_min = std::min<int64_t>(shared_min, tokens[g]);
-    grouped += count_of(g);
+    for (int i = group_starts[g]; i < group_starts[g + 1]; ++i) {
+      SIPA_CHECK(members[i] >= 0 && members[i] < S, SIPA_EINVAL, "group %d has row %d of %d", g, members[i], S);
+      if (shares(g) && length(members[i]) >= tokens[g]) own -= tokens[g];
+    }
+    if (shares(g)) most_rows = std::max<int64_t>(most_rows, (int64_t)count_of(g) * G);
   }
-  const int num_members = num_groups ? group_starts[num_groups] : 0;
   const int cus = sipa_device_cu_count(-1);
   if (cus < 0) return cus;
   sipa_prefix_layout l = {};
   l.tile_rows = most_rows <= 64 ? 64 : 128;
-  const int kt = l.tile_rows == 64 ? 128 : 64;
+  const int kt = kPrefixStage;
   auto tiles_of = [&](int g) { return ((int64_t)count_of(g) * G + l.tile_rows - 1) / l.tile_rows; };
   int64_t work = 0;  // keys times row tiles
   for (int g = 0; g < num_groups; ++g)
     if (shares(g)) work += (int64_t)H * tiles_of(g) * tokens[g];
-  const int64_t share = std::max<int64_t>(256, (work + cus - 1) / cus);
-  auto splits_of = [&](int g) {
+  const int64_t share = std::max<int64_t>(PREFIX_MIN, (work + PREFIX_WGS * cus - 1) / (PREFIX_WGS * cus));
+  struct Cut {
+    int64_t n, chunk;
+  };
+  auto cut_of = [&](int g) {
     const int64_t n = std::max<int64_t>((tokens[g] + share - 1) / share, (tokens[g] + kPrefixMaxChunk - 1) / kPrefixMaxChunk);
     const int64_t chunk = ((tokens[g] + n - 1) / n + kt - 1) / kt * kt;
-    return std::pair<int64_t, int64_t>((tokens[g] + chunk - 1) / chunk, chunk);
+    return Cut{(tokens[g] + chunk - 1) / chunk, chunk};
   };
   int64_t items = 0;
   for (int g = 0; g < num_groups; ++g)
-    if (shares(g)) items += H * tiles_of(g) * splits_of(g).first;
-  // the sequences' own keys
-  int64_t longest = grouped == S && S > 0 ? p->max_context - shared_min : p->max_context;
-  const int64_t pairs = (int64_t)S * H;
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((longest + 255) / 256, 2 * cus / std::max<int64_t>(pairs, 1)));
-  l.own_chunk = (int)(((longest + n - 1) / n + 63) / 64 * 64);
-  l.own_chunk = std::max(l.own_chunk, 64);
-  l.own_splits = (int)std::max<int64_t>(1, (longest + l.own_chunk - 1) / l.own_chunk);
-  SIPA_CHECK(items + pairs * l.own_splits <= 0x7fffffff && items * l.tile_rows <= 0x7fffffff, SIPA_EUNSUPPORTED,
-             "%lld items exceed the grid limit", (long long)(items + pairs * l.own_splits));
+    if (shares(g)) items += H * tiles_of(g) * cut_of(g).n;
+  const int64_t piece = std::min<int64_t>(std::max<int64_t>((own * H + 8 * OWN_WGS * cus - 1) / (8 * OWN_WGS * cus), OWN_MIN), OWN_MAX);
+  auto pieces_of = [&](int s, int shared) {  // for a KV head; one at least, for lengths that come to be another
+    const int n = length(s) >= shared ? length(s) - shared : length(s);
+    return std::max<int64_t>(1, (n + piece - 1) / piece);
+  };
+  // The rows, in the plan's place or counted alone.
+  int64_t pieces = 0;
+  for (int s = 0; s < S; ++s) pieces += H * pieces_of(s, 0);
+  for (int g = 0; g < num_groups; ++g)
+    if (shares(g))
+      for (int i = group_starts[g]; i < group_starts[g + 1]; ++i) pieces += H * (pieces_of(members[i], tokens[g]) - pieces_of(members[i], 0));
+  SIPA_CHECK(pieces >= 0 && items + pieces <= 0x7fffffff / 128, SIPA_EUNSUPPORTED, "%lld items exceed the grid limit",
+             (long long)(items + pieces));
   l.num_items = (int)items;
+  l.num_pieces = (int)pieces;
   l.num_members = num_members;
-  l.plan_ints = 8 * items + 8 * (int64_t)S + num_members;
+  l.plan_ints = 8 * (items + pieces + S) + num_members;
   l.workspace_bytes = prefix_workspace(p, l).total;
   *layout = l;
   if (plan == nullptr) return SIPA_OK;
   SIPA_CHECK(capacity >= l.plan_ints, SIPA_EINVAL, "the plan takes %lld values, room for %lld", (long long)l.plan_ints,
              (long long)capacity);
-  int32_t* rows = plan + 8 * items;
+  int32_t* pcs = plan + 8 * items;
+  int32_t* rows = pcs + 8 * pieces;
   for (int64_t i = 0; i < 8 * (int64_t)S; ++i) rows[i] = i % 8 == 7 ? -1 : 0;
   int64_t at = 0;
   for (int g = 0; g < num_groups; ++g) {
     const int a0 = group_starts[g], count = count_of(g);
     for (int i = 0; i < count; ++i) {
-      const int s = members[a0 + i];
-      SIPA_CHECK(s >= 0 && s < S, SIPA_EINVAL, "group %d has row %d of %d", g, s, S);
-      SIPA_CHECK(rows[8 * (int64_t)s + 7] < 0, SIPA_EINVAL, "row %d in two groups, or twice in one", s);
-      rows[8 * (int64_t)s + 7] = g;
+      int32_t* r = rows + 8 * (int64_t)members[a0 + i];
+      SIPA_CHECK(r[7] < 0, SIPA_EINVAL, "row %d in two groups, or twice in one", members[a0 + i]);
+      r[7] = g;
     }
     if (!shares(g)) continue;
     const int64_t tiles = tiles_of(g);
-    const auto [np, chunk] = splits_of(g);
+    const Cut cut = cut_of(g);
     for (int i = 0; i < count; ++i) {
       int32_t* r = rows + 8 * (int64_t)members[a0 + i];
-      r[0] = tokens[g], r[1] = i * G, r[2] = (int)at, r[3] = (int)np, r[4] = (int)tiles;
+      r[0] = tokens[g], r[1] = i * G, r[2] = (int)at, r[3] = (int)cut.n, r[4] = (int)tiles;
     }
-    for (int h = 0; h < H; ++h)
+    // State (h, tile, split). Workgroup L is dealt to XCD L % 8: the row tiles of the same keys come eight apart.
+    const int64_t units = H * cut.n;
+    for (int64_t u0 = 0, put = at; u0 < units; u0 += 8)
       for (int64_t t = 0; t < tiles; ++t)
-        for (int64_t x = 0; x < np; ++x) {
-          int32_t* it = plan + 8 * at++;
+        for (int64_t u = u0; u < std::min<int64_t>(u0 + 8, units); ++u) {
+          const int64_t h = u / cut.n, x = u - h * cut.n;
+          int32_t* it = plan + 8 * put++;
           it[0] = members[a0], it[1] = a0, it[2] = count * G, it[3] = (int)(t * l.tile_rows);
-          it[4] = h, it[5] = (int)(x * chunk), it[6] = (int)std::min<int64_t>((x + 1) * chunk, tokens[g]), it[7] = 0;
+          it[4] = (int)h, it[5] = (int)(x * cut.chunk), it[6] = (int)std::min<int64_t>((x + 1) * cut.chunk, tokens[g]);
+          it[7] = (int)(at + (h * tiles + t) * cut.n + x);
         }
+    at += units * tiles;
+  }
+  int64_t put = 0;
+  for (int s = 0; s < S; ++s) {
+    int32_t* r = rows + 8 * (int64_t)s;
+    const int64_t n = pieces_of(s, r[0]);
+    r[5] = (int)put, r[6] = (int)n;
+    for (int h = 0; h < H; ++h)
+      for (int64_t x = 0; x < n; ++x, ++put) {
+        int32_t* q = pcs + 8 * put;
+        q[0] = s, q[1] = h, q[2] = (int)x, q[3] = (int)n, q[4] = r[0], q[5] = (int)put, q[6] = q[7] = 0;
+      }
   }
   for (int i = 0; i < num_members; ++i) rows[8 * (int64_t)S + i] = members[i];
   return SIPA_OK;
@@ -723,11 +762,10 @@ extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_gro
 
 template <int D, int MODE>
 static void launch_prefix(int tile_rows, dim3 grid, hipStream_t st, const PrefixArgs& a) {
-  constexpr int NPRE = D == 64 ? 4 : 3;
+  constexpr int NPRE = D == 64 ? 3 : 2;
   if (tile_rows == 64) hipLaunchKernelGGL((prefix_attention_kernel<D, MODE, 2, NPRE>), grid, dim3(kPrefixThreads), 0, st, a);
   else hipLaunchKernelGGL((prefix_attention_kernel<D, MODE, 1, NPRE>), grid, dim3(kPrefixThreads), 0, st, a);
-  const int threads = a.S * a.Hkv * a.G * (D / 4);
-  hipLaunchKernelGGL((prefix_merge_kernel<D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((prefix_merge_kernel<D>), dim3((unsigned)((a.S * a.Hkv * a.G + 3) / 4)), dim3(256), 0, st, a);
 }
 
 extern "C" int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stream) {
@@ -760,11 +798,10 @@ extern "C" int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stre
                "scales must be aligned to their element size");
   }
   const sipa_prefix_layout& l = p->layout;
-  SIPA_CHECK((l.tile_rows == 64 || l.tile_rows == 128) && l.num_items >= 0 && l.num_members >= 0 && l.own_splits >= 1 &&
-                 l.own_chunk >= 64 && l.own_chunk % 64 == 0 && ((uintptr_t)p->plan & 15) == 0 &&
-                 (int64_t)p->num_seqs * p->num_kv_heads * l.own_splits + l.num_items <= 0x7fffffff,
-             SIPA_EINVAL, "the layout is not one of sipa_prefix_plan");
-  const PrefixLayout w = prefix_workspace(p, l);
+  SIPA_CHECK((l.tile_rows == 64 || l.tile_rows == 128) && l.num_items >= 0 && l.num_members >= 0 &&
+                 l.num_pieces >= (int64_t)p->num_seqs * p->num_kv_heads && (int64_t)l.num_items + l.num_pieces <= 0x7fffffff / 128 &&
+                 ((uintptr_t)p->plan & 15) == 0, SIPA_EINVAL, "the layout is not one of sipa_prefix_plan for these sizes");
+  const PrefixStates w = prefix_workspace(p, l);
   SIPA_CHECK(p->workspace != nullptr && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= w.total, SIPA_EWORKSPACE,
              "a 256-byte aligned workspace of %lld bytes is needed (have %lld)", (long long)w.total, (long long)p->workspace_bytes);
   PrefixArgs a;
@@ -791,9 +828,11 @@ extern "C" int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stre
   a.vs_sh = p->vs_stride_h;
   a.vs_sn = p->vs_stride_n;
   a.items = p->plan;
-  a.rows = p->plan + 8 * (int64_t)l.num_items;
+  a.pieces = p->plan + 8 * (int64_t)l.num_items;
+  a.rows = a.pieces + 8 * (int64_t)l.num_pieces;
   a.members = a.rows + 8 * (int64_t)p->num_seqs;
   a.num_items = l.num_items;
+  a.num_pieces = l.num_pieces;
   a.num_members = l.num_members;
   a.S = p->num_seqs;
   a.Hkv = p->num_kv_heads;
@@ -801,18 +840,11 @@ extern "C" int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stre
   a.nb = p->num_blocks;
   a.max_ctx = p->max_context;
   a.log_b = p->block_size == 16 ? 4 : p->block_size == 32 ? 5 : 6;
-  a.nsplit = l.own_splits;
-  a.chunk = l.own_chunk;
   a.tile_rows = l.tile_rows;
   a.scale_log2 = p->scale * 1.4426950408889634f;
-  char* ws = (char*)p->workspace;
-  a.p_m = (float*)(ws + w.p_m);
-  a.p_l = (float*)(ws + w.p_l);
-  a.p_o = (float*)(ws + w.p_o);
-  a.s_m = (float*)(ws + w.s_m);
-  a.s_l = (float*)(ws + w.s_l);
-  a.s_o = (float*)(ws + w.s_o);
-  const dim3 grid((unsigned)(l.num_items + (int64_t)p->num_seqs * p->num_kv_heads * l.own_splits));
+  a.st_o = (float*)p->workspace;
+  a.st_ml = (float2*)((char*)p->workspace + w.ml);
+  const dim3 grid((unsigned)(l.num_items + (l.num_pieces + kPrefixWaves - 1) / kPrefixWaves));
   hipStream_t st = (hipStream_t)stream;
   if (p->head_dim == 64) {
     if (int8) launch_prefix<64, 1>(l.tile_rows, grid, st, a);

@@ -163,7 +163,7 @@ class LogitsParams(ctypes.Structure):
 class PrefixLayout(ctypes.Structure):
     """Mirror of struct sipa_prefix_layout."""
     _fields_ = [
-        ("num_items", i32), ("num_members", i32), ("tile_rows", i32), ("own_splits", i32), ("own_chunk", i32),
+        ("num_items", i32), ("num_pieces", i32), ("num_members", i32), ("tile_rows", i32), ("reserved", i32),
         ("plan_ints", i64), ("workspace_bytes", i64),
     ]
 

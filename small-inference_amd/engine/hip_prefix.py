@@ -73,8 +73,8 @@ class PrefixPlan:
     included; a sequence of none gets zeros); max_context, known on the host, bounds them. groups [(rows, tokens)]: rows of the
     batch whose tables agree in their first tokens / B entries, tokens whole blocks; a row is in one group at most. Groups
     change the time, not the result: every row attends the positions below its context length, and one whose context is
-    shorter than its group's tokens is read by itself. host_context_lens: the lengths as a list, where the caller has
-    them, for a better division of the work.
+    shorter than its group's tokens is read by itself. host_context_lens: the lengths as a list, by which the work is
+    divided; None: they are read from the device once, which waits for it (in a capture max_context is taken for each).
 
     The workspace is made for the call that needs it, so plans, streams and graphs share none. Threads may call one plan at
     the same time: each call fills the parameter block and launches under the plan's lock."""
@@ -100,6 +100,8 @@ class PrefixPlan:
         if host_context_lens is not None and (len(host_context_lens) != S or max(host_context_lens, default=0) > max_context):
             raise ValueError("host_context_lens must hold S lengths, none above max_context")
         _hip.require_gpu(q, k_cache, v_cache, block_tables, context_lens)
+        if host_context_lens is None and not torch.cuda.is_current_stream_capturing():
+            host_context_lens = context_lens.tolist()
         self.shape, self.pool_shape, self.device = (S, Hq, D), tuple(k_cache.shape), q.device
         self.pool_dtype = torch.bfloat16 if quant is None else torch.int8
         self._pool_strides = (N * B * D, B * D, D, 1)  # of a contiguous layer
