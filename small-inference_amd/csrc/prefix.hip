@@ -191,9 +191,10 @@ struct RowState {
   }
 };
 
+template <int D>
 __device__ __forceinline__ bf16x8 bf16_ones() {
   bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
-  asm volatile("" : "+v"(ones));  // kept in registers
+  if constexpr (D == 64) asm volatile("" : "+v"(ones));  // kept in registers, where there is room
   return ones;
 }
 
@@ -214,7 +215,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
   constexpr int KT = kPrefixStage, KPW = KT / KW, P = D + 16, KS = D / 32, DT = D / 16;
   constexpr int PT = kPrefixThreads, RW = kPrefixWaves / KW, ROWS = 16 * RW;
   constexpr int CH = MODE == 0 ? 8 : 16, CPK = D / CH, NCH = KT * CPK;  // 16-byte parts of a key, of a stage
-  constexpr int LPT = (NCH + PT - 1) / PT, SPT = MODE == 0 ? 1 : (2 * KT + PT - 1) / PT;
+  constexpr int LPT = (NCH + PT - 1) / PT;
   uint16_t(*sm)[2][KT * P] = (uint16_t(*)[2][KT * P]) smem;
   const int item = index, tid = threadIdx.x, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
@@ -241,12 +242,12 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
   RowState<D> st;
   st.clear();
   const int tr_off = tr16_offset(r, q4, P);
-  const bf16x8 ones = bf16_ones();
+  const bf16x8 ones = bf16_ones<D>();
   __syncthreads();  // block ids
 
   const int ntiles = (nkeys + KT - 1) / KT;
   u32x4 rk[NPRE][LPT], rv[NPRE][LPT];
-  u32x2 rs[NPRE][SPT];
+  u32x2 rs[NPRE];
   // A thread's parts of a stage keep their place in their blocks from stage to stage (a stage is whole blocks): what changes
   // is the block id. Keys past the item's end are read too, inside its last block; they are hidden, and their V is zero.
   const int es = MODE == 0 ? 2 : 1, last_id = (nkeys - 1) >> a.log_b;
@@ -261,10 +262,15 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
     kbase[i] = (const uint8_t*)a.k + e;
     part_id[i] = key >> a.log_b;
   }
-  // The scales' thread-wise choice among copies: a choice among the arguments' addresses puts them into memory, whose own
-  // address comes from the launch's packet on the host, at 50 ns a workgroup (128 sequences of 500 tokens 25 -> 12 us).
+  // Threads 0 .. KT - 1 bring a stage's scales of K, the next KT those of V. (Chosen among copies: a choice among the arguments'
+  // addresses puts them into memory, whose own address comes from the launch's packet on the host, at 50 ns a workgroup: 128
+  // sequences of 500 tokens 25 -> 12 us.)
   const void *k_scales = a.ks, *v_scales = a.vs;
   const int64_t ks_head = (int64_t)h * a.ks_sh, vs_head = (int64_t)h * a.vs_sh, ks_sn = a.ks_sn, vs_sn = a.vs_sn;
+  const bool of_k = tid < KT, scale_f32 = of_k ? k_f32 : v_f32;
+  const void* scales = (const char*)(of_k ? k_scales : v_scales) +
+                       ((of_k ? ks_head : vs_head) + (tid & ((1 << a.log_b) - 1))) * (scale_f32 ? 4 : 2);
+  const int64_t scale_block = of_k ? ks_sn : vs_sn;
   auto gload = [&](int set, int t) {
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
@@ -274,16 +280,8 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
       rv[set][i] = *(const u32x4*)(kbase[i] + b + v_from_k);
     }
     if constexpr (MODE == 1) {
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) {
-        const int c = tid + PT * i;
-        if (2 * KT % PT != 0 && c >= 2 * KT) break;
-        const int key = c % KT, off = key & ((1 << a.log_b) - 1);
-        const int64_t blk = bids[min((KT * t >> a.log_b) + (key >> a.log_b), last_id)];
-        const bool of_k = c < KT;
-        rs[set][i] = load_scale(of_k ? k_scales : v_scales, of_k ? k_f32 : v_f32,
-                                (of_k ? ks_head : vs_head) + blk * (of_k ? ks_sn : vs_sn) + off);
-      }
+      if (tid < 2 * KT)
+        rs[set] = load_scale(scales, scale_f32, bids[min((KT * t >> a.log_b) + (tid % KT >> a.log_b), last_id)] * scale_block);
     }
   };
   auto sstore = [&](int set, int t) {
@@ -314,12 +312,7 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* smem, flo
       }
     }
     if constexpr (MODE == 1) {
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) {
-        const int c = tid + PT * i;
-        if (2 * KT % PT != 0 && c >= 2 * KT) break;
-        sscale[buf][c / KT][c % KT] = one_scale(rs[set][i], c < KT ? k_f32 : v_f32) * (c < KT ? scale_log2 : 1.f);
-      }
+      if (tid < 2 * KT) sscale[buf][tid / KT][tid % KT] = one_scale(rs[set], scale_f32) * (of_k ? scale_log2 : 1.f);
     }
   };
   // At head_dim 128 half of the wave's keys at a time: the scores of 64 would not fit the registers of two workgroups a CU.
@@ -444,7 +437,7 @@ __device__ __forceinline__ void own_piece(const PrefixArgs& a, char* smem, int i
   st.clear();
   uint16_t* sv = (uint16_t*)smem + wave * 32 * P;
   const int tr_off = tr16_offset(r, q4, P);
-  const bf16x8 ones = bf16_ones();
+  const bf16x8 ones = bf16_ones<D>();
   const int halves = 2 * ((end - lo_key + 31) / 32);
   u32x4 rk[NH][KS], rv[NH][VL];
   u32x4 rks[NH], rvs[NH];
@@ -609,13 +602,6 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
 
 using namespace sipa;
 
-#ifndef PREFIX_MIN
-#define PREFIX_MIN 128
-#define PREFIX_WGS 2
-#define OWN_MIN 64
-#define OWN_MAX 512
-#define OWN_WGS 2
-#endif
 static int prefix_check(const sipa_prefix_params* p) {
   SIPA_CHECK(p != nullptr && p->struct_size == (int32_t)sizeof(sipa_prefix_params), SIPA_EINVAL,
              "struct_size does not match this library's sipa_prefix_params (%d bytes)", (int)sizeof(sipa_prefix_params));
@@ -680,7 +666,14 @@ extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_gro
   int64_t work = 0;  // keys times row tiles
   for (int g = 0; g < num_groups; ++g)
     if (shares(g)) work += (int64_t)H * tiles_of(g) * tokens[g];
-  const int64_t share = std::max<int64_t>(PREFIX_MIN, (work + PREFIX_WGS * cus - 1) / (PREFIX_WGS * cus));
+  // Two workgroups a CU are resident: the own pieces take as many as they need with 64 keys a piece, or 128 .. 512 where those
+  // would not all be resident, and the items share the rest, half of a CU's at least, with 128 keys each at least. (64 beams of
+  // 4096 + 300 tokens: 512 items beside 75 workgroups of pieces 19.0 us, 352 14.5; two documents of 30016 tokens, 37 sequences
+  // each: 256 items 45.8, 480 33. Pieces of 64 / 128 keys: 128 sequences of 100 tokens 17.2 / 21.1, 200 of 1000 44 / 40.)
+  int64_t piece = 64;
+  while (piece < 512 && own * H > piece * 8 * 2 * cus) piece *= 2;
+  const int64_t free = std::max<int64_t>(2 * cus - (own * H / piece + S * H) / 8, cus / 2);
+  const int64_t share = std::max<int64_t>(128, (work + free - 1) / free);
   struct Cut {
     int64_t n, chunk;
   };
@@ -692,7 +685,6 @@ extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_gro
   int64_t items = 0;
   for (int g = 0; g < num_groups; ++g)
     if (shares(g)) items += H * tiles_of(g) * cut_of(g).n;
-  const int64_t piece = std::min<int64_t>(std::max<int64_t>((own * H + 8 * OWN_WGS * cus - 1) / (8 * OWN_WGS * cus), OWN_MIN), OWN_MAX);
   auto pieces_of = [&](int s, int shared) {  // for a KV head; one at least, for lengths that come to be another
     const int n = length(s) >= shared ? length(s) - shared : length(s);
     return std::max<int64_t>(1, (n + piece - 1) / piece);
