@@ -657,8 +657,7 @@ extern "C" int32_t sipa_prefix_plan(const sipa_prefix_params* p, int32_t num_gro
     }
     if (shares(g)) most_rows = std::max<int64_t>(most_rows, (int64_t)count_of(g) * G);
   }
-  const int cus = sipa_device_cu_count(-1);
-  if (cus < 0) return cus;
+  const int found = sipa_device_cu_count(-1), cus = found > 0 ? found : 256;  // planned without a GPU: an MI355X's
   sipa_prefix_layout l = {};
   l.tile_rows = most_rows <= 64 ? 64 : 128;
   const int kt = kPrefixStage;

@@ -253,6 +253,13 @@ def _kernel_rows(q: torch.Tensor) -> bool:
 
 
 class PagedKVCache:
+    # Bytes of a layer's K and V that decode rows with shared prefixes would read more than once, from which on they go to the
+    # shared-prefix kernel. Its two launches and its joins take 9 us (head_dim 64) to 13 us (128) at least, the decode kernel 6,
+    # which reads shared blocks from the caches; in us, shared-prefix / decode kernel: 16 rows, 4096 tokens of 0.5B, 31 MB 11.7 /
+    # 9.2; 16 groups of 4, 2048 tokens, 50 MB 12.4 / 16.0; 1.5B: 16 groups of 4, 512 tokens, 25 MB 12.9 / 10.9, 1024, 50 MB 15.5 /
+    # 16.5, 2048, 101 MB 18.6 / 26.7; INT8 1024, 26 MB 15.9 / 13.5, 2048, 51 MB 18.0 / 18.7.
+    prefix_min_bytes = 48 << 20
+
     def __init__(self, cfg: ModelConfig, num_blocks: int, block_size: int, device: str | torch.device,
                  dtype: torch.dtype, attn_backend: str = "gather"):
         """K and V pools of [layers, H_kv, num_blocks, block_size, d]; contents are garbage until written."""
@@ -402,7 +409,9 @@ class PagedKVCache:
         S, Hq, d = q.shape
         if not prefix_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads, max_context):
             return False
-        return sum((len(rows) - 1) * tokens for rows, tokens in self._shared) > 0
+        token = 2 * self.cfg.num_kv_heads * (d * self.k.element_size() + (2 if self.k.dtype is torch.int8 else 0))
+        again = sum((len(rows) - 1) * tokens for rows, tokens in self._shared) * token
+        return again >= self.prefix_min_bytes
 
     def _attend_prefill(self, layer: int, q: torch.Tensor, scale: float, out: torch.Tensor) -> None:
         """Multi-token rows of the forward, written into their rows of out [T, Hq, d] by the prefill kernel."""

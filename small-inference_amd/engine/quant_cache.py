@@ -358,10 +358,10 @@ class QuantPagedKVCache(PagedKVCache):
         if self.fmt == "int8":
             super().copy_blocks(copies)
             return
-        copy_blocks((self.v, self.v_scale), copies)
         # (a block without a slot: none of its tokens has been written yet)
         staged = [(src, dst, n) for src, dst, n in copies if src in self._stage_of]
         self._book.assign([dst for _, dst, _ in staged if dst not in self._stage_of])
+        copy_blocks((self.v, self.v_scale), copies)
         copy_blocks((self.stage,), [(self._stage_of[src], self._stage_of[dst], n) for src, dst, n in staged])
 
     def _commit_pools(self) -> tuple:

@@ -213,6 +213,23 @@ def test_streams_and_threads():
         assert len(outs) == 20 and all(torch.equal(w, o) for o in outs)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_blocks_past_four_gigabytes(fmt):
+    """The same batch at the far end of a pool whose bytes and elements pass 32 bits."""
+    x = batch([(128, [20, 40, 3])], [60], heads=(7, 1), seed=18, fmt=fmt)
+    want = run(x)
+    n, far = x.k.shape[1], (5 << 30) // (x.k.element_size() * 1024)
+    k, v = (torch.empty(1, far, 16, 64, dtype=x.k.dtype, device="cuda") for _ in range(2))
+    k[:, far - n:], v[:, far - n:] = x.k, x.v
+    if fmt == "int8":
+        ks, vs = (torch.empty(1, far, 16, dtype=torch.float16, device="cuda") for _ in range(2))
+        ks[:, far - n:], vs[:, far - n:] = x.ks, x.vs
+        x.quant = QuantKV(1, ks, vs)
+    x.bt = torch.where(x.bt >= 0, x.bt + (far - n), x.bt)
+    got = paged_prefix_attention(x.q, k, v, x.bt, x.ctx, x.groups, x.scale, x.max_ctx, quant=x.quant)
+    assert torch.equal(got, want)
+
+
 def test_no_sequences():
     x = batch([], [1], seed=16)
     q = x.q[:0]

@@ -24,9 +24,13 @@ FORMATS = ["bf16", "int8", "int8-kchannel"]
 
 
 def make_cache(fmt, m, backend="hip"):
+    """A cache that takes the shared-prefix kernel however little is shared."""
     if fmt == "bf16":
-        return PagedKVCache(CFG, m.num_blocks, m.block_size, "cuda", torch.bfloat16, backend)
-    return QuantPagedKVCache(CFG, m.num_blocks, m.block_size, "cuda", torch.bfloat16, backend, fmt=fmt, manager=m, n_stage=64)
+        cache = PagedKVCache(CFG, m.num_blocks, m.block_size, "cuda", torch.bfloat16, backend)
+    else:
+        cache = QuantPagedKVCache(CFG, m.num_blocks, m.block_size, "cuda", torch.bfloat16, backend, fmt=fmt, manager=m, n_stage=64)
+    cache.prefix_min_bytes = 1
+    return cache
 
 
 def contents(cache, layer, i):
@@ -238,3 +242,21 @@ def test_metadata_of_groups_is_kept_by_replace():
         outs.append(type(cache._plan))
     assert outs[1] is PrefixPlan and outs[3] is DecodePlan
     assert (outs[0].double() - outs[2].double()).abs().max() <= 2 ** -6 * outs[2].double().abs().max()
+
+
+@pytest.mark.parametrize("fmt,rows,kernel", [("bf16", 384, DecodePlan), ("bf16", 386, PrefixPlan), ("int8", 743, DecodePlan),
+                                             ("int8", 747, PrefixPlan)])
+def test_the_kernel_is_chosen_by_what_is_shared(fmt, rows, kernel):
+    """48 MiB that would be read again: 384 times 512 tokens of 256 bytes (bf16), 745 of 132 (INT8)."""
+    m = BlockManager(32 + rows, 16)
+    cache = make_cache(fmt, m)
+    del cache.prefix_min_bytes
+    m.allocate(0, 512)
+    m.fork(0, list(range(1, rows)))
+    for s in range(rows):
+        m.append_slot(s)
+    cache.k.zero_(), cache.v.zero_()
+    meta = build_metadata(m, [(s, 512, 1) for s in range(rows)], "cuda")
+    cache.begin(rows, meta)
+    out = cache.attend(0, torch.zeros(rows, 7, 64, device="cuda").bfloat16(), meta.positions, 0.125)
+    assert type(cache._plan) is kernel and out.shape == (rows, 448)
