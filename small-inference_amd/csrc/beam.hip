@@ -8,6 +8,8 @@
 //               are collected in LDS and put into order by counting.
 //   beam_merge  a workgroup a group, a wave a row: joins the pieces' sums in 64 bits and puts a row's candidates, then the
 //               group's, in order in the same way.
+// 512 rows of 151936 bf16 logits, 16 candidates of 8 rows each: 37.5 us and 6.5 (30.6 as a copy's rate reads them), bound by
+// memory and the exponentials' vector operations in turn; a few rows by the round trips of both kernels, 5 and 6 us.
 // It reads every logit once; no sum depends on the order in which workgroups or waves run, so equal rows get equal sums.
 #include <algorithm>
 #include <memory>
