@@ -35,8 +35,9 @@ def shared_groups(tables: list[np.ndarray], context_lens: list[int], block_size:
     share more than the others, the smaller groups are taken if the batch then reads fewer tokens."""
     full = [min(t.shape[0], c // block_size) for t, c in zip(tables, context_lens)]
 
-    def split(rows: list[int], depth: int) -> tuple[list[tuple[list[int], int]], int]:
-        """The groups of rows, which agree in their first `depth` blocks, and the tokens that they save."""
+    def split(rows: list[int], depth: int, level: int = 0) -> tuple[list[tuple[list[int], int]], int]:
+        """The groups of rows, which agree in their first `depth` blocks, and the blocks that they save; at most 32 groups
+        within each other are looked at."""
         if len(rows) < 2:
             return [], 0
         first = tables[rows[0]]
@@ -47,12 +48,12 @@ def shared_groups(tables: list[np.ndarray], context_lens: list[int], block_size:
                 same = depth + int(other[0])
         whole = ([(rows, same * block_size)] if same else []), (len(rows) - 1) * same
         parts: dict[int, list[int]] = {}
-        for r in rows:
+        for r in rows if level < 32 else ():
             if full[r] > same:
                 parts.setdefault(int(tables[r][same]), []).append(r)
         groups, saved = [], 0
         for part in parts.values():
-            g, s = split(part, same)
+            g, s = split(part, same, level + 1)
             groups += g
             saved += s
         return (groups, saved) if saved > whole[1] else whole
@@ -74,7 +75,7 @@ class PrefixPlan:
     batch whose tables agree in their first tokens / B entries, tokens whole blocks; a row is in one group at most. Groups
     change the time, not the result: every row attends the positions below its context length, and one whose context is
     shorter than its group's tokens is read by itself. host_context_lens: the lengths as a list, by which the work is
-    divided; None: they are read from the device once, which waits for it (in a capture max_context is taken for each).
+    divided; None: they are read from the device once, which waits for it. Calls can be captured, a plan is built before.
 
     The workspace is made for the call that needs it, so plans, streams and graphs share none. Threads may call one plan at
     the same time: each call fills the parameter block and launches under the plan's lock."""
@@ -100,7 +101,9 @@ class PrefixPlan:
         if host_context_lens is not None and (len(host_context_lens) != S or max(host_context_lens, default=0) > max_context):
             raise ValueError("host_context_lens must hold S lengths, none above max_context")
         _hip.require_gpu(q, k_cache, v_cache, block_tables, context_lens)
-        if host_context_lens is None and not torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("a PrefixPlan uploads its work list: build it before the graph capture")
+        if host_context_lens is None:
             host_context_lens = context_lens.tolist()
         self.shape, self.pool_shape, self.device = (S, Hq, D), tuple(k_cache.shape), q.device
         self.pool_dtype = torch.bfloat16 if quant is None else torch.int8

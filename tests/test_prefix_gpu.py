@@ -192,6 +192,19 @@ def test_captured_calls():
         check(eager, x, [min(n, f) for f in full])
 
 
+def test_plans_are_refused_in_a_capture():
+    x = batch([(64, [9, 20])], [33], seed=19)
+    run(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = x.q + 1
+        with pytest.raises(ValueError, match="before the graph capture"):
+            plan_of(x)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, x.q + 1)
+
+
 def test_streams_and_threads():
     x = batch([(512, [100] * 4)], [300], seed=15)
     plan = plan_of(x)

@@ -199,6 +199,17 @@ def test_shared_groups():
     assert shared_groups(tables, [84] * 3, 4) == [([0, 1, 2], 80)]
 
 
+def test_shared_groups_of_a_long_chain():
+    """Row i shares i blocks with the rows behind it: groups within groups, more than Python's stack holds."""
+    n = 1500
+    tables = [np.concatenate([np.arange(i), [10 ** 6 + i]]).astype(np.int32) for i in range(1, n + 1)]
+    found = shared_groups(tables, [4 * len(t) for t in tables], 4)
+    rows = [r for g, _ in found for r in g]
+    assert len(rows) == len(set(rows)) and found
+    for g, tokens in found:
+        assert tokens % 4 == 0 and all((tables[r][:tokens // 4] == tables[g[0]][:tokens // 4]).all() for r in g)
+
+
 def test_metadata_names_the_groups_of_decode_rows():
     m = BlockManager(40, 4)
     m.allocate(0, 9)
