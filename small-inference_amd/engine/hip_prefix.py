@@ -40,10 +40,10 @@ def shared_groups(tables: list[np.ndarray], context_lens: list[int], block_size:
         within each other are looked at."""
         if len(rows) < 2:
             return [], 0
-        first = tables[rows[0]]
         same = min(full[r] for r in rows)
-        for r in rows[1:]:
-            other = np.flatnonzero(tables[r][depth:same] != first[depth:same])
+        if same > depth:
+            ids = np.stack([tables[r][depth:same] for r in rows])
+            other = np.flatnonzero((ids != ids[0]).any(axis=0))
             if other.size:
                 same = depth + int(other[0])
         whole = ([(rows, same * block_size)] if same else []), (len(rows) - 1) * same
