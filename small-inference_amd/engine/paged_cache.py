@@ -338,7 +338,8 @@ class PagedKVCache:
             self._decode = (rows, bt, ctx, [meta.context_lens[i] for i in dec])
             self._decode_seqs = dec
             place = {seq: i for i, seq in enumerate(dec)}
-            self._shared = [([place[i] for i in seqs], tokens) for seqs, tokens in meta.shared]
+            groups = getattr(meta, "shared", ())  # (the reference's own metadata names none)
+            self._shared = [([place[i] for i in seqs], tokens) for seqs, tokens in groups]
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Scatter this forward's k, v [T, H_kv, d] into their slots."""

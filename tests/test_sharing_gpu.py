@@ -260,3 +260,21 @@ def test_the_kernel_is_chosen_by_what_is_shared(fmt, rows, kernel):
     cache.begin(rows, meta)
     out = cache.attend(0, torch.zeros(rows, 7, 64, device="cuda").bfloat16(), meta.positions, 0.125)
     assert type(cache._plan) is kernel and out.shape == (rows, 448)
+
+
+def test_metadata_without_groups():
+    """An object with the reference's fields alone goes to the decode kernel."""
+    m = BlockManager(20, 16)
+    m.allocate(0, 33)
+    meta = build_metadata(m, [(0, 32, 1)], "cuda")
+    names = [f.name for f in dataclasses.fields(meta) if f.name != "shared"]
+    bare = type("Bare", (), {**{n: getattr(meta, n) for n in names}, "num_seqs": 1})()
+    cache = make_cache("bf16", m)
+    cache.k.normal_(), cache.v.normal_()
+    q = torch.randn(1, 7, 64, device="cuda").bfloat16()
+    outs = []
+    for x in (meta, bare):
+        cache.begin(1, x)
+        outs.append(cache.attend(0, q, x.positions, 0.125))
+        assert type(cache._plan) is DecodePlan
+    assert torch.equal(*outs)
