@@ -249,7 +249,8 @@ class BlockManager:
     def fork(self, seq_id: int, new_ids: list[int]) -> list[tuple[int, int, int]]:
         """Create new_ids, each holding the tokens of seq_id: its full blocks are shared, its last one, if it is not full, is
         a block of their own for each. Returns the copies to make, (from block, to block, tokens), before anything is
-        written to or read from the new sequences (PagedKVCache.copy_blocks)."""
+        written to or read from the new sequences (PagedKVCache.copy_blocks). All of new_ids or none: an exception, a table
+        listener's too (device tables without rows left), leaves everything as it was."""
         table, n = self._tables[seq_id], self._lengths[seq_id]
         if len(set(new_ids)) != len(new_ids) or any(i in self._tables for i in new_ids):
             raise ValueError(f"new sequences {new_ids} must be distinct and not live yet")
@@ -260,7 +261,13 @@ class BlockManager:
         own = self._pop_blocks(need)
         for i, new in enumerate(new_ids):
             self._take(table[:full])
-            self._set_table(new, table[:full] + own[i:i + 1], n)
+            try:
+                self._set_table(new, table[:full] + own[i:i + 1], n)
+            except BaseException:
+                self._release(own[i + 1:][::-1])
+                for made in new_ids[i::-1]:
+                    self.free(made)
+                raise
         return [(table[full], b, rest) for b in own]
 
     def reorder(self, seq_ids: list[int], parents: list[int]) -> list[tuple[int, int, int]]:
