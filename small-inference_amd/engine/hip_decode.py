@@ -130,20 +130,29 @@ def split_grid(num_seqs: int, num_kv_heads: int, max_context: int, num_splits: i
 # Workspace (split partials + merge counters) per (device, stream): zero-filled once, the kernels leave the
 # counters zero again, so later calls on the same stream reuse it without a memset.
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}  # those made inside a capture: (its id, workspace)
 
 
 def reserve_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """The split workspace of (device, stream), at least nbytes (and 1 MiB) long. A larger request replaces the
     stream's buffer with a new zeroed one; the old one lives on only while something holds it, so code that keeps
     raw addresses beyond a call (captured graphs) must keep the tensor this returned, or reserve the largest size
-    it will need before it records any address."""
+    it will need before it records any address. One that has to be made inside a graph capture is that capture's alone: it is
+    the graph's memory, and only the graph's replays fill it with zeros."""
     device = torch.device(device)
     index = device.index if device.index is not None else torch.cuda.current_device()
     key = (index, stream)
     ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    capture = _hip.lib().sipa_capture_id(stream)
+    held, ws = _captured.get(key, (0, None)) if capture else (0, None)
+    if held != capture or ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
-        _workspaces[key] = ws
+        if capture:
+            _captured[key] = capture, ws
+        else:
+            _workspaces[key] = ws
     return ws
 
 
