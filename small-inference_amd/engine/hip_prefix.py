@@ -101,7 +101,7 @@ class PrefixPlan:
         if host_context_lens is not None and (len(host_context_lens) != S or max(host_context_lens, default=0) > max_context):
             raise ValueError("host_context_lens must hold S lengths, none above max_context")
         _hip.require_gpu(q, k_cache, v_cache, block_tables, context_lens)
-        if torch.cuda.is_current_stream_capturing():
+        if _hip.lib().sipa_capture_id(_hip.stream_of(q)):
             raise ValueError("a PrefixPlan uploads its work list: build it before the graph capture")
         if host_context_lens is None:
             host_context_lens = context_lens.tolist()

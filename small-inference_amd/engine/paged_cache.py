@@ -23,6 +23,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from . import _hip
 from ._hip import layer_ptr
 from .attention import attention
 from .block_manager import BlockManager
@@ -406,8 +407,11 @@ class PagedKVCache:
                                  cfg.num_q_heads // cfg.num_kv_heads, max_context)
 
     def _prefix_kernel_ok(self, q: torch.Tensor, max_context: int) -> bool:
-        """Whether the forward's decode rows go to the shared-prefix kernel, which reads a group's keys once."""
+        """Whether the forward's decode rows go to the shared-prefix kernel, which reads a group's keys once. Not inside a graph
+        capture: its plan uploads a work list."""
         S, Hq, d = q.shape
+        if _hip.lib().sipa_capture_id(_hip.stream_of(q)):
+            return False
         if not prefix_supported(q.dtype, self.k.dtype, self.block_size, d, Hq // self.cfg.num_kv_heads, max_context):
             return False
         token = 2 * self.cfg.num_kv_heads * (d * self.k.element_size() + (2 if self.k.dtype is torch.int8 else 0))

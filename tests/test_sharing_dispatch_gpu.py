@@ -1,0 +1,71 @@
+"""Forwards over forked sequences that the shared-prefix kernel cannot take as they come: each is answered, as it is where the
+sequences share nothing."""
+
+import pytest
+import torch
+
+from engine.block_manager import BlockManager
+from engine.config import ModelConfig
+from engine.hip_decode import DecodePlan
+from engine.hip_prefix import PrefixPlan
+from engine.paged_cache import PagedKVCache, build_metadata
+from engine.quant_cache import QuantPagedKVCache
+
+pytestmark = pytest.mark.gpu
+CFG = ModelConfig(vocab_size=64, hidden_size=448, intermediate_size=64, num_layers=2, num_q_heads=7, num_kv_heads=1, head_dim=64)
+
+
+def forked(fmt="bf16", members=4, tokens=700):
+    """A cache that takes the shared-prefix kernel however little is shared, and the metadata of a step over forked sequences."""
+    m = BlockManager(60 + members, 16)
+    if fmt == "bf16":
+        cache = PagedKVCache(CFG, m.num_blocks, 16, "cuda", torch.bfloat16, "hip")
+        cache.k.normal_(), cache.v.normal_()
+    else:
+        cache = QuantPagedKVCache(CFG, m.num_blocks, 16, "cuda", torch.bfloat16, "hip", fmt=fmt, manager=m)
+        for t in (cache.k, cache.v):
+            t.copy_(torch.randint(-127, 128, t.shape, device="cuda"))
+        for t in (cache.k_scale, cache.v_scale):
+            t.uniform_(0.005, 0.02)
+    cache.prefix_min_bytes = 1
+    m.allocate(0, tokens)
+    m.fork(0, list(range(1, members)))
+    for s in range(members):
+        m.append_slot(s)
+    meta = build_metadata(m, [(s, tokens, 1) for s in range(members)], "cuda")
+    assert meta.shared
+    return cache, meta
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_captured_forwards_go_to_the_decode_kernel(fmt):
+    cache, meta = forked(fmt)
+    q = [torch.randn(4, 7, 64, device="cuda").bfloat16() for _ in range(2)]
+
+    def step():
+        cache.begin(4, meta)
+        return [cache.attend(layer, q[layer], meta.positions, 0.125) for layer in range(2)]
+
+    shared = meta.shared
+    step()
+    assert type(cache._plan) is PrefixPlan
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    assert type(cache._plan) is DecodePlan
+    for _ in range(4):
+        for x in q:
+            x.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        meta.shared = []
+        want = step()
+        assert type(cache._plan) is DecodePlan and all(torch.equal(a, b) for a, b in zip(out, want))
+        meta.shared = shared
+        eager = step()
+        assert type(cache._plan) is PrefixPlan
+        # each kernel: 2^-8 of the result (its rounding), and under 2^-12 of the weights' sum of |v| (scores, exponentials, two
+        # bf16 terms of the weights), which is at most the largest |v|, under 8
+        for a, b in zip(eager, want):
+            assert ((a.double() - b.double()).abs() <= 2 ** -7 * b.double().abs() + 2 * 2 ** -12 * 8).all()
