@@ -449,12 +449,14 @@ class PagedKVCache:
         in_place = type(rows) is slice
         out = None if rows is None else torch.empty(T, Hq * d, device=q.device, dtype=q.dtype)
         q_dec = q if rows is None else q[rows]
-        if in_place and not _kernel_rows(q_dec):  # as the gather would lay them out
+        fresh = self._plan is None or self._plan_scale != scale  # first layer of the forward: validate once
+        shared = bool(self._shared) and self._prefix_kernel_ok(q_dec, max(lens)) if fresh else type(self._plan) is PrefixPlan
+        if (in_place or shared) and not _kernel_rows(q_dec):  # as the gather would lay them out
             q_dec = q_dec.clone(memory_format=torch.contiguous_format)
         dec_out = out[rows].view(-1, Hq, d) if in_place else None
-        if self._plan is None or self._plan_scale != scale:  # first layer of the forward: validate once
+        if fresh:
             # The host-side lengths let a ragged batch run from a work list (built once, used by every layer).
-            if self._shared and self._prefix_kernel_ok(q_dec, max(lens)):
+            if shared:
                 self._plan = PrefixPlan(q_dec, self.k[layer], self.v[layer], bt, ctx, self._shared, scale, max(lens),
                                         quant=self._kernel_quant(layer), host_context_lens=lens)
                 dec = self._plan(q_dec, self.k[layer], self.v[layer], out=dec_out)

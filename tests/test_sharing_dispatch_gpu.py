@@ -69,3 +69,19 @@ def test_captured_forwards_go_to_the_decode_kernel(fmt):
         # bf16 terms of the weights), which is at most the largest |v|, under 8
         for a, b in zip(eager, want):
             assert ((a.double() - b.double()).abs() <= 2 ** -7 * b.double().abs() + 2 * 2 ** -12 * 8).all()
+
+
+@pytest.mark.parametrize("rows", ["head stride", "row stride", "address"])
+def test_rows_at_any_alignment(rows):
+    """q that the decode kernels take although no 16-byte load fits it: the first layer's, or a later one's alone."""
+    cache, meta = forked()
+    q = torch.randn(4, 7, 64, device="cuda").bfloat16()
+    odd = {"head stride": lambda: torch.empty(4, 7, 65, device="cuda", dtype=torch.bfloat16)[..., :64],
+           "row stride": lambda: torch.empty(4, 7 * 64 + 1, device="cuda", dtype=torch.bfloat16)[:, :448].view(4, 7, 64),
+           "address": lambda: torch.empty(4 * 448 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 7, 64)}[rows]().copy_(q)
+    cache.begin(4, meta)
+    want = [cache.attend(layer, q, meta.positions, 0.125) for layer in range(2)]
+    for first, second in ((odd, odd), (q, odd), (odd, q)):
+        cache.begin(4, meta)
+        got = [cache.attend(layer, x, meta.positions, 0.125) for layer, x in enumerate((first, second))]
+        assert type(cache._plan) is PrefixPlan and all(torch.equal(a, b) for a, b in zip(got, want))
