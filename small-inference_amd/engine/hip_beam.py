@@ -123,6 +123,23 @@ def _select_torch(logits, scores, starts, beams: int, groups: int, candidates: i
     return out
 
 
+def _flat(copies: Sequence[tuple[int, int, int]], blocks: int, block_size: int) -> array:
+    """The copies' numbers, one after the other."""
+    try:
+        flat = array("i", itertools.chain.from_iterable(copies))
+    except OverflowError:
+        raise ValueError(f"copies past the {blocks} blocks of {block_size} tokens") from None
+    if len(flat) != 3 * len(copies) or not set(map(len, copies)) <= {3}:
+        raise ValueError("copies must be (src, dst, tokens)")
+    return flat
+
+
+def check_copies(copies: Sequence[tuple[int, int, int]], blocks: int, block_size: int) -> None:
+    """ValueError unless copy_blocks takes these copies in pools of `blocks` blocks of block_size tokens."""
+    flat = _flat(copies, blocks, block_size)
+    _hip.check(_hip.lib().sipa_check_copies(flat.buffer_info()[0], len(copies), blocks, block_size), "copy_blocks")
+
+
 def copy_blocks(pools: Sequence[torch.Tensor], copies: Sequence[tuple[int, int, int]]) -> None:
     """For each (src, dst, tokens) of copies, the first `tokens` tokens of block src become those of block dst, in every layer
     and head of the pools, in place (sipa_copy_blocks; one launch for 424 copies). No block may be the destination of two
@@ -150,12 +167,7 @@ def copy_blocks(pools: Sequence[torch.Tensor], copies: Sequence[tuple[int, int, 
         ptrs[i], st_l[i], st_h[i], row_bytes[i] = t.data_ptr(), st[0] * size, st[1] * size, row * size
     if not n:
         return
-    try:
-        flat = array("i", itertools.chain.from_iterable(copies))
-    except OverflowError:
-        raise ValueError(f"copies past the {N} blocks of {B} tokens") from None
-    if len(flat) != 3 * n or set(map(len, copies)) != {3}:
-        raise ValueError("copies must be (src, dst, tokens)")
+    flat = _flat(copies, N, B)
     at = flat.buffer_info()[0]
     if not first.is_cuda:
         _hip.check(_hip.lib().sipa_check_copies(at, n, N, B), "copy_blocks")

@@ -26,7 +26,7 @@ import torch
 
 from .block_manager import BlockManager
 from .config import ModelConfig
-from .hip_beam import copy_blocks
+from .hip_beam import check_copies, copy_blocks
 from .hip_decode import QuantKV
 from .hip_quant import (kchan_write_rows, quantize_store_block_rows, quantize_store_blocks, quantize_store_layer,
                         quantize_store_tokens, store_tokens)
@@ -358,11 +358,17 @@ class QuantPagedKVCache(PagedKVCache):
         if self.fmt == "int8":
             super().copy_blocks(copies)
             return
+        check_copies(copies, self.num_blocks, self.block_size)  # before any block is given a slot
         # (a block without a slot: none of its tokens has been written yet)
         staged = [(src, dst, n) for src, dst, n in copies if src in self._stage_of]
-        self._book.assign([dst for _, dst, _ in staged if dst not in self._stage_of])
-        copy_blocks((self.v, self.v_scale), copies)
-        copy_blocks((self.stage,), [(self._stage_of[src], self._stage_of[dst], n) for src, dst, n in staged])
+        fresh = [dst for _, dst, _ in staged if dst not in self._stage_of]
+        self._book.assign(fresh)
+        try:
+            copy_blocks((self.v, self.v_scale), copies)
+            copy_blocks((self.stage,), [(self._stage_of[src], self._stage_of[dst], n) for src, dst, n in staged])
+        except BaseException:
+            self._book.release(fresh[::-1])
+            raise
 
     def _commit_pools(self) -> tuple:
         if self.fmt != "int8":
