@@ -41,6 +41,7 @@ class BlockManager:
         self._free_listeners: list[Callable[[list[int]], None]] = []
         self._table_listeners: list[Callable[[int, int], None]] = []
         self._truncate_checks: list[Callable[[int], None]] = []
+        self._copy_checks: list[Callable[[list[int], list[int]], None]] = []
 
     # ---- queries -------------------------------------------------------------------------------------------------
 
@@ -129,6 +130,11 @@ class BlockManager:
     def add_truncate_check(self, fn: Callable[[int], None]) -> None:
         """Call fn(block) before a truncate() that keeps part of the tokens of a sequence's `block`; an exception refuses it."""
         self._truncate_checks.append(fn)
+
+    def add_copy_check(self, fn: Callable[[list[int], list[int]], None]) -> None:
+        """Call fn(sources, released) before a fork() or reorder() that asks for copies: a block for each copy's source, and the
+        blocks that return to the stack before the copies are made; an exception refuses it."""
+        self._copy_checks.append(fn)
 
     def add_table_listener(self, fn: Callable[[int, int], None]) -> None:
         """Call fn(seq_id, first) when a sequence's table is created (first = 0) or gains blocks from index first
@@ -250,7 +256,8 @@ class BlockManager:
         """Create new_ids, each holding the tokens of seq_id: its full blocks are shared, its last one, if it is not full, is
         a block of their own for each. Returns the copies to make, (from block, to block, tokens), before anything is
         written to or read from the new sequences (PagedKVCache.copy_blocks). All of new_ids or none: an exception, a table
-        listener's too (device tables without rows left), leaves everything as it was."""
+        listener's too (device tables without rows left) or that of an int8-kchannel cache with too few idle staging slots,
+        leaves everything as it was."""
         table, n = self._tables[seq_id], self._lengths[seq_id]
         if len(set(new_ids)) != len(new_ids) or any(i in self._tables for i in new_ids):
             raise ValueError(f"new sequences {new_ids} must be distinct and not live yet")
@@ -258,6 +265,9 @@ class BlockManager:
         need = len(new_ids) if rest else 0
         if need > len(self._free):
             raise OutOfBlocks(f"{len(new_ids)} forks of sequence {seq_id} take {need} blocks; the pool has {len(self._free)} free")
+        if need:
+            for fn in self._copy_checks:
+                fn([table[full]] * need, [])
         own = self._pop_blocks(need)
         for i, new in enumerate(new_ids):
             self._take(table[:full])
@@ -274,7 +284,7 @@ class BlockManager:
         """Sequence seq_ids[i] goes on from what seq_ids[parents[i]] holds (beams after a selection): it gives up its own
         blocks and shares that one's full ones; a last block that is not full stays with one of them, and the others get
         copies. Returns the copies to make, as fork does. No more blocks are held afterwards than len(seq_ids) tables of the
-        longest would take; OutOfBlocks and ValueError leave everything as it was."""
+        longest would take; OutOfBlocks, ValueError and a cache's refusal (too few staging slots) leave everything as it was."""
         if len(set(seq_ids)) != len(seq_ids) or len(parents) != len(seq_ids):
             raise ValueError(f"{len(parents)} parents of {len(seq_ids)} sequences, which must be distinct")
         if any(not 0 <= p < len(seq_ids) for p in parents):
@@ -299,9 +309,13 @@ class BlockManager:
                 change[b] = change.get(b, 0) - 1
             for b in blocks:
                 change[b] = change.get(b, 0) + 1
-        room = len(self._free) + sum(self._ref[b] + c == 0 for b, c in change.items())
+        given_up = [b for b, c in change.items() if self._ref[b] + c == 0]
+        room = len(self._free) + len(given_up)
         if len(copied) > room:
             raise OutOfBlocks(f"{len(copied)} copies of last blocks; the pool has {room} blocks for them")
+        if copied:
+            for fn in self._copy_checks:
+                fn([tables[parents[i]][-1] for i in copied], given_up)
         for blocks in taken:
             self._take(blocks)
         for i in moved:

@@ -87,6 +87,14 @@ class StagingBook:
             raise ValueError(f"int8-kchannel: block {block} is quantized and cannot keep part of its tokens; truncate to a "
                              f"multiple of the block size or within the staged last block")
 
+    def check_copies(self, sources, released) -> None:
+        """RuntimeError where copies of these blocks, made after `released` have given up their slots, would find too few."""
+        need = sum(b in self.slot_of for b in sources)
+        idle = len(self.free) + sum(b in self.slot_of for b in released)
+        if need > idle:
+            raise RuntimeError(f"copies of {need} partial blocks need as many INT8 staging slots, {idle} of {self.n_stage} are "
+                               f"idle; construct the cache with a larger n_stage")
+
     def release(self, blocks) -> None:
         """Blocks that left staging (quantized into the pool, or freed by the block manager) return their slots,
         in the order given; blocks without a slot are ignored."""
@@ -173,6 +181,7 @@ class QuantPagedKVCache(PagedKVCache):
             self._stage_of, self._free_stage = self._book.slot_of, self._book.free
             manager.add_free_listener(self._book.release)
             manager.add_truncate_check(self._book.check_truncate)
+            manager.add_copy_check(self._book.check_copies)
 
     def _allocate(self, shape: tuple, device: str | torch.device, dtype: torch.dtype) -> None:
         """int8 K/V, fp16 scales, and (format B) the bf16 staging slots; all zero-initialised."""

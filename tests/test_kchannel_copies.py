@@ -67,3 +67,49 @@ def test_copies_that_are_taken():
     for s in (0, 1, 2):
         m.free(s)
     assert not cache._stage_of and len(cache._free_stage) == 4
+
+
+def state(m):
+    return {s: (m.block_table(s), m.seq_len(s)) for s in m.seq_ids()}, m.num_free_blocks(), m.num_shared_blocks()
+
+
+def test_forks_without_staging_slots_are_refused_before_they_are_made():
+    m, cache = filled(n_stage=3)
+    before = state(m), slots(cache)
+    with pytest.raises(RuntimeError, match="staging slots"):
+        m.fork(0, [1, 2, 3])
+    assert (state(m), slots(cache)) == before
+    m.check_invariants()
+    cache.copy_blocks(m.fork(0, [1, 2]))  # as many as there are
+    assert not cache._free_stage
+    m.allocate(7, 4)  # whole blocks are not staged
+    write(cache, m, 7, 0, 4)
+    assert m.fork(7, [8]) == []
+    m.append_slots(8, 1)  # a last block that has not been written holds no slot
+    cache.copy_blocks(m.fork(8, [9]))
+    m.check_invariants()
+
+
+def test_reorders_without_staging_slots_are_refused_before_they_are_made():
+    m, cache = filled(n_stage=2)
+    m.allocate(1, 4)
+    write(cache, m, 1, 0, 4)
+    cache.copy_blocks(m.fork(0, [2]))  # both slots are taken
+    before = state(m), slots(cache)
+    with pytest.raises(RuntimeError, match="staging slots"):
+        m.reorder([0, 1], [0, 0])
+    with pytest.raises(RuntimeError, match="staging slots"):
+        m.reorder([0, 1, 2], [0, 0, 0])  # two copies, of which one slot comes back
+    assert (state(m), slots(cache)) == before
+    m.check_invariants()
+    copies = m.reorder([0, 2], [0, 0])  # sequence 2's slot goes to its copy
+    assert len(copies) == 1
+    cache.copy_blocks(copies)
+    assert m.reorder([0, 1], [1, 1]) == []  # nothing to copy
+    copies = m.reorder([1, 2], [1, 1])  # sequence 1 goes on from 2: the slot that sequence 0 gave up serves the copy
+    cache.copy_blocks(copies)
+    assert set(cache._stage_of) == {b for c in copies for b in c[:2]} and not cache._free_stage
+    for s in (0, 1, 2):
+        m.free(s)
+    assert not cache._stage_of and len(cache._free_stage) == 2
+    m.check_invariants()
