@@ -180,8 +180,11 @@ class QuantPagedKVCache(PagedKVCache):
             self._book = StagingBook(n_stage)
             self._stage_of, self._free_stage = self._book.slot_of, self._book.free
             manager.add_free_listener(self._book.release)
-            manager.add_truncate_check(self._book.check_truncate)
-            manager.add_copy_check(self._book.check_copies)
+            # (the reference's own manager neither truncates nor forks)
+            for name, check in (("add_truncate_check", self._book.check_truncate), ("add_copy_check", self._book.check_copies)):
+                add = getattr(manager, name, None)
+                if add is not None:
+                    add(check)
 
     def _allocate(self, shape: tuple, device: str | torch.device, dtype: torch.dtype) -> None:
         """int8 K/V, fp16 scales, and (format B) the bf16 staging slots; all zero-initialised."""
