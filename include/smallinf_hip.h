@@ -798,7 +798,9 @@ int32_t sipa_prefix_attention(const sipa_prefix_params* p, void* stream);
  * The best continuations of beams: of the rows of each group, the num_candidates tokens v of largest
  *   scores[r] + logits[r, v] - log(sum_v exp(logits[r, v])),
  * in descending order; equal ones by row, then by token. A row's tokens are ordered by their logits, rows against each other
- * by these sums in 64 bits, from which out_scores are rounded once. Group g has the rows g * beams .. (g + 1) * beams - 1, or
+ * by these sums, from which out_scores are rounded once. A row's exponentials, and sums of eight of them, are fp32, everything
+ * after that fp64: its log is within 2^-19, so candidates of different rows whose scores are closer than 2^-18 may change
+ * places; rows of equal logits get equal logs. Group g has the rows g * beams .. (g + 1) * beams - 1, or
  * with starts [num_groups + 1] rows starts[g] .. starts[g + 1] - 1 (clamped to the rows, 1024 of a group at most). Tokens of
  * logit -inf are none of them, nor are those of a row whose score or sum is not finite (NaN or +inf among its logits, all of
  * them -inf). Where there are fewer than num_candidates: score -inf, beam and token -1.

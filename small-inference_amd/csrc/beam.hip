@@ -11,6 +11,9 @@
 // 512 rows of 151936 bf16 logits, 16 candidates of 8 rows each: 37.5 us and 6.5 (30.6 as a copy's rate reads them), bound by
 // memory and the exponentials' vector operations in turn; a few rows by the round trips of both kernels, 5 and 6 us.
 // It reads every logit once; no sum depends on the order in which workgroups or waves run, so equal rows get equal sums.
+// A row's log-sum is within 2^-19: of its terms exp(-d), d the distance to the piece's largest logit, an exponent's argument is
+// off by d 2^-22.8 at most (difference, constant and product rounded), exp2 by 2^-23, the sum of eight by 7 2^-24; the mean of d
+// over a piece's weights is under 6.8 whatever the piece's 16384 logits are (one on top, the others W(16384 / e) below it).
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamArgs 
     const uint32_t key[4] = {upper_key(of[0]), upper_key(of[1]), upper_key(of[2]), upper_key(of[3])};
     low = upper_value(nth_key(key, a.N));
   }
-  // exp(l - top) as exp2((l - top) log2 e): its argument is rounded, 2^-20 of the term at most where the term matters.
+  // exp(l - top) as exp2((l - top) log2 e), the argument rounded (the bound of the sum is at the top).
   const float off = top == kNegInf ? 0.f : top;
   low = fmaxf(low, -__FLT_MAX__);  // never -inf (or NaN, which the key 0 stands for)
   double sum = 0.;

@@ -43,7 +43,9 @@ class BeamChoice(NamedTuple):
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int | torch.Tensor, candidates: int) -> BeamChoice:
     """The `candidates` (1 .. 64) best continuations over the beams and the vocabulary of each request, in two launches
     (sipa_beam_select): of row r and token v the score is scores[r] + log_softmax(logits[r])[v], equal ones in the order of
-    their rows, then tokens. The scores decide in 64 bits and are returned in 32.
+    their rows, then tokens. On the GPU a row's log-sum is within 2^-19 of the definition's (exponentials, and sums of eight, in 32
+    bits), all after it is in 64 bits: candidates of different rows whose scores are closer than 2^-18 may change places; those of
+    one row do not, and rows of equal logits and scores tie. Scores are returned in 32 bits.
 
     logits [R, V] bf16, fp16 or fp32 with a contiguous last dim (R the beams of all requests); scores [R] fp32; beams: how
     many rows each request has (1 to 1024, dividing R; 1 for the first step, when there is one row a request), or int32
