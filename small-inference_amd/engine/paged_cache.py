@@ -258,7 +258,10 @@ class PagedKVCache:
     # shared-prefix kernel. Its two launches and its joins take 9 us (head_dim 64) to 13 us (128) at least, the decode kernel 6,
     # which reads shared blocks from the caches; in us, shared-prefix / decode kernel: 16 rows, 4096 tokens of 0.5B, 31 MB 11.7 /
     # 9.2; 16 groups of 4, 2048 tokens, 50 MB 12.4 / 16.0; 1.5B: 16 groups of 4, 512 tokens, 25 MB 12.9 / 10.9, 1024, 50 MB 15.5 /
-    # 16.5, 2048, 101 MB 18.6 / 26.7; INT8 1024, 26 MB 15.9 / 13.5, 2048, 51 MB 18.0 / 18.7.
+    # 16.5, 2048, 101 MB 18.6 / 26.7; INT8 1024, 26 MB 15.9 / 13.5, 2048, 51 MB 18.0 / 18.7. Over 4900 drawn batches (equal and
+    # unequal groups, pairs, sequences alone; pools past the caches) the mean time is 1.007 (bf16, head_dim 64), 1.006 (bf16, 128)
+    # and 1.014 (INT8, 128) of the better kernel's in each; with 32 MiB 1.013, 1.009, 1.021, with 96 MiB 1.040, 1.038, 1.025, the
+    # decode kernel alone 1.38, 1.64, 1.20. (INT8 at head_dim 64: engine.quant_cache.)
     prefix_min_bytes = 48 << 20
 
     def __init__(self, cfg: ModelConfig, num_blocks: int, block_size: int, device: str | torch.device,

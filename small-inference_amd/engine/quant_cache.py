@@ -170,6 +170,11 @@ class QuantPagedKVCache(PagedKVCache):
             raise ValueError(f"fmt must be int8 or int8-kchannel, got {fmt}")
         self.fmt, self.n_stage = fmt, n_stage
         super().__init__(cfg, num_blocks, block_size, device, dtype, attn_backend)
+        if cfg.head_dim == 64:
+            # Where the shared-prefix kernel spends as long on converting codes as it saves in bytes: the mean over 1340 drawn
+            # batches is 1.016 of the better kernel's time from 160 MiB on, 1.090 from 48, 1.022 from 128, 1.016 from 192; the
+            # decode kernel alone 1.038. (64 pairs of 4096 + 1000 tokens, 66 MiB: 74 us, decode kernel 33.)
+            self.prefix_min_bytes = 160 << 20
         self.fused_writes = self.on_gpu  # HIP quantize-and-store on GPU pools; torch quantizer otherwise
         self._staged = self._done = self._direct = None
         self._rows_write = None  # format B decode step: (staging slot per row, quantization block per row or None)

@@ -85,3 +85,25 @@ def test_rows_at_any_alignment(rows):
         cache.begin(4, meta)
         got = [cache.attend(layer, x, meta.positions, 0.125) for layer, x in enumerate((first, second))]
         assert type(cache._plan) is PrefixPlan and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("fmt,head_dim,rows,kernel", [("int8", 64, 311, DecodePlan), ("int8", 64, 312, PrefixPlan), ("int8", 128, 48, DecodePlan),
+                                                      ("int8", 128, 49, PrefixPlan), ("bf16", 64, 48, DecodePlan), ("bf16", 64, 49, PrefixPlan)])
+def test_what_a_cache_takes_the_kernel_for(fmt, head_dim, rows, kernel):
+    """A cache's own limits, for one KV head and 4096 shared tokens: INT8 at head_dim 64 from 160 MiB that would be read again
+    (310.3 times 4096 tokens of 132 bytes), at 128 from 48 MiB (47.3 times, 260 bytes), bf16 from 48 MiB (48 times, 256 bytes)."""
+    cfg = ModelConfig(vocab_size=64, hidden_size=448, intermediate_size=64, num_layers=1, num_q_heads=7, num_kv_heads=1, head_dim=head_dim)
+    m = BlockManager(256 + rows, 16)
+    if fmt == "bf16":
+        cache = PagedKVCache(cfg, m.num_blocks, 16, "cuda", torch.bfloat16, "hip")
+    else:
+        cache = QuantPagedKVCache(cfg, m.num_blocks, 16, "cuda", torch.bfloat16, "hip", fmt=fmt, manager=m)
+    cache.k.zero_(), cache.v.zero_()
+    m.allocate(0, 4096)
+    m.fork(0, list(range(1, rows)))
+    for s in range(rows):
+        m.append_slot(s)
+    meta = build_metadata(m, [(s, 4096, 1) for s in range(rows)], "cuda")
+    cache.begin(rows, meta)
+    out = cache.attend(0, torch.zeros(rows, 7, head_dim, device="cuda").bfloat16(), meta.positions, 0.125)
+    assert type(cache._plan) is kernel and not out.any()
