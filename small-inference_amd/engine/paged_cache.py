@@ -96,10 +96,13 @@ class PagedMetadata:
 
 def decode_groups(manager: BlockManager, tables: list[np.ndarray], context_lens: list[int],
                   new_tokens: list[int]) -> list[tuple[list[int], int]]:
-    """The groups of a forward's sequences of one new token whose tables share blocks ([] for managers that share none)."""
+    """The groups of a forward's sequences of one new token whose tables share blocks ([] for managers that share none). Shared
+    blocks are the first ones of their tables: sequences whose first block is their own are not searched."""
     if not getattr(manager, "num_shared_blocks", int)():
         return []
-    dec = [i for i, n in enumerate(new_tokens) if n == 1]
+    dec = [i for i, n in enumerate(new_tokens) if n == 1 and manager.ref_count(tables[i].item(0)) > 1]
+    if len(dec) < 2:
+        return []
     found = shared_groups([tables[i] for i in dec], [context_lens[i] for i in dec], manager.block_size)
     return [([dec[r] for r in rows], tokens) for rows, tokens in found]
 
