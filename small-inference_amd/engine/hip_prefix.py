@@ -179,7 +179,7 @@ class PrefixPlan:
         the plan called with pools[layer] and the like, without making those views."""
         for t in (k_pools, v_pools):
             if t.shape[1:] != self.pool_shape or t.dtype is not self.pool_dtype or t.device != self.device or \
-                    t.stride()[1:] != self._pool_strides:
+                    (t.stride()[1:] != self._pool_strides and not _hip.layers_contiguous(t)):
                 raise ValueError("the pools do not match the plan")
         self._check_quant(quant, k_pools.shape[:1])
         with self._lock:

@@ -265,7 +265,7 @@ class TreePlan:
         self._bind_q(q)
         p = self.params
         p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-        p.kv_stride_h, p.kv_stride_n = k_cache.stride(0), k_cache.stride(1)
+        p.kv_stride_h, p.kv_stride_n = self._pool_strides[:2]
         self._check_quant(quant, ())
         if quant is not None:
             ks, vs = quant.k_scale, quant.v_scale
@@ -278,14 +278,14 @@ class TreePlan:
         the plan called with pools[layer] and the like, without making those views."""
         for t in (k_pools, v_pools):
             if t.shape[1:] != self.pool_shape or t.dtype is not self.pool_dtype or t.device != self.device or \
-                    t.stride()[1:] != self._pool_strides:
+                    (t.stride()[1:] != self._pool_strides and not _hip.layers_contiguous(t)):
                 raise ValueError("the pools do not match the plan")
         self._check_quant(quant, k_pools.shape[:1])
         with self._lock:
             self._bind_q(q)
             p = self.params
             p.k_cache, p.v_cache = _hip.layer_ptr(k_pools, layer), _hip.layer_ptr(v_pools, layer)
-            p.kv_stride_h, p.kv_stride_n = k_pools.stride(1), k_pools.stride(2)
+            p.kv_stride_h, p.kv_stride_n = self._pool_strides[:2]
             self._k, self._v, self._quant = k_pools, v_pools, quant
             if quant is not None:
                 ks, vs = quant.k_scale, quant.v_scale
