@@ -555,7 +555,8 @@ static int beam_layout(const sipa_beam_params* p, BeamLayout* l) {
   l->piece = ((p->vocab + l->ns - 1) / l->ns + e - 1) / e * e;  // alike, whole parts
   l->ns = (p->vocab + l->piece - 1) / l->piece;
   const int64_t pieces = (int64_t)p->num_rows * l->ns;
-  SIPA_CHECK(pieces <= 0x7fffffff, SIPA_EUNSUPPORTED, "%d rows of %d pieces exceed the grid limit", p->num_rows, l->ns);
+  SIPA_CHECK(pieces <= (int64_t)(0xffffffffu / kBeamThreads) && p->num_groups <= (int32_t)(0xffffffffu / (64 * kMergeWaves)),
+             SIPA_EUNSUPPORTED, "%d rows of %d pieces, %d groups: a launch holds 2^32 threads", p->num_rows, l->ns, p->num_groups);
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   l->sum = up(pieces * 4);
   l->key = l->sum + up(pieces * 8);
