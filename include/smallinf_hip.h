@@ -741,7 +741,7 @@ uint64_t sipa_capture_id(void* stream);
  *   out[s, h*G + g, :] = sum_j softmax_j(scale * q[s, h*G + g, :] . k_j) v_j over the positions j < context_lens[s] of s's
  * block table; a row without any gets zeros. What is shared changes the time, not the result: a group is a promise of the
  * caller that its members' tables agree in their first tokens / B entries. A member whose context is shorter than that is
- * read by itself. bf16 q and out; pools bf16 (SIPA_KV_PLAIN) or int8 with per-token scales (SIPA_KV_INT8_TOKEN). head_dim 64
+ * read by itself. Probabilities keep 16 bits in the product with V, states are fp32. bf16 q and out; pools bf16 (SIPA_KV_PLAIN) or int8 with per-token scales (SIPA_KV_INT8_TOKEN). head_dim 64
  * or 128, blocks of 16, 32 or 64 tokens, groups of up to 16 query heads a KV head. K and V behind the contexts' ends may hold
  * anything.
  *

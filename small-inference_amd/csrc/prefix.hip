@@ -9,10 +9,13 @@
 // of 16, a wave each, eight to a workgroup: most are short, and a wave needs no other. Both kinds are in one launch, so that the
 // pieces' loads run beside the items' products; a second, small one joins a row's parts.
 //
+// A row is in one group: of prefixes within prefixes the plan's caller chooses one level, the others' keys are read for every row.
+//
 // What bounds it: with long contexts of their own the pools' bytes (256 sequences behind 2048 tokens with about 600 of their own,
-// head_dim 128, 16-bit pools: 40 us, 32 of them for the bytes at a copy's rate; read apart 93); with long prefixes and many rows
-// the vector ALUs and LDS reads of the items (2 x 37 sequences at 30016 tokens: 35 us, 5.7 for the products); short batches the
-// round trips of two launches, 9 us.
+// head_dim 128, 16-bit pools: 49 us with pools that change from call to call, 32 of them for the bytes at a copy's rate, and 40 with
+// pools that stay in the caches; read apart 93); with long prefixes and many rows the vector ALUs and LDS reads of the items, and
+// tiles that are not full (2 x 37 sequences at 30016 tokens: 35 us, 5.7 for the products; each group's 259 rows make two tiles of
+// 128 and one of 3); INT8 the conversion of codes; short batches the round trips of two launches, 9 us.
 #include <algorithm>
 
 #include "decode_common.h"
@@ -119,8 +122,11 @@ struct RowState {
   // Takes up N keys' scores (hidden ones -inf), N a multiple of 32, score (mt, i) that of key 16 mt + 4 q4 + i: raises the
   // running max where one exceeds it by more than 2^16 (p stays far inside fp32), and returns the probabilities as two bf16
   // terms, 16 bits of them: one alone gives errors as large as the result's own rounding. The second is taken from
-  // p (1 + 2^-20), so that it is never zero against an infinite V. MODE 0: raw scores; MODE 1: scores in log2 units, with V's
-  // scales at vs, and l takes the unscaled p.
+  // p (1 + 2^-20), so that it is never zero against an infinite V. What is left off is under 2^-15 of p (and the 2^-20, which the
+  // sums take too in MODE 0), 2^-8 is the result's rounding. The decode kernel has as many bits over 16-bit blocks of 16 tokens
+  // and 24 over larger blocks: of 1000 results 3 to 6 are neighbours of its own in either case, and the error against 64 bits is
+  // the same to five digits (1.67e-3 of the norm); over INT8 blocks of 16 tokens, where it takes fp16 weights, 100 of 1000 and a
+  // little less. MODE 0: raw scores; MODE 1: scores in log2 units, with V's scales at vs, and l takes the unscaled p.
   template <int MODE, int N>
   __device__ __forceinline__ void add(const f32x4 (&sc)[N / 16], float scale_log2, float inv_scale_log2, bf16x8 ones,
                                       const f32x4* vs, u32x4 (&hi)[N / 32], u32x4 (&lo)[N / 32]) {

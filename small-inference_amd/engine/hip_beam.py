@@ -148,7 +148,8 @@ def copy_blocks(pools: Sequence[torch.Tensor], copies: Sequence[tuple[int, int, 
     copies, or of one and the source of another.
 
     pools: one to four tensors [L, Hkv, N, B, ...], a cache's K, V and their per-token scales, each head's blocks contiguous.
-    Blocks of up to 255 tokens on the GPU. The copies are the host's: a graph captures the ones it was given. CPU pools are copied by torch operations."""
+    Blocks of up to 255 tokens on the GPU. The copies are the host's: a graph captures the ones it was given. CPU pools are copied
+    by torch operations."""
     P, n = len(pools), len(copies)
     if not 1 <= P <= 4:
         raise ValueError(f"{P} pools (1 to 4)")

@@ -30,9 +30,10 @@ def prefix_supported(q_dtype: torch.dtype, pool_dtype: torch.dtype, block_size: 
 
 
 def shared_groups(tables: list[np.ndarray], context_lens: list[int], block_size: int) -> list[tuple[list[int], int]]:
-    """Groups [(rows, tokens)] of a batch whose rows' tables (int arrays of block ids) begin with the same blocks: rows in
-    no group share nothing. tokens are whole blocks, all of them inside every member's context. Where some members of a group
-    share more than the others, the smaller groups are taken if the batch then reads fewer tokens."""
+    """Groups [(rows, tokens)] of a batch whose rows' tables (int arrays of block ids) begin with the same blocks. tokens are
+    whole blocks, all of them inside every member's context. A row is in one group at most, so of groups within groups one level
+    is taken, that with which the batch reads fewer tokens: what the groups of the other level share is read for every row (64
+    requests of 4 beams, 1024 tokens each, behind a common 4096: one group of 256 rows, 266 thousand keys read of 70 thousand)."""
     full = [min(t.shape[0], c // block_size) for t, c in zip(tables, context_lens)]
 
     def split(rows: list[int], depth: int, level: int = 0) -> tuple[list[tuple[list[int], int]], int]:
