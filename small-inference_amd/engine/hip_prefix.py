@@ -76,9 +76,11 @@ class PrefixPlan:
     batch whose tables agree in their first tokens / B entries, tokens whole blocks; a row is in one group at most. Groups
     change the time, not the result: every row attends the positions below its context length, and one whose context is
     shorter than its group's tokens is read by itself. host_context_lens: the lengths as a list, by which the work is
-    divided; None: they are read from the device once, which waits for it. Calls can be captured, a plan is built before.
+    divided; None: they are read from the device once, which waits for it. Calls can be captured, a plan is built before and has to
+    be kept as long as the graph is replayed.
 
-    The workspace is made for the call that needs it, so plans, streams and graphs share none. Threads may call one plan at
+    The workspace is made for the call that needs it, so plans, streams and graphs share none. Calls may be on any stream of the
+    device (a plan that is dropped keeps its work list until they have read it). Threads may call one plan at
     the same time: each call fills the parameter block and launches under the plan's lock."""
 
     def __init__(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -130,6 +132,7 @@ class PrefixPlan:
         plan = torch.from_numpy(plan).to(self.device)
         p.plan = plan.data_ptr()
         self._keep = (block_tables, context_lens, plan)
+        self._list, self._stream = plan, _hip.stream_of(q)  # the work list, and the stream whose memory it is
         self._ws_bytes = p.layout.workspace_bytes
         self._lock = threading.Lock()
         self._bind(q, k_cache, v_cache, quant)
@@ -211,10 +214,13 @@ class PrefixPlan:
         if self.shape[0] == 0:
             return out
         p.out, p.out_stride_s, p.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+        stream = _hip.stream_of(out)
+        if stream != self._stream:
+            self._list.record_stream(torch.cuda.current_stream(self.device))
         with _hip.on_device(self.device):
             ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
             p.workspace, p.workspace_bytes = ws.data_ptr(), self._ws_bytes
-            rc = self._lib.sipa_prefix_attention(self._ref, _hip.stream_of(out))
+            rc = self._lib.sipa_prefix_attention(self._ref, stream)
         if rc:
             _hip.check(rc, "prefix attention")
         return out
