@@ -42,6 +42,7 @@ class BlockManager:
         self._table_listeners: list[Callable[[int, int], None]] = []
         self._truncate_checks: list[Callable[[int], None]] = []
         self._copy_checks: list[Callable[[list[int], list[int]], None]] = []
+        self._copy_listeners: list[Callable[[list[tuple[int, int, int]]], None]] = []
 
     # ---- queries -------------------------------------------------------------------------------------------------
 
@@ -135,6 +136,10 @@ class BlockManager:
         """Call fn(sources, released) before a fork() or reorder() that asks for copies: a block for each copy's source, and the
         blocks that return to the stack before the copies are made; an exception refuses it."""
         self._copy_checks.append(fn)
+
+    def add_copy_listener(self, fn: Callable[[list[tuple[int, int, int]]], None]) -> None:
+        """Call fn(copies) with the copies that each fork() or reorder() returns, once its sequences exist."""
+        self._copy_listeners.append(fn)
 
     def add_table_listener(self, fn: Callable[[int, int], None]) -> None:
         """Call fn(seq_id, first) when a sequence's table is created (first = 0) or gains blocks from index first
@@ -278,7 +283,10 @@ class BlockManager:
                 for made in new_ids[i::-1]:
                     self.free(made)
                 raise
-        return [(table[full], b, rest) for b in own]
+        copies = [(table[full], b, rest) for b in own]
+        for fn in self._copy_listeners:
+            fn(copies)
+        return copies
 
     def reorder(self, seq_ids: list[int], parents: list[int]) -> list[tuple[int, int, int]]:
         """Sequence seq_ids[i] goes on from what seq_ids[parents[i]] holds (beams after a selection): it gives up its own
@@ -328,6 +336,8 @@ class BlockManager:
                 copies.append((tables[p][-1], own[i], lengths[p] % self.block_size))
                 blocks = [*blocks, own[i]]
             self._set_table(seq_ids[i], blocks, lengths[p])
+        for fn in self._copy_listeners:
+            fn(copies)
         return copies
 
     # ---- checking ------------------------------------------------------------------------------------------------

@@ -95,6 +95,11 @@ class StagingBook:
             raise RuntimeError(f"copies of {need} partial blocks need as many INT8 staging slots, {idle} of {self.n_stage} are "
                                f"idle; construct the cache with a larger n_stage")
 
+    def expect_copies(self, copies) -> None:
+        """Give the destinations of copies of staged blocks their slots, which check_copies has counted, before the copies are
+        made: what is forked next finds them taken."""
+        self.assign([dst for src, dst, _ in copies if src in self.slot_of and dst not in self.slot_of])
+
     def release(self, blocks) -> None:
         """Blocks that left staging (quantized into the pool, or freed by the block manager) return their slots,
         in the order given; blocks without a slot are ignored."""
@@ -186,10 +191,11 @@ class QuantPagedKVCache(PagedKVCache):
             self._stage_of, self._free_stage = self._book.slot_of, self._book.free
             manager.add_free_listener(self._book.release)
             # (the reference's own manager neither truncates nor forks)
-            for name, check in (("add_truncate_check", self._book.check_truncate), ("add_copy_check", self._book.check_copies)):
+            for name, fn in (("add_truncate_check", self._book.check_truncate), ("add_copy_check", self._book.check_copies),
+                             ("add_copy_listener", self._book.expect_copies)):
                 add = getattr(manager, name, None)
                 if add is not None:
-                    add(check)
+                    add(fn)
 
     def _allocate(self, shape: tuple, device: str | torch.device, dtype: torch.dtype) -> None:
         """int8 K/V, fp16 scales, and (format B) the bf16 staging slots; all zero-initialised."""
@@ -376,7 +382,7 @@ class QuantPagedKVCache(PagedKVCache):
             super().copy_blocks(copies)
             return
         check_copies(copies, self.num_blocks, self.block_size)  # before any block is given a slot
-        # (a block without a slot: none of its tokens has been written yet)
+        # (a source without a slot: none of its tokens has been written yet; destinations have theirs from the fork, if there was one)
         staged = [(src, dst, n) for src, dst, n in copies if src in self._stage_of]
         fresh = [dst for _, dst, _ in staged if dst not in self._stage_of]
         self._book.assign(fresh)

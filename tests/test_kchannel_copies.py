@@ -113,3 +113,29 @@ def test_reorders_without_staging_slots_are_refused_before_they_are_made():
         m.free(s)
     assert not cache._stage_of and len(cache._free_stage) == 2
     m.check_invariants()
+
+
+def test_forks_count_the_slots_of_copies_that_are_still_to_be_made():
+    """Copies of several forks made in one call: the second fork finds the slots that the first one's copies will take."""
+    m, cache = filled(n_stage=3)
+    m.allocate(7, 7)
+    write(cache, m, 7, 0, 7)
+    copies = m.fork(0, [1])
+    before = state(m), slots(cache)
+    with pytest.raises(RuntimeError, match="staging slots"):
+        m.fork(7, [8])
+    with pytest.raises(RuntimeError, match="staging slots"):
+        m.fork(1, [8])
+    assert (state(m), slots(cache)) == before
+    copies += m.reorder([0, 7], [0, 0])  # the slot of sequence 7's block goes to its copy
+    cache.copy_blocks(copies)
+    assert set(cache._stage_of) == {1} | {d for _, d, _ in copies}
+    for _, d, n in copies:
+        assert torch.equal(cache.stage[:, :, cache._stage_of[d], :n], cache.stage[:, :, cache._stage_of[1], :n])
+    m.free(1)  # a fork that is given up before its copies are made gives its slot back
+    m.fork(0, [9])
+    m.free(9)
+    for s in (0, 7):
+        m.free(s)
+    assert not cache._stage_of and sorted(cache._free_stage) == [0, 1, 2]
+    m.check_invariants()
